@@ -24,6 +24,8 @@ def build():
 
     sources = [
         os.path.join(REPO, "csrc", "npf_hip", "ext.cpp"),
+        os.path.join(REPO, "csrc", "npf_hip", "ext_norms.cpp"),
+        os.path.join(REPO, "csrc", "npf_hip", "ext_diff_attn.cpp"),
         os.path.join(REPO, "csrc", "npf_hip", "attn.hip"),
         os.path.join(REPO, "csrc", "npf_hip", "attn_mfma.hip"),
         os.path.join(REPO, "csrc", "npf_hip", "setconv.hip"),
@@ -34,13 +36,19 @@ def build():
         os.path.join(REPO, "csrc", "npf_hip", "gauss_kl.hip"),
         os.path.join(REPO, "csrc", "npf_hip", "mlp_chain.hip"),
         os.path.join(REPO, "csrc", "npf_hip", "attender.hip"),
+        os.path.join(REPO, "csrc", "npf_hip", "layernorm.hip"),
+        os.path.join(REPO, "csrc", "npf_hip", "grad_norm.hip"),
+        os.path.join(REPO, "csrc", "npf_hip", "diff_attn.hip"),
     ]
     ext = CUDAExtension(
         name="npf._hip_C",
         sources=sources,
         extra_compile_args={
             "cxx": ["-O3"],
-            "nvcc": ["-O3", "--offload-arch=gfx950"],
+            # packed fp32 instructions stay off: some of their forms have
+            # given wrong results on these machines
+            "nvcc": ["-O3", "--offload-arch=gfx950", "-Xclang",
+                     "-target-feature", "-Xclang", "-packed-fp32-ops"],
         },
     )
 

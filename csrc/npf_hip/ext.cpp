@@ -13,6 +13,8 @@
 
 #include <ATen/hip/HIPContext.h>
 
+#include "bindings.h"
+
 extern "C" {
 void npf_attn_fwd_launch_f32(const void*, const void*, const void*, void*,
                              float*, int, int, int, int, int, float,
@@ -788,5 +790,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "fused MFMA MLP chain forward -> [y, act_0..act_{L-2}]");
   m.def("mlp_chain_bwd", &mlp_chain_bwd,
         "fused MLP chain backward -> [dx, dz_0.., db_0..]");
+  npf_bind_norms(m);
+  npf_bind_diff_attn(m);
   m.attr("_arch") = "gfx950";
 }

@@ -1,0 +1,160 @@
+// Norm of many gradient tensors taken as one vector, and clipping by it.
+//
+//   n = (sum |g|^p)^(1/p), p = 1, 2 or inf;  c = min(1, max_norm / (n + 1e-6))
+//   g *= c
+//
+// One launch leaves a partial sum a block, the next adds all partials in their
+// order (every block for itself: a few thousand values) and scales.  No
+// atomics, so the result does not change between runs.  Sums are held in 64
+// bits: squares of 32-bit values neither overflow nor lose small terms.
+
+#include "common.h"
+#include "grad_norm.h"
+#include "types.h"
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kMostBlocks = 2048;
+
+__device__ __forceinline__ double join(double a, double b, int norm) {
+  if (norm != NPF_NORM_INF) return a + b;
+  return (a > b || a != a) ? a : b;  // NaN stays
+}
+
+__device__ __forceinline__ double value_of(double v, int norm) {
+  return norm == NPF_NORM_2 ? v * v : fabs(v);
+}
+
+__device__ __forceinline__ double block_join(double x, int norm,
+                                             double* smem) {
+  for (int off = NPF_WAVE / 2; off > 0; off >>= 1)
+    x = join(x, __shfl_xor(x, off, NPF_WAVE), norm);
+  if ((threadIdx.x & (NPF_WAVE - 1)) == 0) smem[threadIdx.x / NPF_WAVE] = x;
+  __syncthreads();
+  x = smem[0];
+  for (int w = 1; w < kThreads / NPF_WAVE; ++w) x = join(x, smem[w], norm);
+  return x;
+}
+
+__device__ __forceinline__ double norm_of(const double* partial, int n,
+                                          int norm, double* smem) {
+  double s = 0.;
+  for (int i = threadIdx.x; i < n; i += kThreads)
+    s = join(s, partial[i], norm);
+  s = block_join(s, norm, smem);
+  return norm == NPF_NORM_2 ? sqrt(s) : s;
+}
+
+__device__ __forceinline__ int size_of(int type) {
+  return type == NPF_F64 ? 8 : type == NPF_F32 ? 4 : 2;
+}
+
+// the span that holds a chunk
+__device__ __forceinline__ int span_of(const NpfGradSpans& s, int chunk) {
+  int lo = 0, hi = s.n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if (s.first_chunk[mid] <= chunk) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+template <typename T>
+__device__ __forceinline__ double sum_chunk(const T* p, long n, int norm) {
+  double s = 0.;
+  for (long i = threadIdx.x; i < n; i += kThreads)
+    s = join(s, value_of((double)p[i], norm), norm);
+  return s;
+}
+
+template <typename T>
+__device__ __forceinline__ void scale_chunk(T* p, long n, float c) {
+  for (long i = threadIdx.x; i < n; i += kThreads) p[i] = (T)(p[i] * c);
+}
+
+__global__ void __launch_bounds__(kThreads)
+    grad_partial(NpfGradSpans s, int norm, double* partial) {
+  __shared__ double smem[kThreads / NPF_WAVE];
+  double sum = 0.;
+  for (int c = blockIdx.x; c < s.first_chunk[s.n]; c += gridDim.x) {
+    const int i = span_of(s, c);
+    const long per = kGradChunkBytes / size_of(s.type[i]);
+    const long at = (long)(c - s.first_chunk[i]) * per;
+    const long n = s.count[i] - at < per ? s.count[i] - at : per;
+    double part;
+    switch (s.type[i]) {
+      case NPF_F32: part = sum_chunk((const float*)s.ptr[i] + at, n, norm); break;
+      case NPF_BF16: part = sum_chunk((const npf_bf16*)s.ptr[i] + at, n, norm); break;
+      case NPF_F16: part = sum_chunk((const npf_f16*)s.ptr[i] + at, n, norm); break;
+      default: part = sum_chunk((const double*)s.ptr[i] + at, n, norm);
+    }
+    sum = join(sum, part, norm);
+  }
+  sum = block_join(sum, norm, smem);
+  if (threadIdx.x == 0) partial[blockIdx.x] = sum;
+}
+
+__global__ void __launch_bounds__(kThreads)
+    grad_total(const double* partial, int n, int norm, void* total,
+               int total_type) {
+  __shared__ double smem[kThreads / NPF_WAVE];
+  const double t = norm_of(partial, n, norm, smem);
+  if (threadIdx.x == 0) store_coded(total, total_type, 0, t);
+}
+
+__global__ void __launch_bounds__(kThreads)
+    grad_scale(NpfGradSpans s, const double* partial, int n, int norm,
+               double max_norm, void* total,
+               int total_type) {
+  __shared__ double smem[kThreads / NPF_WAVE];
+  const double t = norm_of(partial, n, norm, smem);
+  if (total && blockIdx.x == 0 && threadIdx.x == 0) store_coded(total, total_type, 0, t);
+  const double ratio = max_norm / (t + 1e-6);
+  // a norm that is no number makes every gradient none
+  const float scale = ratio >= 1. ? 1.f : (float)ratio;
+  if (scale == 1.f) return;  // nothing to change
+  for (int c = blockIdx.x; c < s.first_chunk[s.n]; c += gridDim.x) {
+    const int i = span_of(s, c);
+    const long per = kGradChunkBytes / size_of(s.type[i]);
+    const long at = (long)(c - s.first_chunk[i]) * per;
+    const long m = s.count[i] - at < per ? s.count[i] - at : per;
+    switch (s.type[i]) {
+      case NPF_F32: scale_chunk((float*)s.ptr[i] + at, m, scale); break;
+      case NPF_BF16: scale_chunk((npf_bf16*)s.ptr[i] + at, m, scale); break;
+      case NPF_F16: scale_chunk((npf_f16*)s.ptr[i] + at, m, scale); break;
+      default: {
+        double* p = (double*)s.ptr[i] + at;
+        for (long k = threadIdx.x; k < m; k += kThreads) p[k] *= ratio;
+      }
+    }
+  }
+}
+
+}  // namespace
+
+int npf_grad_blocks(int chunks) {
+  return chunks < kMostBlocks ? chunks : kMostBlocks;
+}
+
+hipError_t npf_grad_partial(const NpfGradSpans& s, int norm, double* partial,
+                            hipStream_t stream) {
+  grad_partial<<<npf_grad_blocks(s.first_chunk[s.n]), kThreads, 0, stream>>>(
+      s, norm, partial);
+  return hipGetLastError();
+}
+
+hipError_t npf_grad_total(const double* partial, int n, int norm, void* total,
+                          int total_type, hipStream_t stream) {
+  grad_total<<<1, kThreads, 0, stream>>>(partial, n, norm, total,
+                                          total_type);
+  return hipGetLastError();
+}
+
+hipError_t npf_grad_scale(const NpfGradSpans& s, const double* partial, int n,
+                          int norm, double max_norm, void* total,
+                          int total_type, hipStream_t stream) {
+  grad_scale<<<npf_grad_blocks(s.first_chunk[s.n]), kThreads, 0, stream>>>(
+      s, partial, n, norm, max_norm, total, total_type);
+  return hipGetLastError();
+}

@@ -33,7 +33,8 @@ def get_attender(attention, kq_size, value_size, out_size, **kwargs):
     """Build an attender by name or callable (reference attention.py:16-86).
 
     Supported names: multiplicative, additive, scaledot, cosine, manhattan,
-    euclidean, weighted_dist, multihead, transformer.
+    euclidean, weighted_dist, multihead, transformer, differential,
+    differential_transformer.
     """
     if not isinstance(attention, str):
         return attention(kq_size, value_size, out_size, **kwargs)
@@ -420,3 +421,145 @@ class TransformerAttender(MultiheadAttender):
             # caller's dtype (under autocast bf16 flows on unchanged)
             out = out.to(queries.dtype)
         return out
+
+
+@_register("differential")
+class DifferentialAttender(nn.Module):
+    """Multi-head differential attention: each head's map is the difference of
+    two softmax maps, ``softmax(q1 k1^T) - lam softmax(q2 k2^T)``, so that what
+    both maps give to every context point cancels.
+
+    The weight is learned, ``lam = exp(lq1 . lk1) - exp(lq2 . lk2) + lam_init``
+    with ``lam_init = 0.8 - 0.6 exp(-0.3 (depth - 1))``, and every head's result
+    is normed by itself and scaled by ``1 - lam_init``, which leaves gradients
+    the size that one map would give them.
+
+    Parameters
+    ----------
+    n_heads : int
+        Query heads; each holds two maps of ``kq_size / (2 n_heads)`` values.
+    n_kv_heads : int, optional
+        Key and value heads, shared by ``n_heads / n_kv_heads`` query heads
+        each; `n_heads` by default.
+    depth : int
+        The layer's place in a stack, from 1; sets ``lam_init``.
+    is_post_process : bool
+        Linear map of the joined heads; needed where sizes differ.
+    """
+
+    def __init__(
+        self,
+        kq_size,
+        value_size,
+        out_size,
+        n_heads=4,
+        n_kv_heads=None,
+        depth=1,
+        is_post_process=True,
+    ):
+        super().__init__()
+        n_kv_heads = n_heads if n_kv_heads is None else n_kv_heads
+        if kq_size % (2 * n_heads):
+            raise ValueError(f"kq_size {kq_size} is no multiple of {2 * n_heads}")
+        if value_size % n_heads:
+            raise ValueError(f"value_size {value_size} is no multiple of {n_heads}")
+        if n_kv_heads < 1 or n_heads % n_kv_heads:
+            raise ValueError(f"{n_heads} heads cannot share {n_kv_heads} key heads")
+        if depth < 1:
+            raise ValueError(f"depth starts at 1, got {depth}")
+        self.kq_size = kq_size
+        self.value_size = value_size
+        self.out_size = out_size
+        self.n_heads = n_heads
+        self.n_kv_heads = n_kv_heads
+        self.kq_head_size = kq_size // n_heads  # both maps
+        self.value_head_size = value_size // n_heads
+        self.lam_init = 0.8 - 0.6 * math.exp(-0.3 * (depth - 1))
+        self.key_transform = nn.Linear(
+            kq_size, n_kv_heads * self.kq_head_size, bias=False
+        )
+        self.query_transform = nn.Linear(kq_size, kq_size)
+        self.value_transform = nn.Linear(
+            value_size, n_kv_heads * self.value_head_size, bias=False
+        )
+        map_size = self.kq_head_size // 2
+        self.lam_vectors = nn.Parameter(torch.empty(4, map_size))
+        self.head_norm = nn.LayerNorm(self.value_head_size)
+        self.post_processor = (
+            nn.Linear(value_size, out_size)
+            if is_post_process or value_size != out_size
+            else None
+        )
+        self.reset_parameters()
+
+    def reset_parameters(self):
+        weights_init(self)
+        nn.init.normal_(self.lam_vectors, std=0.1)
+
+    def lam(self):
+        """The weight of the second map, a 0-d fp32 tensor."""
+        with torch.autocast(self.lam_vectors.device.type, enabled=False):
+            lq1, lk1, lq2, lk2 = self.lam_vectors.float()
+            return (lq1 * lk1).sum().exp() - (lq2 * lk2).sum().exp() + self.lam_init
+
+    def forward(self, keys, queries, values, key_lengths=None):
+        """keys [B,K,kq], queries [B,Q,kq], values [B,K,v] -> [B,Q,out].
+
+        key_lengths: int [B], the valid contexts of each task; 0 is allowed.
+        """
+        B, Q, _ = queries.shape
+        k = self._heads(self.key_transform(keys), self.n_kv_heads)
+        q = self._heads(self.query_transform(queries), self.n_heads)
+        v = self._heads(self.value_transform(values), self.n_kv_heads)
+        context = ops.differential_attention(
+            k, q, v, self.lam(), key_lengths=key_lengths
+        )
+        # [B, Q, H, Dv]: heads are joined by a view
+        context = ops.layer_norm(
+            context.transpose(1, 2),
+            self.head_norm.weight,
+            self.head_norm.bias,
+            eps=self.head_norm.eps,
+        ) * (1.0 - self.lam_init)
+        context = context.reshape(B, Q, self.value_size)
+        if self.post_processor is not None:
+            context = self.post_processor(context)
+        return context
+
+    @staticmethod
+    def _heads(x, n_heads):
+        """[B, N, H*h] -> [B, H, N, h], a view."""
+        return x.view(*x.shape[:2], n_heads, -1).transpose(1, 2)
+
+
+@_register("differential_transformer")
+class DifferentialTransformerAttender(DifferentialAttender):
+    """Differential attention with the transformer attender's block around it:
+    residual and norm, then an MLP with residual and norm."""
+
+    def __init__(self, *args, **kwargs):
+        super().__init__(*args, is_post_process=False, **kwargs)
+        if self.kq_size != self.out_size:
+            raise ValueError(
+                f"queries have size {self.kq_size}, the residual {self.out_size}"
+            )
+        self.layer_norm1 = nn.LayerNorm(self.out_size)
+        self.layer_norm2 = nn.LayerNorm(self.out_size)
+        self.mlp = MLP(
+            self.out_size, self.out_size, hidden_size=self.out_size, activation=nn.ReLU()
+        )
+        self.reset_parameters()
+
+    def forward(self, keys, queries, values, key_lengths=None):
+        context = super().forward(keys, queries, values, key_lengths=key_lengths)
+        context = self._add_norm(self.layer_norm1, context, queries)
+        return self._add_norm(self.layer_norm2, self.mlp(context), context)
+
+    @staticmethod
+    def _add_norm(norm, x, residual):
+        # under autocast the products are 16 bit and the residual may not be
+        dtype = torch.promote_types(x.dtype, residual.dtype)
+        return ops.layer_norm(
+            x.to(dtype), norm.weight, norm.bias, eps=norm.eps,
+            residual=residual.to(dtype),
+        )

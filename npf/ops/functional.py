@@ -9,10 +9,11 @@ SURVEY.md §2.3; reference call-sites cited per op.
 import math
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _backend
 
-__all__ = ["attention_qkv", "setconv_gaussian", "gaussian_nll_sum", "gaussian_nll_logmeanexp", "conv_block_1d", "conv_block_2d", "grid_density", "gaussian_kl_sum", "mlp_chain"]
+__all__ = ["attention_qkv", "setconv_gaussian", "gaussian_nll_sum", "gaussian_nll_logmeanexp", "conv_block_1d", "conv_block_2d", "grid_density", "gaussian_kl_sum", "mlp_chain", "layer_norm", "differential_attention", "grad_norm", "clip_grad_norm_"]
 
 
 # --------------------------------------------------------------------------- #
@@ -825,3 +826,316 @@ def mlp_chain(x, weights, biases):
     xb = x.reshape(-1, x.shape[-1]).to(torch.bfloat16).contiguous()
     y = _MLPChainFn.apply(xb, len(weights), *weights, *biases)
     return y.reshape(*lead, y.shape[-1])
+
+
+# --------------------------------------------------------------------------- #
+# Layer norm over the last axis (csrc/npf_hip/layernorm.hip).
+# --------------------------------------------------------------------------- #
+
+
+def _widened(t):
+    """16-bit floats as fp32; the composed paths round once, like the kernels."""
+    return t.float() if t.dtype in (torch.bfloat16, torch.float16) else t
+
+
+def _layer_norm_ref(x, weight, bias, eps, residual):
+    z = _widened(x) if residual is None else _widened(x) + _widened(residual)
+    c = z - z.mean(-1, keepdim=True)
+    y = c * torch.rsqrt((c * c).mean(-1, keepdim=True) + eps)
+    if weight is not None:
+        y = y * weight
+    if bias is not None:
+        y = y + bias
+    return y.to(x.dtype)
+
+
+def _as_rows(t):
+    """[..., D] as [rows, D] with contiguous rows, copied only where no
+    stride describes them."""
+    rows = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
+    return rows if rows.stride(1) == 1 or rows.shape[1] == 1 else rows.contiguous()
+
+
+class _LayerNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, weight, bias, eps):
+        ext = _backend.extension()
+        xr = _as_rows(x)
+        rr = None if residual is None else _as_rows(residual)
+        y, mean, rstd = ext.layer_norm_fwd(xr, rr, weight, bias, eps, True)
+        ctx.save_for_backward(xr, rr, weight, bias, mean, rstd)
+        return y.view(x.shape)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        ext = _backend.extension()
+        xr, rr, weight, bias, mean, rstd = ctx.saved_tensors
+        need_x, need_r, need_w, need_b = ctx.needs_input_grad[:4]
+        dx, dw, db = ext.layer_norm_bwd(
+            dy.reshape(xr.shape).contiguous(), xr, rr, weight, bias, mean, rstd,
+            need_x or need_r, need_w, need_b,
+        )
+        if dx is not None:
+            dx = dx.view(dy.shape)
+        return dx if need_x else None, dx if need_r else None, dw, db, None
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5, residual=None):
+    """Layer norm of `x` (or of ``x + residual``) over the last axis.
+
+    x, residual: [..., D] of one shape and type (fp32, bf16 or fp16), any
+    D >= 1, any strides; weight, bias: [D] or None, of one floating type that
+    need not be x's.  Returns x's shape and type.
+
+    Statistics are fp32 and the sum of x and residual is not rounded; the
+    result is rounded once.  Differentiable once in all four tensors; sums of
+    the weight's gradient run in a fixed order.  Under autocast the inputs'
+    own types count.
+    """
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"layer_norm needs a last axis, got {tuple(x.shape)}")
+    D = x.shape[-1]
+    if not x.is_floating_point():
+        raise TypeError(f"layer_norm takes floating tensors, got {x.dtype}")
+    if residual is not None:
+        if residual.shape != x.shape:
+            raise ValueError(
+                f"residual has shape {tuple(residual.shape)}, x {tuple(x.shape)}"
+            )
+        if residual.dtype != x.dtype:
+            raise TypeError(f"residual is {residual.dtype}, x is {x.dtype}")
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is not None and tuple(t.shape) != (D,):
+            raise ValueError(f"{name} has shape {tuple(t.shape)}, needs ({D},)")
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise TypeError(f"weight is {weight.dtype}, bias is {bias.dtype}")
+    if not x.is_cuda:
+        return _layer_norm_ref(x, weight, bias, eps, residual)
+    ext = _backend.require_extension("layer_norm")
+    if ext is None:
+        return _layer_norm_ref(x, weight, bias, eps, residual)
+    if weight is not None:
+        weight = weight.contiguous()
+    if bias is not None:
+        bias = bias.contiguous()
+    if torch.is_grad_enabled() and any(
+        t is not None and t.requires_grad for t in (x, residual, weight, bias)
+    ):
+        return _LayerNormFn.apply(x, residual, weight, bias, eps)
+    xr = _as_rows(x)
+    rr = None if residual is None else _as_rows(residual)
+    return ext.layer_norm_fwd(xr, rr, weight, bias, eps, False)[0].view(x.shape)
+
+
+# --------------------------------------------------------------------------- #
+# Differential attention (csrc/npf_hip/diff_attn.hip): the difference of two
+# softmax maps over the same values, the second one weighted by lam.
+# --------------------------------------------------------------------------- #
+
+
+def _differential_attention_ref(keys, queries, values, lam, scale, key_lengths):
+    dtype = queries.dtype
+    keys, queries, values = _widened(keys), _widened(queries), _widened(values)
+    H, K, Hk = queries.shape[1], keys.shape[2], keys.shape[1]
+    D = queries.shape[-1] // 2
+    if key_lengths is not None:
+        at = torch.arange(K, device=keys.device)
+        live = (at < key_lengths.to(at.device)[:, None])[:, None, :, None]
+        # whatever a masked place holds stays out of every product
+        keys = keys.masked_fill(~live, 0)
+        values = values.masked_fill(~live, 0)
+    if Hk != H:
+        keys = keys.repeat_interleave(H // Hk, 1)
+        values = values.repeat_interleave(H // Hk, 1)
+    maps = []
+    for part in (slice(0, D), slice(D, 2 * D)):
+        q, k = queries[..., part], keys[..., part]
+        logits = torch.matmul(q, k.transpose(-1, -2).contiguous()) * scale
+        if key_lengths is None:
+            maps.append(logits.softmax(-1))
+        else:
+            row = live.transpose(-1, -2)
+            low = torch.finfo(logits.dtype).min
+            maps.append(logits.masked_fill(~row, low).softmax(-1) * row)
+    lam = lam.to(maps[0].dtype).reshape(-1, 1, 1)
+    return torch.matmul(maps[0] - lam * maps[1], values.contiguous()).to(dtype)
+
+
+def _as_heads(t):
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+class _DifferentialAttentionFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, keys, queries, values, lam, scale, key_lengths):
+        ext = _backend.extension()
+        out, o2, lse = ext.diff_attn_fwd(
+            queries, keys, values, lam, scale, key_lengths, True
+        )
+        ctx.save_for_backward(keys, queries, values, lam, out, o2, lse, key_lengths)
+        ctx.scale = scale
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        ext = _backend.extension()
+        keys, queries, values, lam, out, o2, lse, key_lengths = ctx.saved_tensors
+        need_k, need_q, need_v, need_lam = ctx.needs_input_grad[:4]
+        dq, dk, dv, dlam = ext.diff_attn_bwd(
+            _as_heads(dout), queries, keys, values, lam, out, o2, lse, ctx.scale,
+            key_lengths, need_q, need_k, need_v, need_lam,
+        )
+        return dk, dq, dv, dlam, None, None
+
+
+def differential_attention(keys, queries, values, lam, scale=None, key_lengths=None):
+    """(softmax(scale q1 k1^T) - lam softmax(scale q2 k2^T)) V, over the keys.
+
+    keys [B, Hk, K, 2D] and queries [B, H, Q, 2D] hold both maps' vectors, the
+    first map's in the first half; values [B, Hk, K, Dv]; result
+    [B, H, Q, Dv].  Query head h reads key head h // (H // Hk), so Hk < H
+    shares keys between heads.  All three of one type (fp32, bf16, fp16), any
+    strides with a contiguous last axis (others are copied), D <= 128,
+    Dv <= 2 * max(D, 16) rounded up to the next of 32, 64, 128, 256.
+
+    lam: 0-d, or [H] for one weight a head, any floating type.
+    scale: positive; 1 / sqrt(D) by default.
+    key_lengths: int [B] on the same device; batch entry b attends to its
+    first key_lengths[b] keys (values outside 0..K count as the nearest of the
+    two) and later keys are not read.  Rows without keys give zeros, and take
+    no part in any gradient.
+
+    Scores, statistics and sums are fp32; the maps' values are rounded to the
+    inputs' type for the products with V.  Differentiable once in keys,
+    queries, values and lam, with sums in a fixed order.
+    """
+    if keys.dim() != 4 or queries.dim() != 4 or values.dim() != 4:
+        raise ValueError("keys, queries and values must be [batch, heads, length, size]")
+    B, H, Q, D2 = queries.shape
+    Hk, K = keys.shape[1], keys.shape[2]
+    if D2 < 2 or D2 % 2 or keys.shape[-1] != D2:
+        raise ValueError(
+            "queries and keys must hold two maps of one size, got "
+            f"{D2} and {keys.shape[-1]} values"
+        )
+    if keys.shape[0] != B or values.shape[:3] != keys.shape[:3]:
+        raise ValueError(
+            f"batch, heads or lengths differ: queries {tuple(queries.shape)}, "
+            f"keys {tuple(keys.shape)}, values {tuple(values.shape)}"
+        )
+    if Hk < 1 or H % Hk:
+        raise ValueError(f"{H} query heads cannot share {Hk} key heads")
+    if not queries.dtype == keys.dtype == values.dtype:
+        raise TypeError(
+            f"keys {keys.dtype}, queries {queries.dtype} and values "
+            f"{values.dtype} must have one type"
+        )
+    if not torch.is_tensor(lam) or lam.dim() > 1 or (lam.dim() and len(lam) != H):
+        raise ValueError("lam must be a tensor of one value, or of one a query head")
+    if not lam.is_floating_point():
+        raise TypeError(f"lam must be floating, got {lam.dtype}")
+    if scale is None:
+        scale = 1.0 / math.sqrt(D2 // 2)
+    if not 0.0 < scale < math.inf:
+        raise ValueError(f"scale must be positive, got {scale}")
+    if key_lengths is not None:
+        if tuple(key_lengths.shape) != (B,):
+            raise ValueError(f"key_lengths has shape {tuple(key_lengths.shape)}, needs ({B},)")
+        if key_lengths.dtype not in (torch.int32, torch.int64):
+            raise TypeError(f"key_lengths must be int32 or int64, got {key_lengths.dtype}")
+    ext = _backend.require_extension("differential_attention") if queries.is_cuda else None
+    if ext is None:
+        return _differential_attention_ref(
+            keys, queries, values, lam, scale, key_lengths
+        )
+    keys, queries, values = _as_heads(keys), _as_heads(queries), _as_heads(values)
+    if key_lengths is not None:
+        key_lengths = key_lengths.contiguous()
+    if torch.is_grad_enabled() and (
+        keys.requires_grad or queries.requires_grad
+        or values.requires_grad or lam.requires_grad
+    ):
+        return _DifferentialAttentionFn.apply(
+            keys, queries, values, lam, scale, key_lengths
+        )
+    return ext.diff_attn_fwd(
+        queries, keys, values, lam, scale, key_lengths, False
+    )[0]
+
+
+# --------------------------------------------------------------------------- #
+# Norm of all gradients and clipping by it (csrc/npf_hip/grad_norm.hip).
+# --------------------------------------------------------------------------- #
+
+
+def _gradients(parameters, norm_type):
+    if norm_type not in (1, 2, math.inf):
+        raise ValueError(f"norm_type must be 1, 2 or inf, got {norm_type}")
+    if torch.is_tensor(parameters):
+        parameters = [parameters]
+    grads = [p.grad for p in parameters if p.grad is not None]
+    for g in grads:
+        if g.layout != torch.strided or not g.is_floating_point():
+            raise TypeError("gradients must be dense floating tensors")
+    return grads
+
+
+def _grad_norm_ref(grads, norm_type):
+    norms = [torch.linalg.vector_norm(g, norm_type) for g in grads if g.numel()]
+    if not norms:
+        return torch.zeros((), device=grads[0].device if grads else None)
+    return torch.linalg.vector_norm(torch.stack(norms), norm_type)
+
+
+def grad_norm(parameters, norm_type=2.0):
+    """Norm of the gradients of `parameters` taken as one vector.
+
+    parameters: a tensor or an iterable of tensors; those without a gradient
+    are left out.  norm_type: 1, 2 or inf.  Returns a 0-d tensor on the
+    gradients' device (fp32 on a GPU, fp64 where a gradient is); no host wait.
+    """
+    grads = _gradients(parameters, norm_type)
+    if not grads or not grads[0].is_cuda:
+        return _grad_norm_ref(grads, norm_type)
+    ext = _backend.require_extension("grad_norm")
+    if ext is None:
+        return _grad_norm_ref(grads, norm_type)
+    return ext.grad_norm(grads, norm_type, -1.0)
+
+
+def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
+    """Scale the gradients of `parameters` in place so that their norm, taken
+    as one vector, is at most `max_norm`; returns the norm before.
+
+    Two kernel launches for up to 160 gradients that do not follow each other
+    in memory (gradients that do count as one), no host wait, and capturable
+    into a graph.  The factor is min(1, max_norm / (norm + 1e-6)); a norm that
+    is inf gives zeros (and NaN where a gradient is inf), NaN gives NaN, unless
+    `error_if_nonfinite`, which waits for the norm and raises RuntimeError
+    before any gradient changes.  Gradients must not share memory.
+    """
+    max_norm = float(max_norm)
+    if not max_norm >= 0.0:
+        raise ValueError(f"max_norm must not be negative, got {max_norm}")
+    grads = _gradients(parameters, norm_type)
+    ext = None
+    if grads and grads[0].is_cuda:
+        ext = _backend.require_extension("grad_norm")
+    if error_if_nonfinite or ext is None:
+        total = (
+            _grad_norm_ref(grads, norm_type) if ext is None
+            else ext.grad_norm(grads, norm_type, -1.0)
+        )
+        if error_if_nonfinite and not bool(torch.isfinite(total)):
+            raise RuntimeError(
+                f"the norm of order {norm_type} of the gradients is {float(total)}, "
+                "so they cannot be clipped"
+            )
+        if ext is None:
+            c = torch.clamp(max_norm / (total + 1e-6), max=1.0)
+            for g in grads:
+                g.mul_(c.to(g.device))
+            return total
+    return ext.grad_norm(grads, norm_type, max_norm)

@@ -21,6 +21,7 @@ import torch
 from torch.optim import Adam
 from torch.utils.data import DataLoader, Subset
 
+from npf import ops
 from npf.parallel import ddp as dist_utils
 from npf.train.helpers import get_exponential_decay_gamma, set_seed
 
@@ -285,9 +286,7 @@ class NPFTrainer:
         if self.ddp is not None:
             self.ddp.reduce_()
         if self.grad_clip_norm is not None:
-            torch.nn.utils.clip_grad_norm_(
-                self.module.parameters(), self.grad_clip_norm
-            )
+            ops.clip_grad_norm_(self.module.parameters(), self.grad_clip_norm)
         self.optimizer.step()
         return loss.detach()
 
