@@ -39,6 +39,9 @@ def build():
         os.path.join(REPO, "csrc", "npf_hip", "layernorm.hip"),
         os.path.join(REPO, "csrc", "npf_hip", "grad_norm.hip"),
         os.path.join(REPO, "csrc", "npf_hip", "diff_attn.hip"),
+        os.path.join(REPO, "csrc", "npf_hip", "diff_attn_f32.hip"),
+        os.path.join(REPO, "csrc", "npf_hip", "diff_attn_bf16.hip"),
+        os.path.join(REPO, "csrc", "npf_hip", "diff_attn_f16.hip"),
     ]
     ext = CUDAExtension(
         name="npf._hip_C",

@@ -1,4 +1,4 @@
-// Arguments of the differential attention kernels (diff_attn.hip).
+// Arguments of the differential attention kernels (diff_attn*.hip).
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -14,22 +14,26 @@ struct NpfDiffAttnArgs {
   NpfHeads dout;          // backward
   NpfHeads dq, dk, dv;    // backward; null where not asked for
   float* lse;             // [B, H, Q, 2]: log2 of each map's sum of exponents
-  float* delta;           // backward: [B, H, Q, 2]: dout . (each map's part)
-  double* dlam_partial;   // backward: [B, H, parts]
+  float* stats;           // backward: [B, H, Q, 4]: lse_1, lse_2, delta_1, _2
+  float* dlam_rows;       // backward: [B, H, Q]
   void* dlam;             // backward: [lam_heads], or null
   const void* lam;
   const void* lengths;    // [B] int32 or int64, or null
-  void* split;            // forward over a split key axis: its workspace
+  void* split;            // forward: workspace of a split key axis
   float scale;
   int B, H, Hk, Q, K, D, Dv;
   int type, lam_type, lam_stride;
   int lam_heads;          // values of lam: H or 1
   int lengths64;
-  int parts;
-  int splits;
+  // the plan
+  int pad;     // D and Dv / 2 are padded to this
+  int waves;   // of a forward block
+  int splits;  // parts of the key axis
 };
 
-// rows of dlam_partial for each head of a batch entry
-int npf_diff_attn_parts(int Q);
+// fills the plan; false where no kernel covers the sizes
+bool npf_diff_attn_plan(NpfDiffAttnArgs&);
+// bytes of `split`
+size_t npf_diff_attn_workspace(const NpfDiffAttnArgs&);
 hipError_t npf_diff_attn_fwd(const NpfDiffAttnArgs&, hipStream_t);
 hipError_t npf_diff_attn_bwd(const NpfDiffAttnArgs&, hipStream_t);

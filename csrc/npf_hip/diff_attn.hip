@@ -1,292 +1,211 @@
-// Differential attention: the difference of two softmax maps.
-//
-//   S_i = scale q_i k_i^T;  P_i = softmax(S_i);  O = (P_1 - lam P_2) V
-//   G = dO V^T;  delta_i = rowsum(dO * (P_i V))
-//   dS_1 = P_1 (G - delta_1);  dS_2 = -lam P_2 (G - delta_2)
-//   dq_i = scale dS_i k_i;  dk_i = scale dS_i^T q_i
-//   dV = (P_1 - lam P_2)^T dO;  dlam = -sum delta_2
-//
-// Statistics are kept in units of log2: P_i = exp2(S_i log2(e) - lse_i).
+// Differential attention: the plan, the join of a split key axis, and the
+// backward pass's row sums.  The products are in diff_attn_impl.h.
 
-#include "common.h"
-#include "diff_attn.h"
-#include "types.h"
+#include "diff_attn_impl.h"
+
+hipError_t npf_diff_attn_fwd_f32(const NpfDiffAttnArgs&, hipStream_t);
+hipError_t npf_diff_attn_fwd_bf16(const NpfDiffAttnArgs&, hipStream_t);
+hipError_t npf_diff_attn_fwd_f16(const NpfDiffAttnArgs&, hipStream_t);
+hipError_t npf_diff_attn_bwd_f32(const NpfDiffAttnArgs&, hipStream_t);
+hipError_t npf_diff_attn_bwd_bf16(const NpfDiffAttnArgs&, hipStream_t);
+hipError_t npf_diff_attn_bwd_f16(const NpfDiffAttnArgs&, hipStream_t);
 
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLowest = -3.0e38f;
+using namespace npf_attn;
+
+// one block a row: 4 slices of the splits, each over both maps' values
+constexpr int kJoinThreads = 1024;
 
 template <typename T>
-__device__ __forceinline__ T* row_of(const NpfHeads& t, int b, int h, long l) {
-  return static_cast<T*>(t.p) + b * t.b + h * t.h + l * t.l;
-}
-
-__device__ __forceinline__ int keys_of(const NpfDiffAttnArgs& a, int b) {
-  if (!a.lengths) return a.K;
-  const long n = a.lengths64 ? static_cast<const long*>(a.lengths)[b]
-                             : static_cast<const int*>(a.lengths)[b];
-  return n < 0 ? 0 : n > a.K ? a.K : (int)n;
-}
-
-__device__ __forceinline__ float lam_of(const NpfDiffAttnArgs& a, int h) {
-  return load_coded(a.lam, a.lam_type, (long)h * a.lam_stride);
-}
-
-// one wave a query row
-template <typename T>
-__global__ void __launch_bounds__(64) fwd_row(NpfDiffAttnArgs a) {
-  __shared__ float sq[256];
-  __shared__ float sp[2][64];
-  const int lane = threadIdx.x, h = blockIdx.y, b = blockIdx.z;
-  const int hk = h / (a.H / a.Hk);
-  const int n = keys_of(a, b);
-  const float s2 = a.scale * kLog2e;
-  for (long r = blockIdx.x; r < a.Q; r += gridDim.x) {
-    __syncthreads();
-    for (int d = lane; d < 2 * a.D; d += 64)
-      sq[d] = (float)row_of<T>(a.q, b, h, r)[d];
-    float m[2] = {kLowest, kLowest}, l[2] = {0.f, 0.f};
-    float o[2][4] = {};
-    for (int k0 = 0; k0 < n; k0 += 64) {
-      __syncthreads();
-      const int kn = n - k0 < 64 ? n - k0 : 64;
-      for (int i = 0; i < 2; ++i) {
-        float s = kLowest;
-        if (lane < kn) {
-          const T* kp = row_of<T>(a.k, b, hk, k0 + lane) + i * a.D;
-          s = 0.f;
-          for (int d = 0; d < a.D; ++d) s += sq[i * a.D + d] * (float)kp[d];
-          s *= s2;
-        }
-        const float mn = fmaxf(m[i], wave_allreduce_max(s));
-        const float p = lane < kn ? exp2f(s - mn) : 0.f;
-        const float c = exp2f(m[i] - mn);
-        l[i] = l[i] * c + wave_allreduce_sum(p);
-        m[i] = mn;
-        sp[i][lane] = p;
-        for (int j = 0; j < 4; ++j) o[i][j] *= c;
-      }
-      __syncthreads();
-      for (int k = 0; k < kn; ++k) {
-        const T* vp = row_of<T>(a.v, b, hk, k0 + k);
-        for (int j = 0; j < 4; ++j)
-          if (lane + 64 * j < a.Dv) {
-            const float v = (float)vp[lane + 64 * j];
-            o[0][j] += sp[0][k] * v;
-            o[1][j] += sp[1][k] * v;
-          }
-      }
+__global__ void __launch_bounds__(kJoinThreads) join(NpfDiffAttnArgs a) {
+  __shared__ float part[4][2][256];
+  __shared__ float weight_sum[2];
+  const int group = a.H / a.Hk, rows = group * a.Q;
+  const int row = blockIdx.x % rows, bh = blockIdx.x / rows;
+  const int b = bh / a.Hk, hk = bh % a.Hk;
+  const int h = hk * group + row / a.Q, q = row % a.Q;
+  const long step = split_row_floats(a.Dv);
+  const float* w = static_cast<const float*>(a.split) +
+                   (long)blockIdx.x * a.splits * step;
+  const int slice = threadIdx.x >> 8, t = threadIdx.x & 255;
+  float top[2] = {kLowest, kLowest};
+  for (int s = threadIdx.x & 63; s < a.splits; s += 64)
+    for (int m = 0; m < 2; ++m) top[m] = fmaxf(top[m], w[s * step + 2 * m]);
+  for (int m = 0; m < 2; ++m) top[m] = wave_allreduce_max(top[m]);
+  if (threadIdx.x < 64) {
+    for (int m = 0; m < 2; ++m) {
+      float l = 0.f;
+      for (int s = threadIdx.x; s < a.splits; s += 64)
+        l += exp2f(w[s * step + 2 * m] - top[m]) * w[s * step + 2 * m + 1];
+      l = wave_allreduce_sum(l);
+      if (threadIdx.x == 0) weight_sum[m] = l;
     }
-    const float lam = lam_of(a, h);
-    for (int j = 0; j < 4; ++j)
-      if (lane + 64 * j < a.Dv) {
-        const float o1 = n ? o[0][j] / l[0] : 0.f;
-        const float o2 = n ? o[1][j] / l[1] : 0.f;
-        row_of<T>(a.out, b, h, r)[lane + 64 * j] = (T)(o1 - lam * o2);
-        if (a.o2.p) row_of<T>(a.o2, b, h, r)[lane + 64 * j] = (T)o2;
-      }
-    if (a.lse && lane < 2)
-      a.lse[(((long)b * a.H + h) * a.Q + r) * 2 + lane] =
-          n ? m[lane] + log2f(l[lane]) : 0.f;
   }
-}
-
-// delta_i of a row a wave, and this block's part of dlam
-template <typename T>
-__global__ void __launch_bounds__(256) bwd_delta(NpfDiffAttnArgs a) {
-  __shared__ double part[4];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int h = blockIdx.y, b = blockIdx.z;
-  const float lam = lam_of(a, h);
-  double sum = 0.;
-  for (int i = 0; i < 16; ++i) {
-    const long r = (long)blockIdx.x * 64 + w * 16 + i;
-    if (r >= a.Q) break;
-    float d1 = 0.f, d2 = 0.f;
-    for (int c = lane; c < a.Dv; c += 64) {
-      const float g = (float)row_of<T>(a.dout, b, h, r)[c];
-      const float o2 = (float)row_of<T>(a.o2, b, h, r)[c];
-      d1 += g * ((float)row_of<T>(a.out, b, h, r)[c] + lam * o2);
-      d2 += g * o2;
-    }
-    d1 = wave_allreduce_sum(d1);
-    d2 = wave_allreduce_sum(d2);
-    if (lane == 0) {
-      float* p = a.delta + (((long)b * a.H + h) * a.Q + r) * 2;
-      p[0] = d1;
-      p[1] = d2;
-    }
-    sum += d2;
+  float o[2] = {0.f, 0.f};
+  if (t < a.Dv) {
+#pragma unroll 4
+    for (int s = slice; s < a.splits; s += 4)
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+        o[m] += exp2f(w[s * step + 2 * m] - top[m]) *
+                w[s * step + 4 + m * a.Dv + t];
   }
-  if (lane == 0) part[w] = sum;
+  part[slice][0][t] = o[0];
+  part[slice][1][t] = o[1];
   __syncthreads();
-  if (threadIdx.x == 0)
-    a.dlam_partial[((long)b * a.H + h) * a.parts + blockIdx.x] =
-        part[0] + part[1] + part[2] + part[3];
+  if (slice > 0) return;
+  const bool any = keys_of(a, b) > 0;
+  if (t < a.Dv) {
+    for (int m = 0; m < 2; ++m) {
+      o[m] = part[0][m][t] + part[1][m][t] + part[2][m][t] + part[3][m][t];
+      o[m] = any ? o[m] / weight_sum[m] : 0.f;
+    }
+    row_of<T>(a.out, b, h, q)[t] = (T)(o[0] - lam_of(a, h) * o[1]);
+    if (a.o2.p) row_of<T>(a.o2, b, h, q)[t] = (T)o[1];
+  }
+  if (a.lse && t < 2)
+    a.lse[(((long)b * a.H + h) * a.Q + q) * 2 + t] =
+        any ? top[t] + __log2f(weight_sum[t]) : 0.f;
+}
+
+// delta_i of each row, beside its lse: kLanes lanes of 4 values a row
+template <typename T, int kLanes>
+__global__ void __launch_bounds__(256) row_stats(NpfDiffAttnArgs a) {
+  const long rows = (long)a.B * a.H * a.Q;
+  const long r = (long)blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
+  if (r >= rows) return;  // whole groups of lanes
+  const int q = (int)(r % a.Q);
+  const int h = (int)(r / a.Q % a.H), b = (int)(r / a.Q / a.H);
+  const int c = (threadIdx.x % kLanes) * 4;
+  const float lam = lam_of(a, h);
+  float d1 = 0.f, d2 = 0.f;
+  if (c < a.Dv) {
+    const T* gp = row_of<T>(a.dout, b, h, q) + c;
+    const T* op = row_of<T>(a.out, b, h, q) + c;
+    const T* sp = row_of<T>(a.o2, b, h, q) + c;
+    T g[4] = {}, o[4] = {}, s[4] = {};
+    if (c + 4 <= a.Dv) {
+      load_pack(g, gp);
+      load_pack(o, op);
+      load_pack(s, sp);
+    } else {
+      for (int i = 0; c + i < a.Dv; ++i) {
+        g[i] = gp[i];
+        o[i] = op[i];
+        s[i] = sp[i];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      d1 += (float)g[i] * ((float)o[i] + lam * (float)s[i]);
+      d2 += (float)g[i] * (float)s[i];
+    }
+  }
+#pragma unroll
+  for (int off = kLanes / 2; off > 0; off >>= 1) {
+    d1 += __shfl_xor(d1, off, 64);
+    d2 += __shfl_xor(d2, off, 64);
+  }
+  if (threadIdx.x % kLanes == 0)
+    reinterpret_cast<float4*>(a.stats)[r] =
+        float4{a.lse[2 * r], a.lse[2 * r + 1], d1, d2};
 }
 
 // dlam of one head (of all heads where lam is one number)
-__global__ void __launch_bounds__(256) bwd_dlam(NpfDiffAttnArgs a,
-                                                int heads) {
-  __shared__ double smem[256];
+__global__ void __launch_bounds__(1024) sum_dlam(NpfDiffAttnArgs a,
+                                                 int heads) {
+  __shared__ double smem[1024];
   double s = 0.;
-  const long per = (long)heads * a.parts;
-  for (long i = threadIdx.x; i < a.B * per; i += 256) {
-    const long b = i / per, j = i % per;
-    s += a.dlam_partial[(b * a.H + blockIdx.x * heads) * a.parts + j];
-  }
+  const long per = (long)heads * a.Q;
+#pragma unroll 4
+  for (long i = threadIdx.x; i < a.B * per; i += 1024)
+    s += a.dlam_rows[(i / per * a.H + blockIdx.x * heads) * a.Q + i % per];
   smem[threadIdx.x] = s;
   __syncthreads();
-  for (int n = 128; n > 0; n >>= 1) {
+  for (int n = 512; n > 0; n >>= 1) {
     if (threadIdx.x < n) smem[threadIdx.x] += smem[threadIdx.x + n];
     __syncthreads();
   }
   if (threadIdx.x == 0) store_coded(a.dlam, a.lam_type, blockIdx.x, -smem[0]);
 }
 
-// one wave a query row
 template <typename T>
-__global__ void __launch_bounds__(64) bwd_dq_row(NpfDiffAttnArgs a) {
-  __shared__ float sq[256], sg[256];
-  __shared__ float sd[2][64];
-  const int lane = threadIdx.x, h = blockIdx.y, b = blockIdx.z;
-  const int hk = h / (a.H / a.Hk);
-  const int n = keys_of(a, b);
-  const float lam = lam_of(a, h);
-  for (long r = blockIdx.x; r < a.Q; r += gridDim.x) {
-    __syncthreads();
-    for (int d = lane; d < 2 * a.D; d += 64)
-      sq[d] = (float)row_of<T>(a.q, b, h, r)[d];
-    for (int d = lane; d < a.Dv; d += 64)
-      sg[d] = (float)row_of<T>(a.dout, b, h, r)[d];
-    const long st = (((long)b * a.H + h) * a.Q + r) * 2;
-    float dq[4] = {};
-    for (int k0 = 0; k0 < n; k0 += 64) {
-      __syncthreads();
-      const int kn = n - k0 < 64 ? n - k0 : 64;
-      float ds[2] = {0.f, 0.f};
-      if (lane < kn) {
-        const T* kp = row_of<T>(a.k, b, hk, k0 + lane);
-        const T* vp = row_of<T>(a.v, b, hk, k0 + lane);
-        float g = 0.f, s[2] = {0.f, 0.f};
-        for (int d = 0; d < a.Dv; ++d) g += sg[d] * (float)vp[d];
-        for (int i = 0; i < 2; ++i) {
-          for (int d = 0; d < a.D; ++d)
-            s[i] += sq[i * a.D + d] * (float)kp[i * a.D + d];
-          const float p = exp2f(s[i] * a.scale * kLog2e - a.lse[st + i]);
-          ds[i] = p * (g - a.delta[st + i]) * (i ? -lam : 1.f) * a.scale;
-        }
-      }
-      sd[0][lane] = ds[0];
-      sd[1][lane] = ds[1];
-      __syncthreads();
-      for (int k = 0; k < kn; ++k) {
-        const T* kp = row_of<T>(a.k, b, hk, k0 + k);
-        for (int j = 0; j < 4; ++j) {
-          const int d = lane + 64 * j;
-          if (d < 2 * a.D) dq[j] += sd[d >= a.D][k] * (float)kp[d];
-        }
-      }
-    }
-    for (int j = 0; j < 4; ++j)
-      if (lane + 64 * j < 2 * a.D)
-        row_of<T>(a.dq, b, h, r)[lane + 64 * j] = (T)dq[j];
-  }
-}
-
-// one wave a key row
-template <typename T>
-__global__ void __launch_bounds__(64) bwd_dkv_row(NpfDiffAttnArgs a) {
-  __shared__ float sk[256], sv[256];
-  __shared__ float sd[3][64];
-  const int lane = threadIdx.x, hk = blockIdx.y, b = blockIdx.z;
-  const int group = a.H / a.Hk;
-  const int n = keys_of(a, b);
-  for (long r = blockIdx.x; r < a.K; r += gridDim.x) {
-    __syncthreads();
-    for (int d = lane; d < 2 * a.D; d += 64)
-      sk[d] = (float)row_of<T>(a.k, b, hk, r)[d];
-    for (int d = lane; d < a.Dv; d += 64)
-      sv[d] = (float)row_of<T>(a.v, b, hk, r)[d];
-    float dk[4] = {}, dv[4] = {};
-    for (int h = hk * group; r < n && h < (hk + 1) * group; ++h) {
-      const float lam = lam_of(a, h);
-      for (int q0 = 0; q0 < a.Q; q0 += 64) {
-        __syncthreads();
-        const int qn = a.Q - q0 < 64 ? a.Q - q0 : 64;
-        float ds[2] = {0.f, 0.f}, p[2] = {0.f, 0.f};
-        if (lane < qn) {
-          const long st = (((long)b * a.H + h) * a.Q + q0 + lane) * 2;
-          const T* qp = row_of<T>(a.q, b, h, q0 + lane);
-          const T* gp = row_of<T>(a.dout, b, h, q0 + lane);
-          float g = 0.f, s[2] = {0.f, 0.f};
-          for (int d = 0; d < a.Dv; ++d) g += sv[d] * (float)gp[d];
-          for (int i = 0; i < 2; ++i) {
-            for (int d = 0; d < a.D; ++d)
-              s[i] += sk[i * a.D + d] * (float)qp[i * a.D + d];
-            p[i] = exp2f(s[i] * a.scale * kLog2e - a.lse[st + i]);
-            ds[i] = p[i] * (g - a.delta[st + i]) * (i ? -lam : 1.f) * a.scale;
-          }
-        }
-        sd[0][lane] = ds[0];
-        sd[1][lane] = ds[1];
-        sd[2][lane] = p[0] - lam * p[1];
-        __syncthreads();
-        for (int q = 0; q < qn; ++q) {
-          const T* qp = row_of<T>(a.q, b, h, q0 + q);
-          const T* gp = row_of<T>(a.dout, b, h, q0 + q);
-          for (int j = 0; j < 4; ++j) {
-            const int d = lane + 64 * j;
-            if (d < 2 * a.D) dk[j] += sd[d >= a.D][q] * (float)qp[d];
-            if (d < a.Dv) dv[j] += sd[2][q] * (float)gp[d];
-          }
-        }
-      }
-    }
-    for (int j = 0; j < 4; ++j) {
-      const int d = lane + 64 * j;
-      if (a.dk.p && d < 2 * a.D) row_of<T>(a.dk, b, hk, r)[d] = (T)dk[j];
-      if (a.dv.p && d < a.Dv) row_of<T>(a.dv, b, hk, r)[d] = (T)dv[j];
-    }
-  }
-}
-
-unsigned rows_grid(int rows) { return rows < 65536 ? rows : 65536; }
-
-template <typename T>
-hipError_t launch_bwd(const NpfDiffAttnArgs& a, hipStream_t stream) {
-  bwd_delta<T><<<dim3(a.parts, a.H, a.B), 256, 0, stream>>>(a);
-  if (a.dlam) {
-    bwd_dlam<<<a.lam_heads, 256, 0, stream>>>(a, a.H / a.lam_heads);
-  }
-  if (a.dq.p)
-    bwd_dq_row<T><<<dim3(rows_grid(a.Q), a.H, a.B), 64, 0, stream>>>(a);
-  if (a.dk.p || a.dv.p)
-    bwd_dkv_row<T><<<dim3(rows_grid(a.K), a.Hk, a.B), 64, 0, stream>>>(a);
-  return hipGetLastError();
+void launch_row_stats(const NpfDiffAttnArgs& a, hipStream_t stream) {
+  const long rows = (long)a.B * a.H * a.Q;
+  auto blocks = [&](int lanes) {
+    return (unsigned)((rows * lanes + 255) / 256);
+  };
+  if (a.Dv <= 32)
+    row_stats<T, 8><<<blocks(8), 256, 0, stream>>>(a);
+  else if (a.Dv <= 64)
+    row_stats<T, 16><<<blocks(16), 256, 0, stream>>>(a);
+  else if (a.Dv <= 128)
+    row_stats<T, 32><<<blocks(32), 256, 0, stream>>>(a);
+  else
+    row_stats<T, 64><<<blocks(64), 256, 0, stream>>>(a);
 }
 
 }  // namespace
 
-int npf_diff_attn_parts(int Q) { return (Q + 63) / 64; }
+bool npf_diff_attn_plan(NpfDiffAttnArgs& a) {
+  for (a.pad = 16; a.pad < a.D || 2 * a.pad < a.Dv; a.pad *= 2)
+    if (a.pad == 128) return false;
+  const long rows = (long)(a.H / a.Hk) * a.Q;
+  const long heads = (long)a.B * a.Hk;
+  a.waves = rows <= 32 ? 1 : 4;
+  // Few rows: the key axis is split until every CU has a few blocks, no part
+  // below 256 keys.
+  const long blocks = heads * ((rows + 32 * a.waves - 1) / (32 * a.waves));
+  const long wanted = a.waves == 1 ? 1280 : 512;
+  const long most = (a.K + 255) / 256;
+  long splits = blocks > 0 ? wanted / blocks : 1;
+  splits = splits > most ? most : splits;
+  a.splits = (int)(splits < 1 ? 1 : splits);
+  return true;
+}
+
+size_t npf_diff_attn_workspace(const NpfDiffAttnArgs& a) {
+  if (a.splits <= 1) return 0;
+  return sizeof(float) * a.splits * split_row_floats(a.Dv) * a.B * a.H * a.Q;
+}
 
 hipError_t npf_diff_attn_fwd(const NpfDiffAttnArgs& a, hipStream_t stream) {
-  const dim3 grid(rows_grid(a.Q), a.H, a.B);
+  hipError_t e = hipErrorInvalidValue;
   switch (a.type) {
-    case NPF_F32: fwd_row<float><<<grid, 64, 0, stream>>>(a); break;
-    case NPF_BF16: fwd_row<npf_bf16><<<grid, 64, 0, stream>>>(a); break;
-    case NPF_F16: fwd_row<npf_f16><<<grid, 64, 0, stream>>>(a); break;
-    default: return hipErrorInvalidValue;
+    case NPF_F32: e = npf_diff_attn_fwd_f32(a, stream); break;
+    case NPF_BF16: e = npf_diff_attn_fwd_bf16(a, stream); break;
+    case NPF_F16: e = npf_diff_attn_fwd_f16(a, stream); break;
+  }
+  if (e != hipSuccess || a.splits <= 1) return e;
+  const long rows = (long)a.B * a.H * a.Q;
+  if (rows > 0x7fffffffL) return hipErrorInvalidConfiguration;
+  switch (a.type) {
+    case NPF_F32: join<float><<<(unsigned)rows, kJoinThreads, 0, stream>>>(a); break;
+    case NPF_BF16: join<npf_bf16><<<(unsigned)rows, kJoinThreads, 0, stream>>>(a); break;
+    default: join<npf_f16><<<(unsigned)rows, kJoinThreads, 0, stream>>>(a);
   }
   return hipGetLastError();
 }
 
 hipError_t npf_diff_attn_bwd(const NpfDiffAttnArgs& a, hipStream_t stream) {
+  if ((long)a.B * a.H * a.Q > 0x7fffffffL) return hipErrorInvalidConfiguration;
+  hipError_t e = hipErrorInvalidValue;
   switch (a.type) {
-    case NPF_F32: return launch_bwd<float>(a, stream);
-    case NPF_BF16: return launch_bwd<npf_bf16>(a, stream);
-    case NPF_F16: return launch_bwd<npf_f16>(a, stream);
-    default: return hipErrorInvalidValue;
+    case NPF_F32:
+      launch_row_stats<float>(a, stream);
+      e = npf_diff_attn_bwd_f32(a, stream);
+      break;
+    case NPF_BF16:
+      launch_row_stats<npf_bf16>(a, stream);
+      e = npf_diff_attn_bwd_bf16(a, stream);
+      break;
+    case NPF_F16:
+      launch_row_stats<npf_f16>(a, stream);
+      e = npf_diff_attn_bwd_f16(a, stream);
+      break;
   }
+  if (e != hipSuccess || !a.dlam) return e;
+  sum_dlam<<<a.lam_heads, 1024, 0, stream>>>(a, a.H / a.lam_heads);
+  return hipGetLastError();
 }

@@ -1,0 +1,11 @@
+// Differential attention for one type (a file each, to build side by side).
+
+#include "diff_attn_impl.h"
+
+hipError_t npf_diff_attn_fwd_bf16(const NpfDiffAttnArgs& a, hipStream_t stream) {
+  return npf_attn::fwd_typed<npf_bf16>(a, stream);
+}
+
+hipError_t npf_diff_attn_bwd_bf16(const NpfDiffAttnArgs& a, hipStream_t stream) {
+  return npf_attn::bwd_typed<npf_bf16>(a, stream);
+}

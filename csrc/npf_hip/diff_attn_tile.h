@@ -1,0 +1,289 @@
+// Tiles and matrix products of the differential attention kernels.
+//
+// All products use 32x32 matrix instructions.  A wave's result tile has its
+// column in the lane (lane & 31) and 16 rows in registers: register i of lane
+// half h = lane >> 5 holds row  8 (i / 4) + 4 h + i % 4.  Two facts carry the
+// kernels:
+//
+// - with the score tile taken as (row = key, column = query), a query's
+//   statistics need no more than a register reduction and one exchange between
+//   the lane halves;
+// - a tile in that layout is an operand of the next product as it stands: its
+//   registers hold 16 rows of one column, and the order of the summed axis is
+//   free as long as the other operand follows it.  The other operand, read
+//   against its rows (a transposed read of LDS), follows it.
+//
+// Operands in LDS are row-major tiles of 16-byte chunks.  A row's chunks are
+// permuted by an XOR with a function of the row, chosen so that both reads
+// spread over all 64 banks: 16 rows at one chunk (an operand read along its
+// rows), and 4 + 4 rows at 64 contiguous bytes (the transposed read).
+#pragma once
+
+#include "common.h"
+#include "diff_attn.h"
+#include "types.h"
+
+namespace npf_attn {
+
+using f32x16 = __attribute__((ext_vector_type(16))) float;
+using f32x4 = __attribute__((ext_vector_type(4))) float;
+using u32x4 = __attribute__((ext_vector_type(4))) unsigned;
+using bf16x8 = __attribute__((ext_vector_type(8))) __bf16;
+using f16x8 = __attribute__((ext_vector_type(8))) _Float16;
+using s16x4 = __attribute__((ext_vector_type(4))) short;
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLowest = -3.0e38f;  // below every finite score
+
+// the row that register i holds in lane half 0
+__host__ __device__ constexpr int reg_row(int i) {
+  return 8 * (i / 4) + i % 4;
+}
+
+template <typename T>
+constexpr int kChunk = 16 / (int)sizeof(T);  // values of a chunk
+
+// ------------------------------ products -------------------------------- //
+
+__device__ __forceinline__ f32x16 mma(bf16x8 a, bf16x8 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mma(f16x8 a, f16x8 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mma(float a, float b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0);
+}
+
+template <typename T> struct Vec8;
+template <> struct Vec8<npf_bf16> { using type = bf16x8; };
+template <> struct Vec8<npf_f16> { using type = f16x8; };
+
+// c += a b^T over one chunk a lane half: 16 values of the summed axis in 16
+// bits, 8 (as four products) in 32
+template <typename T>
+__device__ __forceinline__ f32x16 mma_chunk(u32x4 a, u32x4 b, f32x16 c) {
+  if constexpr (sizeof(T) == 2) {
+    using V = typename Vec8<T>::type;
+    return mma(__builtin_bit_cast(V, a), __builtin_bit_cast(V, b), c);
+  } else {
+    const f32x4 x = __builtin_bit_cast(f32x4, a);
+    const f32x4 y = __builtin_bit_cast(f32x4, b);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c = mma(x[i], y[i], c);
+    return c;
+  }
+}
+
+// A 32x32 tile of map values or of their gradients as an operand.  In 16 bits
+// its values are rounded here, once; statistics have seen them in 32.
+template <typename T>
+struct Operand {
+  typename Vec8<T>::type v[2];
+  __device__ __forceinline__ explicit Operand(const f32x16& x) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[t][e] = (T)x[8 * t + e];
+  }
+};
+template <>
+struct Operand<float> {
+  f32x16 v;
+  __device__ __forceinline__ explicit Operand(const f32x16& x) : v(x) {}
+};
+
+// -------------------------------- tiles ---------------------------------- //
+
+template <typename T, int kWidth>
+struct Tile {
+  static constexpr int kRowBytes = kWidth * (int)sizeof(T);
+  static constexpr int kChunks = kRowBytes / 16;
+
+  __device__ static __forceinline__ int permute(int row) {
+    const int low = (row >> 2) & 3;
+    if constexpr (kRowBytes == 64) return low;
+    if constexpr (kRowBytes == 128) return low | (((row >> 1) & 1) << 2);
+    return low | ((row & 3) << 2);
+  }
+  __device__ static __forceinline__ int at(int row, int chunk) {
+    return row * kRowBytes + ((chunk ^ permute(row)) << 4);
+  }
+
+  // one chunk a lane: row `row0 + lane % 32`, chunk `chunk`
+  __device__ static __forceinline__ u32x4 rows(const char* tile, int row,
+                                               int chunk) {
+    return *reinterpret_cast<const u32x4*>(tile + at(row, chunk));
+  }
+
+  // acc[lane % 32 of columns col0 ..][column of p] += tile^T p over the 32
+  // rows from row0 on, for both maps' p at once
+  template <int kMaps>
+  __device__ static __forceinline__ void transposed(
+      const char* tile, int row0, int col0, int lane,
+      const Operand<T> (&p)[kMaps], f32x16* const (&acc)[kMaps]) {
+    const int half = lane >> 5;
+    if constexpr (sizeof(T) == 2) {
+      const int j = lane & 15;
+      // lane j of 16 names 4 values of row j / 4, and gets 4 rows of column j
+      const int chunk = col0 / 8 + 2 * ((lane >> 4) & 1) + ((j & 3) >> 1);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        s16x4 part[2];
+#pragma unroll
+        for (int a = 0; a < 2; ++a) {
+          const int row = row0 + 16 * t + 8 * a + 4 * half + (j >> 2);
+          const char* src = tile + at(row, chunk) + (j & 1) * 8;
+          part[a] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (__attribute__((address_space(3))) s16x4*)(src));
+        }
+        const auto both = __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3,
+                                                  4, 5, 6, 7);
+        const auto v = __builtin_bit_cast(typename Vec8<T>::type, both);
+#pragma unroll
+        for (int m = 0; m < kMaps; ++m) *acc[m] = mma(v, p[m].v[t], *acc[m]);
+      }
+    } else {
+      const int col = col0 + (lane & 31);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int row = row0 + reg_row(i) + 4 * half;
+        const float v = *reinterpret_cast<const float*>(
+            tile + at(row, col >> 2) + (col & 3) * 4);
+#pragma unroll
+        for (int m = 0; m < kMaps; ++m) *acc[m] = mma(v, p[m].v[i], *acc[m]);
+      }
+    }
+  }
+};
+
+// The chunk of a padded row that a thread moves: where its values stand in
+// memory, and how many there are (the rest is padding).
+struct ChunkOf {
+  int offset, count;
+};
+
+// of a row with two maps of `size` values, each padded to kPad
+template <typename T, int kPad>
+__device__ __forceinline__ ChunkOf chunk_of_maps(int chunk, int size) {
+  constexpr int per = kPad / kChunk<T>;
+  const int in_map = (chunk % per) * kChunk<T>;
+  const int left = size - in_map;
+  return {(chunk / per) * size + in_map,
+          left < 0 ? 0 : left > kChunk<T> ? kChunk<T> : left};
+}
+
+template <typename T>
+__device__ __forceinline__ ChunkOf chunk_of_row(int chunk, int size) {
+  const int left = size - chunk * kChunk<T>;
+  return {chunk * kChunk<T>,
+          left < 0 ? 0 : left > kChunk<T> ? kChunk<T> : left};
+}
+
+template <typename T>
+__device__ __forceinline__ u32x4 load_chunk(const T* row, ChunkOf c) {
+  T v[kChunk<T>];
+  if (c.count == kChunk<T>) {
+    load_pack(v, row + c.offset);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kChunk<T>; ++i)
+      v[i] = i < c.count ? row[c.offset + i] : (T)0.f;
+  }
+  u32x4 r;
+  __builtin_memcpy(&r, v, 16);
+  return r;
+}
+
+// Two tiles of kRows rows each moving from memory to LDS through registers,
+// so that the loads of the next pair run under the products of this one.
+template <typename T, int kWidth, int kRows, int kThreads>
+struct Stage {
+  using Lds = Tile<T, kWidth>;
+  static constexpr int kStep = kThreads / Lds::kChunks;  // rows at a time
+  static constexpr int kCount = kRows / kStep;
+  static_assert(kThreads % Lds::kChunks == 0 && kRows % kStep == 0);
+
+  u32x4 x[kCount], y[kCount];
+
+  // rows row0 .. of two tensors; rows from `end` on become zeros
+  __device__ __forceinline__ void load(const T* xp, long xl, ChunkOf xc,
+                                       const T* yp, long yl, ChunkOf yc,
+                                       int row0, int end) {
+    const int first = row0 + (int)threadIdx.x / Lds::kChunks;
+#pragma unroll
+    for (int j = 0; j < kCount; ++j) {
+      const int row = first + j * kStep;
+      x[j] = u32x4{0, 0, 0, 0};
+      y[j] = u32x4{0, 0, 0, 0};
+      if (row < end) {
+        x[j] = load_chunk(xp + row * xl, xc);
+        y[j] = load_chunk(yp + row * yl, yc);
+      }
+    }
+  }
+
+  __device__ __forceinline__ void store(char* xt, char* yt) const {
+    const int first = (int)threadIdx.x / Lds::kChunks;
+    const int chunk = (int)threadIdx.x % Lds::kChunks;
+#pragma unroll
+    for (int j = 0; j < kCount; ++j) {
+      const int at = Lds::at(first + j * kStep, chunk);
+      *reinterpret_cast<u32x4*>(xt + at) = x[j];
+      *reinterpret_cast<u32x4*>(yt + at) = y[j];
+    }
+  }
+};
+
+// ------------------------------- helpers --------------------------------- //
+
+template <typename T>
+__device__ __forceinline__ T* row_of(const NpfHeads& t, int b, int h, long l) {
+  return static_cast<T*>(t.p) + b * t.b + h * t.h + l * t.l;
+}
+
+__device__ __forceinline__ int keys_of(const NpfDiffAttnArgs& a, int b) {
+  if (!a.lengths) return a.K;
+  const long n = a.lengths64 ? static_cast<const long*>(a.lengths)[b]
+                             : (long)static_cast<const int*>(a.lengths)[b];
+  return n < 0 ? 0 : n > a.K ? a.K : (int)n;
+}
+
+__device__ __forceinline__ float lam_of(const NpfDiffAttnArgs& a, int h) {
+  return load_coded(a.lam, a.lam_type, (long)h * a.lam_stride);
+}
+
+// x of the other lane half, for a reduction over both
+struct Halves {
+  float low, high;
+};
+__device__ __forceinline__ Halves halves(float x) {
+  const unsigned u = __builtin_bit_cast(unsigned, x);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  const unsigned low = r[0], high = r[1];
+  return {__builtin_bit_cast(float, low), __builtin_bit_cast(float, high)};
+}
+__device__ __forceinline__ float both_max(float x) {
+  const Halves h = halves(x);
+  return fmaxf(h.low, h.high);
+}
+__device__ __forceinline__ float both_sum(float x) {
+  const Halves h = halves(x);
+  return h.low + h.high;
+}
+
+// 4 consecutive values of a row, of which `count` exist
+template <typename T>
+__device__ __forceinline__ void store4(T* p, int count, float a, float b,
+                                       float c, float d) {
+  const T v[4] = {(T)a, (T)b, (T)c, (T)d};
+  if (count >= 4) {
+    store_pack(p, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < count) p[i] = v[i];
+  }
+}
+
+}  // namespace npf_attn

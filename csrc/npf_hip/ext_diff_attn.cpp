@@ -83,6 +83,9 @@ NpfDiffAttnArgs common_args(const Tensor& q, const Tensor& k, const Tensor& v,
   }
   a.type = npf_type_code(q, "queries");
   a.scale = (float)scale;
+  TORCH_CHECK_VALUE(npf_diff_attn_plan(a),
+                    "differential_attention: sizes ", a.D, " and ", a.Dv,
+                    " of a head are too large");
   a.q = heads_of(q);
   a.k = heads_of(k);
   a.v = heads_of(v);
@@ -105,6 +108,11 @@ std::tuple<Tensor, Tensor, Tensor> diff_attn_fwd(
   if (save) {
     a.o2 = heads_of(o2);
     a.lse = lse.data_ptr<float>();
+  }
+  Tensor split;
+  if (const size_t bytes = npf_diff_attn_workspace(a)) {
+    split = torch::empty({(long)bytes}, q.options().dtype(torch::kUInt8));
+    a.split = split.data_ptr();
   }
   npf_check(npf_diff_attn_fwd(a, at::hip::getCurrentHIPStream()),
             "differential_attention");
@@ -133,16 +141,15 @@ std::tuple<OptTensor, OptTensor, OptTensor, OptTensor> diff_attn_bwd(
     return {dq, dk, dv, dlam};
   }
   auto f32 = q.options().dtype(torch::kFloat32);
-  Tensor delta = torch::empty({(long)a.B * a.H * a.Q * 2}, f32);
-  a.parts = npf_diff_attn_parts(a.Q);
-  Tensor dlam_partial = torch::empty({(long)a.B * a.H * a.parts},
-                                     f32.dtype(torch::kFloat64));
+  const long rows = (long)a.B * a.H * a.Q;
+  Tensor stats = torch::empty({rows, 4}, f32);
+  Tensor dlam_rows = torch::empty({rows}, f32);
   a.out = heads_of(out);
   a.o2 = heads_of(o2);
   a.dout = heads_of(dout);
   a.lse = lse.data_ptr<float>();
-  a.delta = delta.data_ptr<float>();
-  a.dlam_partial = dlam_partial.data_ptr<double>();
+  a.stats = stats.data_ptr<float>();
+  a.dlam_rows = dlam_rows.data_ptr<float>();
   if (dq) a.dq = heads_of(*dq);
   if (dk) a.dk = heads_of(*dk);
   if (dv) a.dv = heads_of(*dv);
