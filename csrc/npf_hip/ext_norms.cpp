@@ -109,7 +109,7 @@ std::tuple<OptTensor, OptTensor, OptTensor> layer_norm_bwd(
   if (need_dweight) dweight = torch::empty_like(*weight);
   if (need_dbias) dbias = torch::empty_like(*bias);
   if (need_dweight || need_dbias) {
-    a.parts = npf_layernorm_parts(a.rows, a.width, type);
+    a.parts = npf_layernorm_parts(a, type);
     partial = torch::empty({a.parts, 2, x.size(1)},
                            x.options().dtype(torch::kFloat32));
     a.partial = partial->data_ptr<float>();
@@ -120,9 +120,8 @@ std::tuple<OptTensor, OptTensor, OptTensor> layer_norm_bwd(
   a.rstd = rstd.data_ptr<float>();
   a.dweight = ptr_of(dweight);
   a.dbias = ptr_of(dbias);
-  npf_check(
-      npf_layernorm_bwd(a, type, need_dx, at::hip::getCurrentHIPStream()),
-      "layer_norm backward");
+  npf_check(npf_layernorm_bwd(a, type, at::hip::getCurrentHIPStream()),
+            "layer_norm backward");
   return {dx, dweight, dbias};
 }
 

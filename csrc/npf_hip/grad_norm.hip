@@ -60,17 +60,63 @@ __device__ __forceinline__ int span_of(const NpfGradSpans& s, int chunk) {
   return lo;
 }
 
+// A chunk is 32 KiB: 8 accesses of 16 bytes a thread, all in flight at once.
 template <typename T>
 __device__ __forceinline__ double sum_chunk(const T* p, long n, int norm) {
+  constexpr int V = 16 / (int)sizeof(T);
+  constexpr long kFull = kGradChunkBytes / (long)sizeof(T);
   double s = 0.;
-  for (long i = threadIdx.x; i < n; i += kThreads)
-    s = join(s, value_of((double)p[i], norm), norm);
+  if (n == kFull) {
+    T v[8][V];
+    double part[4] = {};
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      load_pack(v[k], p + (k * kThreads + threadIdx.x) * V);
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        part[k & 3] = join(part[k & 3], value_of((double)v[k][i], norm), norm);
+    return join(join(part[0], part[1], norm), join(part[2], part[3], norm),
+                norm);
+  }
+  long i = (long)threadIdx.x * V;
+  for (; i + V <= n; i += kThreads * V) {
+    T v[V];
+    load_pack(v, p + i);
+#pragma unroll
+    for (int k = 0; k < V; ++k) s = join(s, value_of((double)v[k], norm), norm);
+  }
+  for (; i < n; ++i) s = join(s, value_of((double)p[i], norm), norm);
   return s;
 }
 
-template <typename T>
-__device__ __forceinline__ void scale_chunk(T* p, long n, float c) {
-  for (long i = threadIdx.x; i < n; i += kThreads) p[i] = (T)(p[i] * c);
+template <typename T, typename C>
+__device__ __forceinline__ void scale_chunk(T* p, long n, C c) {
+  constexpr int V = 16 / (int)sizeof(T);
+  constexpr long kFull = kGradChunkBytes / (long)sizeof(T);
+  if (n == kFull) {
+    T v[8][V];
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      load_pack(v[k], p + (k * kThreads + threadIdx.x) * V);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[k][i] = (T)((C)v[k][i] * c);
+      store_pack(p + (k * kThreads + threadIdx.x) * V, v[k]);
+    }
+    return;
+  }
+  long i = (long)threadIdx.x * V;
+  for (; i + V <= n; i += kThreads * V) {
+    T v[V];
+    load_pack(v, p + i);
+#pragma unroll
+    for (int k = 0; k < V; ++k) v[k] = (T)((C)v[k] * c);
+    store_pack(p + i, v);
+  }
+  for (; i < n; ++i) p[i] = (T)((C)p[i] * c);
 }
 
 __global__ void __launch_bounds__(kThreads)
@@ -123,10 +169,7 @@ __global__ void __launch_bounds__(kThreads)
       case NPF_F32: scale_chunk((float*)s.ptr[i] + at, m, scale); break;
       case NPF_BF16: scale_chunk((npf_bf16*)s.ptr[i] + at, m, scale); break;
       case NPF_F16: scale_chunk((npf_f16*)s.ptr[i] + at, m, scale); break;
-      default: {
-        double* p = (double*)s.ptr[i] + at;
-        for (long k = threadIdx.x; k < m; k += kThreads) p[k] *= ratio;
-      }
+      default: scale_chunk((double*)s.ptr[i] + at, m, ratio);
     }
   }
 }

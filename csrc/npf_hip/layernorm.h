@@ -9,7 +9,8 @@ struct NpfLayerNormArgs {
   const void* weight;    // [width] or null
   const void* bias;      // [width] or null
   const void* dy;        // backward: [rows, width] contiguous
-  void* y;               // forward: y; backward: dx; [rows, width] contiguous
+  void* y;               // forward: y; backward: dx, or null;
+                         // [rows, width] contiguous
   float* mean;           // [rows]; forward: written where not null
   float* rstd;           // [rows]
   float* partial;        // backward: [parts, 2, width], or null
@@ -24,7 +25,6 @@ struct NpfLayerNormArgs {
 };
 
 // rows of `partial` that the backward pass fills for this problem
-int npf_layernorm_parts(long rows, int width, int type);
+int npf_layernorm_parts(const NpfLayerNormArgs&, int type);
 hipError_t npf_layernorm_fwd(const NpfLayerNormArgs&, int type, hipStream_t);
-hipError_t npf_layernorm_bwd(const NpfLayerNormArgs&, int type, bool need_dx,
-                             hipStream_t);
+hipError_t npf_layernorm_bwd(const NpfLayerNormArgs&, int type, hipStream_t);
