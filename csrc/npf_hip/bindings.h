@@ -2,6 +2,7 @@
 #pragma once
 
 #include <hip/hip_runtime.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
 #include "type_codes.h"
@@ -27,4 +28,23 @@ inline int npf_type_code(const torch::Tensor& t, const char* name,
 
 inline void npf_check(hipError_t e, const char* what) {
   TORCH_CHECK(e == hipSuccess, what, ": ", hipGetErrorString(e));
+}
+
+// Gradients of an operator that is differentiable once: where a graph is built
+// over its backward pass, a second derivative is an error rather than zero.
+inline torch::autograd::variable_list npf_once(
+    torch::autograd::variable_list grads, const char* name) {
+  if (!at::GradMode::is_enabled()) return grads;
+  torch::autograd::variable_list some;
+  for (const auto& g : grads)
+    if (g.defined()) some.push_back(g.detach().requires_grad_());
+  if (some.empty()) return grads;
+  const int64_t n = (int64_t)some.size();
+  auto error = std::make_shared<torch::autograd::DelayedError>(
+      std::string(name) + " is differentiable once", n);
+  some = (*error)(std::move(some));
+  size_t i = 0;
+  for (auto& g : grads)
+    if (g.defined()) g = some[i++];
+  return grads;
 }

@@ -72,11 +72,13 @@ __global__ void __launch_bounds__(kJoinThreads) join(NpfDiffAttnArgs a) {
 // delta_i of each row, beside its lse: kLanes lanes of 4 values a row
 template <typename T, int kLanes>
 __global__ void __launch_bounds__(256) row_stats(NpfDiffAttnArgs a) {
-  const long rows = (long)a.B * a.H * a.Q;
-  const long r = (long)blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
+  // (rows are checked to fit 31 bits; divisions of 64 bits would cost more
+  // than the sums)
+  const unsigned rows = (unsigned)a.B * a.H * a.Q;
+  const unsigned r = blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
   if (r >= rows) return;  // whole groups of lanes
-  const int q = (int)(r % a.Q);
-  const int h = (int)(r / a.Q % a.H), b = (int)(r / a.Q / a.H);
+  const int q = (int)(r % (unsigned)a.Q), bh = (int)(r / (unsigned)a.Q);
+  const int h = bh % a.H, b = bh / a.H;
   const int c = (threadIdx.x % kLanes) * 4;
   const float lam = lam_of(a, h);
   float d1 = 0.f, d2 = 0.f;
@@ -109,7 +111,7 @@ __global__ void __launch_bounds__(256) row_stats(NpfDiffAttnArgs a) {
   }
   if (threadIdx.x % kLanes == 0)
     reinterpret_cast<float4*>(a.stats)[r] =
-        float4{a.lse[2 * r], a.lse[2 * r + 1], d1, d2};
+        float4{a.lse[2L * r], a.lse[2L * r + 1], d1, d2};
 }
 
 // dlam of one head (of all heads where lam is one number)
@@ -153,13 +155,12 @@ bool npf_diff_attn_plan(NpfDiffAttnArgs& a) {
     if (a.pad == 128) return false;
   const long rows = (long)(a.H / a.Hk) * a.Q;
   const long heads = (long)a.B * a.Hk;
-  a.waves = rows <= 32 ? 1 : 4;
-  // Few rows: the key axis is split until every CU has a few blocks, no part
+  a.waves = heads * ((rows + 127) / 128) >= kManyBlocks ? 4 : 1;
+  // Few rows: the key axis is split until every SIMD has a wave, no part
   // below 256 keys.
-  const long blocks = heads * ((rows + 32 * a.waves - 1) / (32 * a.waves));
-  const long wanted = a.waves == 1 ? 1280 : 512;
+  const long waves = heads * ((rows + 31) / 32);
   const long most = (a.K + 255) / 256;
-  long splits = blocks > 0 ? wanted / blocks : 1;
+  long splits = a.waves == 1 && waves > 0 && waves < 512 ? 1280 / waves : 1;
   splits = splits > most ? most : splits;
   a.splits = (int)(splits < 1 ? 1 : splits);
   return true;

@@ -3,9 +3,9 @@
 #include "diff_attn_impl.h"
 
 hipError_t npf_diff_attn_fwd_f16(const NpfDiffAttnArgs& a, hipStream_t stream) {
-  return npf_attn::fwd_typed<npf_f16>(a, stream);
+  return npf_attn::typed<npf_f16>(a, false, stream);
 }
 
 hipError_t npf_diff_attn_bwd_f16(const NpfDiffAttnArgs& a, hipStream_t stream) {
-  return npf_attn::bwd_typed<npf_f16>(a, stream);
+  return npf_attn::typed<npf_f16>(a, true, stream);
 }

@@ -3,9 +3,9 @@
 #include "diff_attn_impl.h"
 
 hipError_t npf_diff_attn_fwd_f32(const NpfDiffAttnArgs& a, hipStream_t stream) {
-  return npf_attn::fwd_typed<float>(a, stream);
+  return npf_attn::typed<float>(a, false, stream);
 }
 
 hipError_t npf_diff_attn_bwd_f32(const NpfDiffAttnArgs& a, hipStream_t stream) {
-  return npf_attn::bwd_typed<float>(a, stream);
+  return npf_attn::typed<float>(a, true, stream);
 }

@@ -22,10 +22,20 @@ struct Shape {
   static constexpr int kRowBytes = kWidth * (int)sizeof(T);
   // keys (or queries) a tile: two buffers of two tiles in 64 KiB
   static constexpr int kTile = kRowBytes <= 256 ? 64 : 32;
+  // tiles of 32 that a wave takes through a pass at once
+  static constexpr int kSubs = kPad <= 32 ? 2 : 1;
+  // parts of the values' columns that forward blocks take: the sums of 256
+  // columns for two maps would fill a wave's registers by themselves
+  static constexpr int kParts = kPad == 128 ? 2 : 1;
   static constexpr int kSteps = kPad / (2 * kChunk<T>);  // chunk pairs a map
   static constexpr int kBlocks = kWidth / 32;  // 32 columns of a whole row
   static constexpr int kMapBlocks = kPad / 32 > 0 ? kPad / 32 : 1;
 };
+
+// Waves a SIMD is to hold: two, in half of the registers each and with every
+// matrix result in ordinary registers, where a kernel fits; else one.
+template <typename T, int kPad>
+constexpr int kResident = kPad * (int)sizeof(T) <= 64 ? 2 : 1;
 
 // Columns that block n of map m starts at.  Maps of 16 share one block: each
 // accumulates it whole and keeps its half.
@@ -54,18 +64,24 @@ __device__ __forceinline__ float exp_tile(f32x16& s, float c, float m) {
   return sum;
 }
 
-template <typename T, int kPad, int kWaves>
-__global__ void __launch_bounds__(64 * kWaves)
+template <typename T, int kPad, int kWaves, bool kDirect>
+__global__ void __launch_bounds__(64 * kWaves, (kResident<T, kPad>))
     diff_fwd(NpfDiffAttnArgs a) {
   using S = Shape<T, kPad>;
   using Lds = Tile<T, S::kWidth>;
-  constexpr int kTile = kWaves == 1 ? 32 : S::kTile;
+  constexpr int kTile = kWaves == 1 ? 32 * S::kSubs : S::kTile;
+  constexpr int kSubs = S::kSubs, kCols = S::kBlocks / S::kParts;
   constexpr int kTileBytes = kTile * S::kRowBytes;
-  extern __shared__ __attribute__((aligned(16))) char lds[];
+  // two objects, so that it shows that the next tiles' loads do not touch
+  // what is being read
+  __shared__ __attribute__((aligned(16))) char even[2 * kTileBytes];
+  __shared__ __attribute__((aligned(16))) char odd[2 * kTileBytes];
 
   const int group = a.H / a.Hk, rows = group * a.Q;
   const int row_tiles = (rows + 32 * kWaves - 1) / (32 * kWaves);
   int id = blockIdx.x;
+  const int part = id % S::kParts;
+  id /= S::kParts;
   const int split = id % a.splits;
   id /= a.splits;
   const int row_tile = id % row_tiles, bh = id / row_tiles;
@@ -92,58 +108,55 @@ __global__ void __launch_bounds__(64 * kWaves)
       const ChunkOf c =
           chunk_of_maps<T, kPad>((m * S::kSteps + u) * 2 + half, a.D);
       qf[m][u] = u32x4{0, 0, 0, 0};
-      if (live) qf[m][u] = load_chunk(row_of<T>(a.q, b, h, q), c);
+      if (live) qf[m][u] = load_chunk<kDirect>(row_of<T>(a.q, b, h, q), c);
     }
 
-  f32x16 o[2][S::kBlocks];
+  f32x16 o[2][kCols];
 #pragma unroll
   for (int m = 0; m < 2; ++m)
 #pragma unroll
-    for (int j = 0; j < S::kBlocks; ++j) o[m][j] = f32x16{};
+    for (int j = 0; j < kCols; ++j) o[m][j] = f32x16{};
   float mx[2] = {kLowest, kLowest}, l[2] = {0.f, 0.f};
   const float c = a.scale * kLog2e;
 
-  Stage<T, S::kWidth, kTile, 64 * kWaves> stage;
-  const int chunk = (int)threadIdx.x % Lds::kChunks;
-  const ChunkOf kc = chunk_of_maps<T, kPad>(chunk, a.D);
-  const ChunkOf vc = chunk_of_row<T>(chunk, a.Dv);
+  Stage<T, S::kWidth, kTile, 64 * kWaves, kDirect> stage;
   const T* kp = row_of<T>(a.k, b, hk, 0);
   const T* vp = row_of<T>(a.v, b, hk, 0);
-  if (begin < end) {
-    stage.load(kp, a.k.l, kc, vp, a.v.l, vc, begin, end);
-    stage.store(lds, lds + kTileBytes);
-  }
-  __syncthreads();
-  int buffer = 0;
-  for (int k0 = begin; k0 < end; k0 += kTile, buffer ^= 1) {
-    const bool more = k0 + kTile < end;
-    if (more) stage.load(kp, a.k.l, kc, vp, a.v.l, vc, k0 + kTile, end);
-    const char* kt = lds + buffer * 2 * kTileBytes;
+  // one tile from LDS; kEdge: it may reach behind the last key
+  auto pass = [&](auto edge, int k0, const char* kt) {
+    constexpr bool kEdge = decltype(edge)::value;
     const char* vt = kt + kTileBytes;
 #pragma unroll
-    for (int sub = 0; sub < kTile; sub += 32) {
-      if (k0 + sub >= end) break;
-      f32x16 s[2];
+    for (int sub0 = 0; sub0 < kTile; sub0 += 32 * kSubs) {
+      if (kEdge && k0 + sub0 >= end) break;
+      f32x16 s[2][kSubs];
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int t = 0; t < kSubs; ++t) {
+          s[m][t] = f32x16{};
+#pragma unroll
+          for (int u = 0; u < S::kSteps; ++u)
+            s[m][t] = mma_chunk<T>(
+                Lds::rows(kt, sub0 + 32 * t + col,
+                          (m * S::kSteps + u) * 2 + half),
+                qf[m][u], s[m][t]);
+        }
+      if constexpr (kEdge) {
+#pragma unroll
+        for (int t = 0; t < kSubs; ++t)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (k0 + sub0 + 32 * t + reg_row(i) + 4 * half >= end)
+              s[0][t][i] = s[1][t][i] = -INFINITY;
+      }
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
-        s[m] = f32x16{};
+        float top = s[m][0][0];
 #pragma unroll
-        for (int u = 0; u < S::kSteps; ++u)
-          s[m] = mma_chunk<T>(
-              Lds::rows(kt, sub + col, (m * S::kSteps + u) * 2 + half),
-              qf[m][u], s[m]);
-      }
-      if (k0 + sub + 32 > end) {
+        for (int t = 0; t < kSubs; ++t)
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (k0 + sub + reg_row(i) + 4 * half >= end)
-            s[0][i] = s[1][i] = -INFINITY;
-      }
-#pragma unroll
-      for (int m = 0; m < 2; ++m) {
-        float top = s[m][0];
-#pragma unroll
-        for (int i = 1; i < 16; ++i) top = fmaxf(top, s[m][i]);
+          for (int i = 0; i < 16; ++i) top = fmaxf(top, s[m][t][i]);
         top = both_max(top) * c;
         // The maximum is raised only where it is exceeded by 2^8: exponents
         // stay below that, far from any type's end, and most tiles leave the
@@ -154,22 +167,49 @@ __global__ void __launch_bounds__(64 * kWaves)
           mx[m] = up;
           l[m] *= f;
 #pragma unroll
-          for (int j = 0; j < S::kBlocks; ++j) o[m][j] *= f;
+          for (int j = 0; j < kCols; ++j) o[m][j] *= f;
         }
-        l[m] += exp_tile(s[m], c, mx[m]);
       }
-      const Operand<T> p[2] = {Operand<T>(s[0]), Operand<T>(s[1])};
 #pragma unroll
-      for (int j = 0; j < S::kBlocks; ++j) {
-        f32x16* const acc[2] = {&o[0][j], &o[1][j]};
-        Lds::template transposed<2>(vt, sub, 32 * j, lane, p, acc);
+      for (int t = 0; t < kSubs; ++t) {
+        l[0] += exp_tile(s[0][t], c, mx[0]);
+        l[1] += exp_tile(s[1][t], c, mx[1]);
+        const Operand<T> p[2] = {Operand<T>(s[0][t]), Operand<T>(s[1][t])};
+#pragma unroll
+        for (int j = 0; j < kCols; ++j) {
+          f32x16* const acc[2] = {&o[0][j], &o[1][j]};
+          Lds::template transposed<2>(vt, sub0 + 32 * t,
+                                      32 * (part * kCols + j), lane, p, acc);
+        }
       }
     }
-    if (more)
-      stage.store(lds + (buffer ^ 1) * 2 * kTileBytes,
-                  lds + (buffer ^ 1) * 2 * kTileBytes + kTileBytes);
+  };
+  auto step = [&](int k0, const char* now, char* then) {
+    const int next = k0 + kTile;
+    if (next < end)
+      stage.load(kp, a.k.l, vp, a.v.l, a.D, a.Dv, next, end, then,
+                 then + kTileBytes);
+    pass(std::false_type{}, k0, now);
+    if (next < end) stage.store(end - next, then, then + kTileBytes);
     __syncthreads();
+  };
+  if (begin < end) {
+    stage.load(kp, a.k.l, vp, a.v.l, a.D, a.Dv, begin, end, even,
+               even + kTileBytes);
+    stage.store(end - begin, even, even + kTileBytes);
   }
+  __syncthreads();
+  const int full = (end - begin) / kTile;
+  int k0 = begin;
+  for (int t = 0; t < full;) {
+    step(k0, even, odd);
+    k0 += kTile;
+    if (++t == full) break;
+    step(k0, odd, even);
+    k0 += kTile;
+    ++t;
+  }
+  if (k0 < end) pass(std::true_type{}, k0, full & 1 ? odd : even);
 
 #pragma unroll
   for (int m = 0; m < 2; ++m) l[m] = both_sum(l[m]);
@@ -178,7 +218,7 @@ __global__ void __launch_bounds__(64 * kWaves)
     float* w = static_cast<float*>(a.split) +
                ((long)bh * rows + row) * a.splits * split_row_floats(a.Dv) +
                split * split_row_floats(a.Dv);
-    if (half == 0) {
+    if (half == 0 && part == 0) {
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
         w[2 * m] = mx[m];
@@ -189,10 +229,10 @@ __global__ void __launch_bounds__(64 * kWaves)
 #pragma unroll
     for (int m = 0; m < 2; ++m)
 #pragma unroll
-      for (int j = 0; j < S::kBlocks; ++j)
+      for (int j = 0; j < kCols; ++j)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          const int d = 32 * j + 8 * g + 4 * half;
+          const int d = 32 * (part * kCols + j) + 8 * g + 4 * half;
           const f32x16& x = o[m][j];
           store4(w + m * a.Dv + d, a.Dv - d, x[4 * g], x[4 * g + 1],
                  x[4 * g + 2], x[4 * g + 3]);
@@ -206,10 +246,10 @@ __global__ void __launch_bounds__(64 * kWaves)
   T* out = row_of<T>(a.out, b, h, q);
   T* o2 = a.o2.p ? row_of<T>(a.o2, b, h, q) : nullptr;
 #pragma unroll
-  for (int j = 0; j < S::kBlocks; ++j)
+  for (int j = 0; j < kCols; ++j)
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      const int d = 32 * j + 8 * g + 4 * half;
+      const int d = 32 * (part * kCols + j) + 8 * g + 4 * half;
       float x[4], y[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -219,7 +259,7 @@ __global__ void __launch_bounds__(64 * kWaves)
       store4(out + d, a.Dv - d, x[0], x[1], x[2], x[3]);
       if (o2) store4(o2 + d, a.Dv - d, y[0], y[1], y[2], y[3]);
     }
-  if (a.lse && half == 0) {
+  if (a.lse && half == 0 && part == 0) {
     float* p = a.lse + (((long)b * a.H + h) * a.Q + q) * 2;
 #pragma unroll
     for (int m = 0; m < 2; ++m) p[m] = n ? mx[m] + __log2f(l[m]) : 0.f;
@@ -228,14 +268,18 @@ __global__ void __launch_bounds__(64 * kWaves)
 
 // dq, and each row's part of dlam: a wave holds 32 query rows and passes over
 // the keys
-template <typename T, int kPad, int kWaves>
-__global__ void __launch_bounds__(64 * kWaves)
+template <typename T, int kPad, int kWaves, bool kDirect>
+__global__ void __launch_bounds__(64 * kWaves, (kResident<T, kPad>))
     diff_bwd_dq(NpfDiffAttnArgs a) {
   using S = Shape<T, kPad>;
   using Lds = Tile<T, S::kWidth>;
-  constexpr int kTile = S::kTile;
+  constexpr int kTile = kWaves == 1 ? 32 * S::kSubs : S::kTile;
+  constexpr int kSubs = S::kSubs;
   constexpr int kTileBytes = kTile * S::kRowBytes;
-  extern __shared__ __attribute__((aligned(16))) char lds[];
+  // two objects, so that it shows that the next tiles' loads do not touch
+  // what is being read
+  __shared__ __attribute__((aligned(16))) char even[2 * kTileBytes];
+  __shared__ __attribute__((aligned(16))) char odd[2 * kTileBytes];
 
   const int group = a.H / a.Hk, rows = group * a.Q;
   const int row_tiles = (rows + 32 * kWaves - 1) / (32 * kWaves);
@@ -255,9 +299,9 @@ __global__ void __launch_bounds__(64 * kWaves)
     u32x4 x{0, 0, 0, 0};
     gf[u] = x;
     if (live) {
-      x = load_chunk(row_of<T>(a.q, b, h, q),
+      x = load_chunk<kDirect>(row_of<T>(a.q, b, h, q),
                      chunk_of_maps<T, kPad>(u * 2 + half, a.D));
-      gf[u] = load_chunk(row_of<T>(a.dout, b, h, q),
+      gf[u] = load_chunk<kDirect>(row_of<T>(a.dout, b, h, q),
                          chunk_of_row<T>(u * 2 + half, a.Dv));
     }
     qf[u / S::kSteps][u % S::kSteps] = x;
@@ -273,65 +317,94 @@ __global__ void __launch_bounds__(64 * kWaves)
     for (int j = 0; j < S::kMapBlocks; ++j) dq[m][j] = f32x16{};
   float dlam = 0.f;
 
-  Stage<T, S::kWidth, kTile, 64 * kWaves> stage;
-  const int chunk = (int)threadIdx.x % Lds::kChunks;
-  const ChunkOf kc = chunk_of_maps<T, kPad>(chunk, a.D);
-  const ChunkOf vc = chunk_of_row<T>(chunk, a.Dv);
+  Stage<T, S::kWidth, kTile, 64 * kWaves, kDirect> stage;
   const T* kp = row_of<T>(a.k, b, hk, 0);
   const T* vp = row_of<T>(a.v, b, hk, 0);
-  if (n > 0) {
-    stage.load(kp, a.k.l, kc, vp, a.v.l, vc, 0, n);
-    stage.store(lds, lds + kTileBytes);
-  }
-  __syncthreads();
-  int buffer = 0;
-  for (int k0 = 0; k0 < n; k0 += kTile, buffer ^= 1) {
-    const bool more = k0 + kTile < n;
-    if (more) stage.load(kp, a.k.l, kc, vp, a.v.l, vc, k0 + kTile, n);
-    const char* kt = lds + buffer * 2 * kTileBytes;
+  auto pass = [&](auto edge, int k0, const char* kt) {
+    constexpr bool kEdge = decltype(edge)::value;
     const char* vt = kt + kTileBytes;
 #pragma unroll
-    for (int sub = 0; sub < kTile; sub += 32) {
-      if (k0 + sub >= n) break;
-      f32x16 s[2], g{};
+    for (int sub0 = 0; sub0 < kTile; sub0 += 32 * kSubs) {
+      if (kEdge && k0 + sub0 >= n) break;
+      f32x16 s[2][kSubs], g[kSubs];
 #pragma unroll
-      for (int m = 0; m < 2; ++m) {
-        s[m] = f32x16{};
+      for (int t = 0; t < kSubs; ++t) {
+        const int sub = sub0 + 32 * t;
 #pragma unroll
-        for (int u = 0; u < S::kSteps; ++u)
-          s[m] = mma_chunk<T>(
-              Lds::rows(kt, sub + col, (m * S::kSteps + u) * 2 + half),
-              qf[m][u], s[m]);
-      }
+        for (int m = 0; m < 2; ++m) {
+          s[m][t] = f32x16{};
 #pragma unroll
-      for (int u = 0; u < 2 * S::kSteps; ++u)
-        g = mma_chunk<T>(Lds::rows(vt, sub + col, u * 2 + half), gf[u], g);
-      const bool edge = k0 + sub + 32 > n;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][i], c, -st.x));
-        float p2 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[1][i], c, -st.y));
-        if (edge && k0 + sub + reg_row(i) + 4 * half >= n) p1 = p2 = 0.f;
-        dlam = __builtin_fmaf(p2, g[i], dlam);
-        s[0][i] = p1 * (g[i] - st.z);
-        s[1][i] = p2 * (g[i] - st.w) * -lam;
-      }
-      const Operand<T> ds[2] = {Operand<T>(s[0]), Operand<T>(s[1])};
-#pragma unroll
-      for (int m = 0; m < 2; ++m)
-#pragma unroll
-        for (int j = 0; j < S::kMapBlocks; ++j) {
-          const Operand<T> one[1] = {ds[m]};
-          f32x16* const acc[1] = {&dq[m][j]};
-          Lds::template transposed<1>(kt, sub, map_col<kPad>(m, j), lane, one,
-                                      acc);
+          for (int u = 0; u < S::kSteps; ++u)
+            s[m][t] = mma_chunk<T>(
+                Lds::rows(kt, sub + col, (m * S::kSteps + u) * 2 + half),
+                qf[m][u], s[m][t]);
         }
+        g[t] = f32x16{};
+#pragma unroll
+        for (int u = 0; u < 2 * S::kSteps; ++u)
+          g[t] = mma_chunk<T>(Lds::rows(vt, sub + col, u * 2 + half), gf[u],
+                              g[t]);
+      }
+      if constexpr (kEdge) {
+#pragma unroll
+        for (int t = 0; t < kSubs; ++t)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (k0 + sub0 + 32 * t + reg_row(i) + 4 * half >= n)
+              s[0][t][i] = s[1][t][i] = -INFINITY;
+      }
+#pragma unroll
+      for (int t = 0; t < kSubs; ++t) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float gi = g[t][i];
+          const float p1 = __builtin_amdgcn_exp2f(
+              __builtin_fmaf(s[0][t][i], c, -st.x));
+          const float p2 = __builtin_amdgcn_exp2f(
+              __builtin_fmaf(s[1][t][i], c, -st.y));
+          dlam = __builtin_fmaf(p2, gi, dlam);
+          s[0][t][i] = p1 * (gi - st.z);
+          s[1][t][i] = p2 * (gi - st.w) * -lam;
+        }
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+          const Operand<T> ds[1] = {Operand<T>(s[m][t])};
+#pragma unroll
+          for (int j = 0; j < S::kMapBlocks; ++j) {
+            f32x16* const acc[1] = {&dq[m][j]};
+            Lds::template transposed<1>(kt, sub0 + 32 * t, map_col<kPad>(m, j),
+                                        lane, ds, acc);
+          }
+        }
+      }
     }
-    if (more)
-      stage.store(lds + (buffer ^ 1) * 2 * kTileBytes,
-                  lds + (buffer ^ 1) * 2 * kTileBytes + kTileBytes);
+  };
+  auto step = [&](int k0, const char* now, char* then) {
+    const int next = k0 + kTile;
+    if (next < n)
+      stage.load(kp, a.k.l, vp, a.v.l, a.D, a.Dv, next, n, then,
+                 then + kTileBytes);
+    pass(std::false_type{}, k0, now);
+    if (next < n) stage.store(n - next, then, then + kTileBytes);
     __syncthreads();
+  };
+  if (0 < n) {
+    stage.load(kp, a.k.l, vp, a.v.l, a.D, a.Dv, 0, n, even,
+               even + kTileBytes);
+    stage.store(n, even, even + kTileBytes);
   }
+  __syncthreads();
+  const int full = (n) / kTile;
+  int k0 = 0;
+  for (int t = 0; t < full;) {
+    step(k0, even, odd);
+    k0 += kTile;
+    if (++t == full) break;
+    step(k0, odd, even);
+    k0 += kTile;
+    ++t;
+  }
+  if (k0 < n) pass(std::true_type{}, k0, full & 1 ? odd : even);
 
   dlam = both_sum(dlam);
   if (!live) return;
@@ -354,17 +427,20 @@ __global__ void __launch_bounds__(64 * kWaves)
 
 // dk and dv: a wave holds 32 keys and passes over the queries of the heads
 // that share them
-template <typename T, int kPad, int kWaves, bool kDk, bool kDv>
-__global__ void __launch_bounds__(64 * kWaves)
+template <typename T, int kPad, int kWaves, bool kDirect, bool kDk, bool kDv>
+__global__ void __launch_bounds__(64 * kWaves, (kResident<T, kPad>))
     diff_bwd_dkv(NpfDiffAttnArgs a) {
   using S = Shape<T, kPad>;
   using Lds = Tile<T, S::kWidth>;
-  constexpr int kTile = S::kTile;
+  constexpr int kTile = kWaves == 1 ? 32 : S::kTile;
   constexpr int kTileBytes = kTile * S::kRowBytes;
-  extern __shared__ __attribute__((aligned(16))) char lds[];
-  // both buffers' statistics, one array each of lse_1, lse_2, delta_1, delta_2
-  float(*stats)[4][kTile] =
-      reinterpret_cast<float(*)[4][kTile]>(lds + 4 * kTileBytes);
+  // two objects, so that it shows that the next tiles' loads do not touch
+  // what is being read
+  __shared__ __attribute__((aligned(16))) char even[2 * kTileBytes];
+  __shared__ __attribute__((aligned(16))) char odd[2 * kTileBytes];
+  // of each tile's queries: lse_1, lse_2, delta_1, delta_2
+  __shared__ __attribute__((aligned(16))) float even_stats[4][kTile];
+  __shared__ __attribute__((aligned(16))) float odd_stats[4][kTile];
 
   const int group = a.H / a.Hk;
   const int key_tiles = (a.K + 32 * kWaves - 1) / (32 * kWaves);
@@ -382,10 +458,10 @@ __global__ void __launch_bounds__(64 * kWaves)
     u32x4 x{0, 0, 0, 0};
     vf[u] = x;
     if (live) {
-      x = load_chunk(row_of<T>(a.k, b, hk, key),
+      x = load_chunk<kDirect>(row_of<T>(a.k, b, hk, key),
                      chunk_of_maps<T, kPad>(u * 2 + half, a.D));
       if (kDk)
-        vf[u] = load_chunk(row_of<T>(a.v, b, hk, key),
+        vf[u] = load_chunk<kDirect>(row_of<T>(a.v, b, hk, key),
                            chunk_of_row<T>(u * 2 + half, a.Dv));
     }
     kf[u / S::kSteps][u % S::kSteps] = x;
@@ -400,16 +476,13 @@ __global__ void __launch_bounds__(64 * kWaves)
   const int q_tiles = (a.Q + kTile - 1) / kTile;
   const int steps =
       key_tile * 32 * kWaves < n ? group * q_tiles : 0;
-  Stage<T, S::kWidth, kTile, 64 * kWaves> stage;
-  const int chunk = (int)threadIdx.x % Lds::kChunks;
-  const ChunkOf qc = chunk_of_maps<T, kPad>(chunk, a.D);
-  const ChunkOf gc = chunk_of_row<T>(chunk, a.Dv);
+  Stage<T, S::kWidth, kTile, 64 * kWaves, kDirect> stage;
   float4 st;
-  auto load = [&](int step) {
+  auto load = [&](int step, char* to) {
     const int h = hk * group + step / q_tiles;
     const int q0 = step % q_tiles * kTile;
-    stage.load(row_of<T>(a.q, b, h, 0), a.q.l, qc, row_of<T>(a.dout, b, h, 0),
-               a.dout.l, gc, q0, a.Q);
+    stage.load(row_of<T>(a.q, b, h, 0), a.q.l, row_of<T>(a.dout, b, h, 0),
+               a.dout.l, a.D, a.Dv, q0, a.Q, to, to + kTileBytes);
     const int q = q0 + (int)threadIdx.x;
     // rows that are not there have no weight
     st = float4{-kLowest, -kLowest, 0.f, 0.f};
@@ -417,32 +490,20 @@ __global__ void __launch_bounds__(64 * kWaves)
       st = reinterpret_cast<const float4*>(
           a.stats)[((long)b * a.H + h) * a.Q + q];
   };
-  auto store = [&](int buffer) {
-    stage.store(lds + buffer * 2 * kTileBytes,
-                lds + buffer * 2 * kTileBytes + kTileBytes);
+  auto store = [&](int step, char* to, float (*to_stats)[kTile]) {
+    stage.store(a.Q - step % q_tiles * kTile, to, to + kTileBytes);
     if (threadIdx.x < kTile) {
-      stats[buffer][0][threadIdx.x] = st.x;
-      stats[buffer][1][threadIdx.x] = st.y;
-      stats[buffer][2][threadIdx.x] = st.z;
-      stats[buffer][3][threadIdx.x] = st.w;
+      to_stats[0][threadIdx.x] = st.x;
+      to_stats[1][threadIdx.x] = st.y;
+      to_stats[2][threadIdx.x] = st.z;
+      to_stats[3][threadIdx.x] = st.w;
     }
   };
-  if (steps > 0) {
-    load(0);
-    store(0);
-  }
-  __syncthreads();
-  int buffer = 0;
-  for (int step = 0; step < steps; ++step, buffer ^= 1) {
-    const bool more = step + 1 < steps;
-    if (more) load(step + 1);
+  auto pass = [&](int step, const char* qt, const float (*stats)[kTile]) {
     const float lam = lam_of(a, hk * group + step / q_tiles);
-    const int q0 = step % q_tiles * kTile;
-    const char* qt = lds + buffer * 2 * kTileBytes;
     const char* gt = qt + kTileBytes;
 #pragma unroll
     for (int sub = 0; sub < kTile; sub += 32) {
-      if (q0 + sub >= a.Q) break;
       f32x16 s[2], g{};
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
@@ -462,10 +523,10 @@ __global__ void __launch_bounds__(64 * kWaves)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int at = sub + 8 * r + 4 * half;
-        const f32x4 lse1 = *(const f32x4*)&stats[buffer][0][at];
-        const f32x4 lse2 = *(const f32x4*)&stats[buffer][1][at];
-        const f32x4 d1 = *(const f32x4*)&stats[buffer][2][at];
-        const f32x4 d2 = *(const f32x4*)&stats[buffer][3][at];
+        const f32x4 lse1 = *(const f32x4*)&stats[0][at];
+        const f32x4 lse2 = *(const f32x4*)&stats[1][at];
+        const f32x4 d1 = *(const f32x4*)&stats[2][at];
+        const f32x4 d2 = *(const f32x4*)&stats[3][at];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int i = 4 * r + e;
@@ -500,8 +561,25 @@ __global__ void __launch_bounds__(64 * kWaves)
         }
       }
     }
-    if (more) store(buffer ^ 1);
+  };
+  auto turn = [&](int step, const char* now, const float (*now_stats)[kTile],
+                  char* then, float (*then_stats)[kTile]) {
+    const bool more = step + 1 < steps;
+    if (more) load(step + 1, then);
+    pass(step, now, now_stats);
+    if (more) store(step + 1, then, then_stats);
     __syncthreads();
+  };
+  if (steps > 0) {
+    load(0, even);
+    store(0, even, even_stats);
+  }
+  __syncthreads();
+  for (int step = 0; step < steps;) {
+    turn(step, even, even_stats, odd, odd_stats);
+    if (++step == steps) break;
+    turn(step, odd, odd_stats, even, even_stats);
+    ++step;
   }
 
   if (key >= a.K) return;
@@ -538,81 +616,101 @@ __global__ void __launch_bounds__(64 * kWaves)
   }
 }
 
+// blocks of 4 waves that reach every CU
+constexpr long kManyBlocks = 256;
+
 // -------------------------------- launches -------------------------------- //
 
 template <typename K>
-hipError_t launch(K kernel, long blocks, int threads, int lds,
-                  const NpfDiffAttnArgs& a, hipStream_t stream) {
+hipError_t launch(K kernel, long blocks, int threads, const NpfDiffAttnArgs& a,
+                  hipStream_t stream) {
   if (blocks > 0x7fffffffL) return hipErrorInvalidConfiguration;
-  if (lds > 65536) {
-    const hipError_t e = hipFuncSetAttribute(
-        reinterpret_cast<const void*>(kernel),
-        hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-    if (e != hipSuccess) return e;
-  }
-  kernel<<<(unsigned)blocks, threads, lds, stream>>>(a);
+  kernel<<<(unsigned)blocks, threads, 0, stream>>>(a);
   return hipGetLastError();
 }
 
-template <typename T, int kPad>
+// Blocks of 4 waves share their tiles; where they would not reach every CU,
+// blocks of one wave do.
+template <typename T, int kPad, bool kDirect>
 hipError_t fwd_sized(const NpfDiffAttnArgs& a, hipStream_t stream) {
   using S = Shape<T, kPad>;
   const long heads = (long)a.B * a.Hk, rows = (long)(a.H / a.Hk) * a.Q;
+  const long each = heads * a.splits * S::kParts;
   if (a.waves == 1)
-    return launch(diff_fwd<T, kPad, 1>, heads * ((rows + 31) / 32) * a.splits,
-                  64, 4 * 32 * S::kRowBytes, a, stream);
-  return launch(diff_fwd<T, kPad, 4>, heads * ((rows + 127) / 128) * a.splits,
-                256, 4 * S::kTile * S::kRowBytes, a, stream);
+    return launch(diff_fwd<T, kPad, 1, kDirect>, each * ((rows + 31) / 32), 64,
+                  a, stream);
+  return launch(diff_fwd<T, kPad, 4, kDirect>, each * ((rows + 127) / 128),
+                256, a, stream);
 }
 
-template <typename T, int kPad>
-hipError_t bwd_sized(const NpfDiffAttnArgs& a, hipStream_t stream) {
-  using S = Shape<T, kPad>;
-  const long heads = (long)a.B * a.Hk, rows = (long)(a.H / a.Hk) * a.Q;
-  const int lds = 4 * S::kTile * S::kRowBytes;
-  if (a.dq.p || a.dlam) {
-    const hipError_t e = launch(diff_bwd_dq<T, kPad, 4>,
-                                heads * ((rows + 127) / 128), 256, lds, a,
-                                stream);
-    if (e != hipSuccess) return e;
-  }
-  const long blocks = heads * ((a.K + 127) / 128);
-  const int more = 2 * 4 * S::kTile * (int)sizeof(float);
-  if constexpr (sizeof(T) == 4 && kPad == 128) {
+template <typename T, int kPad, int kWaves, bool kDirect, bool kDk, bool kDv>
+hipError_t dkv_launch(const NpfDiffAttnArgs& a, hipStream_t stream) {
+  const long heads = (long)a.B * a.Hk;
+  return launch(diff_bwd_dkv<T, kPad, kWaves, kDirect, kDk, kDv>,
+                heads * ((a.K + 32 * kWaves - 1) / (32 * kWaves)), 64 * kWaves,
+                a, stream);
+}
+
+template <typename T, int kPad, int kWaves, bool kDirect>
+hipError_t dkv_sized(const NpfDiffAttnArgs& a, hipStream_t stream) {
+  if constexpr (kPad == 128) {
     // both gradients at once would not fit a wave's registers
     if (a.dk.p) {
-      const hipError_t e = launch(diff_bwd_dkv<T, kPad, 4, true, false>, blocks,
-                                  256, lds + more, a, stream);
+      const hipError_t e =
+          dkv_launch<T, kPad, kWaves, kDirect, true, false>(a, stream);
       if (e != hipSuccess) return e;
     }
     if (a.dv.p)
-      return launch(diff_bwd_dkv<T, kPad, 4, false, true>, blocks, 256,
-                    lds + more, a, stream);
+      return dkv_launch<T, kPad, kWaves, kDirect, false, true>(a, stream);
     return hipSuccess;
   } else {
     if (!a.dk.p && !a.dv.p) return hipSuccess;
-    return launch(diff_bwd_dkv<T, kPad, 4, true, true>, blocks, 256, lds + more,
-                  a, stream);
+    return dkv_launch<T, kPad, kWaves, kDirect, true, true>(a, stream);
   }
 }
 
-template <typename T>
-hipError_t fwd_typed(const NpfDiffAttnArgs& a, hipStream_t stream) {
-  switch (a.pad) {
-    case 16: return fwd_sized<T, 16>(a, stream);
-    case 32: return fwd_sized<T, 32>(a, stream);
-    case 64: return fwd_sized<T, 64>(a, stream);
-    default: return fwd_sized<T, 128>(a, stream);
+template <typename T, int kPad, bool kDirect>
+hipError_t bwd_sized(const NpfDiffAttnArgs& a, hipStream_t stream) {
+  const long heads = (long)a.B * a.Hk, rows = (long)(a.H / a.Hk) * a.Q;
+  if (a.dq.p || a.dlam) {
+    const hipError_t e =
+        heads * ((rows + 127) / 128) >= kManyBlocks
+            ? launch(diff_bwd_dq<T, kPad, 4, kDirect>,
+                     heads * ((rows + 127) / 128), 256, a, stream)
+            : launch(diff_bwd_dq<T, kPad, 1, kDirect>, heads * ((rows + 31) / 32),
+                     64, a, stream);
+    if (e != hipSuccess) return e;
   }
+  return heads * ((a.K + 127) / 128) >= kManyBlocks
+             ? dkv_sized<T, kPad, 4, kDirect>(a, stream)
+             : dkv_sized<T, kPad, 1, kDirect>(a, stream);
+}
+
+// whether rows can move to LDS by themselves: no padding, 16-byte aligned
+template <typename T>
+bool direct(const NpfHeads& t) {
+  const long n = kChunk<T>;
+  return reinterpret_cast<size_t>(t.p) % 16 == 0 && t.b % n == 0 &&
+         t.h % n == 0 && t.l % n == 0;
+}
+
+template <typename T, int kPad>
+hipError_t sized(const NpfDiffAttnArgs& a, bool bwd, hipStream_t stream) {
+  if (a.D == kPad && a.Dv == 2 * kPad && direct<T>(a.k) && direct<T>(a.v) &&
+      (!bwd || (direct<T>(a.q) && direct<T>(a.dout))))
+    return bwd ? bwd_sized<T, kPad, true>(a, stream)
+               : fwd_sized<T, kPad, true>(a, stream);
+  return bwd ? bwd_sized<T, kPad, false>(a, stream)
+             : fwd_sized<T, kPad, false>(a, stream);
 }
 
 template <typename T>
-hipError_t bwd_typed(const NpfDiffAttnArgs& a, hipStream_t stream) {
+hipError_t typed(const NpfDiffAttnArgs& a, bool bwd, hipStream_t stream) {
   switch (a.pad) {
-    case 16: return bwd_sized<T, 16>(a, stream);
-    case 32: return bwd_sized<T, 32>(a, stream);
-    case 64: return bwd_sized<T, 64>(a, stream);
-    default: return bwd_sized<T, 128>(a, stream);
+    case 16: return sized<T, 16>(a, bwd, stream);
+    case 32: return sized<T, 32>(a, bwd, stream);
+    case 64: return sized<T, 64>(a, bwd, stream);
+    default: return sized<T, 128>(a, bwd, stream);
   }
 }
 

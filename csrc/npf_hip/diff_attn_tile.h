@@ -23,6 +23,8 @@
 #include "diff_attn.h"
 #include "types.h"
 
+#include <type_traits>
+
 namespace npf_attn {
 
 using f32x16 = __attribute__((ext_vector_type(16))) float;
@@ -180,10 +182,11 @@ __device__ __forceinline__ ChunkOf chunk_of_row(int chunk, int size) {
           left < 0 ? 0 : left > kChunk<T> ? kChunk<T> : left};
 }
 
-template <typename T>
+// kFull: no chunk has padding
+template <bool kFull, typename T>
 __device__ __forceinline__ u32x4 load_chunk(const T* row, ChunkOf c) {
   T v[kChunk<T>];
-  if (c.count == kChunk<T>) {
+  if (kFull || c.count == kChunk<T>) {
     load_pack(v, row + c.offset);
   } else {
 #pragma unroll
@@ -195,10 +198,59 @@ __device__ __forceinline__ u32x4 load_chunk(const T* row, ChunkOf c) {
   return r;
 }
 
-// Two tiles of kRows rows each moving from memory to LDS through registers,
-// so that the loads of the next pair run under the products of this one.
+// Two tiles of kRows rows each on their way from memory to LDS, the next pair
+// under the products of this one.
+//
+// kDirect: rows without padding, 16-byte aligned.  The loads write LDS
+// themselves and hold no registers; a wave's 64 chunks land side by side, so
+// the permutation is in what each lane reads.  Rows behind the end read the
+// last one again: no weight meets them, and what they hold has met a weight
+// where it counts.
+//
+// Otherwise the chunks come through registers, each lane testing its own, and
+// rows behind the end become zeros.
+template <typename T, int kWidth, int kRows, int kThreads, bool kDirect>
+struct Stage;
+
 template <typename T, int kWidth, int kRows, int kThreads>
-struct Stage {
+struct Stage<T, kWidth, kRows, kThreads, true> {
+  using Lds = Tile<T, kWidth>;
+  static constexpr int kCount = kRows * Lds::kChunks / kThreads;
+  static_assert(kRows * Lds::kChunks % kThreads == 0 && Lds::kChunks <= 64);
+
+  __device__ __forceinline__ static void one(const T* p, long l, int row0,
+                                             int end, char* tile) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int j = 0; j < kCount; ++j) {
+      const int first = j * kThreads + wave * 64;  // chunk of lane 0
+      const int row = first / Lds::kChunks + lane / Lds::kChunks;
+      const int chunk = lane % Lds::kChunks ^ Lds::permute(row);
+      const int at = row0 + row < end ? row0 + row : end - 1;
+      __builtin_amdgcn_global_load_lds(
+          (__attribute__((address_space(1))) void*)(p + at * l +
+                                                    chunk * kChunk<T>),
+          (__attribute__((address_space(3))) void*)(tile + first * 16), 16, 0,
+          0);
+    }
+  }
+
+  __device__ __forceinline__ void load(const T* xp, long xl, const T* yp,
+                                       long yl, int, int, int row0, int end,
+                                       char* xt, char* yt) {
+    one(xp, xl, row0, end, xt);
+    one(yp, yl, row0, end, yt);
+  }
+
+  // before the barrier that shows the tiles to every wave
+  __device__ __forceinline__ void store(int, char*, char*) {
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0), the other counters free
+  }
+};
+
+template <typename T, int kWidth, int kRows, int kThreads>
+struct Stage<T, kWidth, kRows, kThreads, false> {
   using Lds = Tile<T, kWidth>;
   static constexpr int kStep = kThreads / Lds::kChunks;  // rows at a time
   static constexpr int kCount = kRows / kStep;
@@ -206,26 +258,31 @@ struct Stage {
 
   u32x4 x[kCount], y[kCount];
 
-  // rows row0 .. of two tensors; rows from `end` on become zeros
-  __device__ __forceinline__ void load(const T* xp, long xl, ChunkOf xc,
-                                       const T* yp, long yl, ChunkOf yc,
-                                       int row0, int end) {
+  __device__ __forceinline__ void load(const T* xp, long xl, const T* yp,
+                                       long yl, int map_size, int row_size,
+                                       int row0, int end, char*, char*) {
+    const int chunk = (int)threadIdx.x % Lds::kChunks;
+    const ChunkOf xc = chunk_of_maps<T, kWidth / 2>(chunk, map_size);
+    const ChunkOf yc = chunk_of_row<T>(chunk, row_size);
     const int first = row0 + (int)threadIdx.x / Lds::kChunks;
 #pragma unroll
     for (int j = 0; j < kCount; ++j) {
       const int row = first + j * kStep;
-      x[j] = u32x4{0, 0, 0, 0};
-      y[j] = u32x4{0, 0, 0, 0};
-      if (row < end) {
-        x[j] = load_chunk(xp + row * xl, xc);
-        y[j] = load_chunk(yp + row * yl, yc);
-      }
+      const int at = row < end ? row : end - 1;
+      x[j] = load_chunk<false>(xp + at * xl, xc);
+      y[j] = load_chunk<false>(yp + at * yl, yc);
     }
   }
 
-  __device__ __forceinline__ void store(char* xt, char* yt) const {
+  // `count` rows of the tiles are there
+  __device__ __forceinline__ void store(int count, char* xt, char* yt) {
     const int first = (int)threadIdx.x / Lds::kChunks;
     const int chunk = (int)threadIdx.x % Lds::kChunks;
+    if (count < kRows) {
+#pragma unroll
+      for (int j = 0; j < kCount; ++j)
+        if (first + j * kStep >= count) x[j] = y[j] = u32x4{0, 0, 0, 0};
+    }
 #pragma unroll
     for (int j = 0; j < kCount; ++j) {
       const int at = Lds::at(first + j * kStep, chunk);

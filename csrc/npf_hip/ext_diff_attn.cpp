@@ -35,7 +35,7 @@ Tensor heads_like(const Tensor& q, int64_t B, int64_t H, int64_t L,
 
 NpfDiffAttnArgs common_args(const Tensor& q, const Tensor& k, const Tensor& v,
                             const Tensor& lam, double scale,
-                            const OptTensor& lengths) {
+                            const Tensor& lengths) {
   check_heads(q, q, "queries");
   check_heads(k, q, "keys");
   check_heads(v, q, "values");
@@ -69,17 +69,17 @@ NpfDiffAttnArgs common_args(const Tensor& q, const Tensor& k, const Tensor& v,
   a.lam_type = npf_type_code(lam, "lam", true);
   a.lam_heads = lam.dim() == 0 ? 1 : a.H;
   a.lam_stride = lam.dim() == 0 ? 0 : (int)lam.stride(0);
-  if (lengths) {
-    TORCH_CHECK_VALUE(lengths->dim() == 1 && lengths->size(0) == a.B &&
-                          lengths->device() == q.device() &&
-                          lengths->is_contiguous(),
-                      "key_lengths must be a contiguous [", a.B,
-                      "] on the GPU of the queries");
-    TORCH_CHECK_TYPE(lengths->scalar_type() == torch::kInt32 ||
-                         lengths->scalar_type() == torch::kInt64,
+  if (lengths.defined()) {
+    TORCH_CHECK_VALUE(lengths.dim() == 1 && lengths.size(0) == a.B &&
+                          lengths.device() == q.device() &&
+                          lengths.is_contiguous(),
+                      "key_lengths must have ", a.B,
+                      " values on the GPU of the queries");
+    TORCH_CHECK_TYPE(lengths.scalar_type() == torch::kInt32 ||
+                         lengths.scalar_type() == torch::kInt64,
                      "key_lengths must be int32 or int64");
-    a.lengths = lengths->data_ptr();
-    a.lengths64 = lengths->scalar_type() == torch::kInt64;
+    a.lengths = lengths.data_ptr();
+    a.lengths64 = lengths.scalar_type() == torch::kInt64;
   }
   a.type = npf_type_code(q, "queries");
   a.scale = (float)scale;
@@ -92,23 +92,21 @@ NpfDiffAttnArgs common_args(const Tensor& q, const Tensor& k, const Tensor& v,
   return a;
 }
 
-// (out, o2, lse); the last two are empty unless `save`
-std::tuple<Tensor, Tensor, Tensor> diff_attn_fwd(
-    const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& lam,
-    double scale, const OptTensor& lengths, bool save) {
+// out, and where `save` the second map's part and the statistics
+Tensor attn_forward(const Tensor& q, const Tensor& k, const Tensor& v,
+                    const Tensor& lam, double scale, const Tensor& lengths,
+                    bool save, Tensor* o2, Tensor* lse) {
   NpfDiffAttnArgs a = common_args(q, k, v, lam, scale, lengths);
-  c10::DeviceGuard guard(q.device());
   Tensor out = heads_like(q, a.B, a.H, a.Q, a.Dv);
-  Tensor o2 = save ? heads_like(q, a.B, a.H, a.Q, a.Dv)
-                   : torch::empty({0}, q.options());
-  Tensor lse = torch::empty({save ? (long)a.B * a.H * a.Q * 2 : 0},
-                            q.options().dtype(torch::kFloat32));
-  if (out.numel() == 0) return {out, o2, lse};
   a.out = heads_of(out);
   if (save) {
-    a.o2 = heads_of(o2);
-    a.lse = lse.data_ptr<float>();
+    *o2 = heads_like(q, a.B, a.H, a.Q, a.Dv);
+    *lse = torch::empty({(long)a.B * a.H * a.Q * 2},
+                        q.options().dtype(torch::kFloat32));
+    a.o2 = heads_of(*o2);
+    a.lse = lse->data_ptr<float>();
   }
+  if (out.numel() == 0) return out;
   Tensor split;
   if (const size_t bytes = npf_diff_attn_workspace(a)) {
     split = torch::empty({(long)bytes}, q.options().dtype(torch::kUInt8));
@@ -116,54 +114,92 @@ std::tuple<Tensor, Tensor, Tensor> diff_attn_fwd(
   }
   npf_check(npf_diff_attn_fwd(a, at::hip::getCurrentHIPStream()),
             "differential_attention");
-  return {out, o2, lse};
+  return out;
 }
 
-// (dq, dk, dv, dlam); those that are not asked for are None
-std::tuple<OptTensor, OptTensor, OptTensor, OptTensor> diff_attn_bwd(
-    const Tensor& dout, const Tensor& q, const Tensor& k, const Tensor& v,
-    const Tensor& lam, const Tensor& out, const Tensor& o2, const Tensor& lse,
-    double scale, const OptTensor& lengths, bool need_dq, bool need_dk,
-    bool need_dv, bool need_dlam) {
-  NpfDiffAttnArgs a = common_args(q, k, v, lam, scale, lengths);
-  check_heads(dout, q, "dout");
-  TORCH_CHECK_VALUE(dout.sizes() == out.sizes() && o2.sizes() == out.sizes(),
-                    "dout must have the shape of the output");
-  c10::DeviceGuard guard(q.device());
-  OptTensor dq, dk, dv, dlam;
-  if (need_dq) dq = heads_like(q, a.B, a.H, a.Q, 2 * a.D);
-  if (need_dk) dk = heads_like(k, a.B, a.Hk, a.K, 2 * a.D);
-  if (need_dv) dv = heads_like(v, a.B, a.Hk, a.K, a.Dv);
-  if (need_dlam) dlam = torch::empty(lam.sizes(), lam.options());
-  if (out.numel() == 0 || a.K == 0) {
-    for (OptTensor* t : {&dq, &dk, &dv, &dlam})
-      if (*t) (*t)->zero_();
-    return {dq, dk, dv, dlam};
+// along the last axis the kernels take contiguous values alone
+Tensor as_heads(const Tensor& t) {
+  return t.size(-1) == 1 || t.stride(-1) == 1 ? t : t.contiguous();
+}
+
+struct DiffAttn : torch::autograd::Function<DiffAttn> {
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& k,
+                        const Tensor& q, const Tensor& v, const Tensor& lam,
+                        const OptTensor& lengths_, double scale) {
+    const Tensor lengths = lengths_.value_or(Tensor());
+    Tensor o2, lse;
+    Tensor out =
+        attn_forward(q, k, v, lam, scale, lengths, true, &o2, &lse);
+    ctx->saved_data["needs"] =
+        (int64_t)(k.requires_grad() + 2 * q.requires_grad() +
+                  4 * v.requires_grad() + 8 * lam.requires_grad());
+    ctx->saved_data["scale"] = scale;
+    ctx->save_for_backward({k, q, v, lam, lengths, out, o2, lse});
+    return out;
   }
-  auto f32 = q.options().dtype(torch::kFloat32);
-  const long rows = (long)a.B * a.H * a.Q;
-  Tensor stats = torch::empty({rows, 4}, f32);
-  Tensor dlam_rows = torch::empty({rows}, f32);
-  a.out = heads_of(out);
-  a.o2 = heads_of(o2);
-  a.dout = heads_of(dout);
-  a.lse = lse.data_ptr<float>();
-  a.stats = stats.data_ptr<float>();
-  a.dlam_rows = dlam_rows.data_ptr<float>();
-  if (dq) a.dq = heads_of(*dq);
-  if (dk) a.dk = heads_of(*dk);
-  if (dv) a.dv = heads_of(*dv);
-  if (dlam) a.dlam = dlam->data_ptr();
-  npf_check(npf_diff_attn_bwd(a, at::hip::getCurrentHIPStream()),
-            "differential_attention backward");
-  return {dq, dk, dv, dlam};
+
+  static torch::autograd::variable_list backward(
+      torch::autograd::AutogradContext* ctx,
+      torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const int64_t needs = ctx->saved_data["needs"].toInt();
+    const Tensor &k = saved[0], &q = saved[1], &v = saved[2], &lam = saved[3],
+                 &lengths = saved[4], &out = saved[5], &o2 = saved[6],
+                 &lse = saved[7];
+    c10::DeviceGuard guard(q.device());
+    NpfDiffAttnArgs a = common_args(q, k, v, lam,
+                                    ctx->saved_data["scale"].toDouble(),
+                                    lengths);
+    const Tensor dout = as_heads(grads[0]);
+    check_heads(dout, q, "dout");
+    Tensor dk, dq, dv, dlam;
+    if (needs & 1) dk = heads_like(k, a.B, a.Hk, a.K, 2 * a.D);
+    if (needs & 2) dq = heads_like(q, a.B, a.H, a.Q, 2 * a.D);
+    if (needs & 4) dv = heads_like(v, a.B, a.Hk, a.K, a.Dv);
+    if (needs & 8) dlam = torch::empty(lam.sizes(), lam.options());
+    if (out.numel() == 0 || a.K == 0) {
+      for (Tensor* t : {&dk, &dq, &dv, &dlam})
+        if (t->defined()) t->zero_();
+    } else {
+      const long rows = (long)a.B * a.H * a.Q;
+      Tensor stats = torch::empty({rows, 4}, lse.options());
+      Tensor dlam_rows = torch::empty({rows}, lse.options());
+      a.out = heads_of(out);
+      a.o2 = heads_of(o2);
+      a.dout = heads_of(dout);
+      a.lse = lse.data_ptr<float>();
+      a.stats = stats.data_ptr<float>();
+      a.dlam_rows = dlam_rows.data_ptr<float>();
+      if (dq.defined()) a.dq = heads_of(dq);
+      if (dk.defined()) a.dk = heads_of(dk);
+      if (dv.defined()) a.dv = heads_of(dv);
+      if (dlam.defined()) a.dlam = dlam.data_ptr();
+      npf_check(npf_diff_attn_bwd(a, at::hip::getCurrentHIPStream()),
+                "differential_attention backward");
+    }
+    return npf_once({dk, dq, dv, dlam, Tensor(), Tensor()},
+                    "differential_attention");
+  }
+};
+
+Tensor differential_attention(const Tensor& k_, const Tensor& q_,
+                              const Tensor& v_, const Tensor& lam, double scale,
+                              const OptTensor& lengths_) {
+  const Tensor k = as_heads(k_), q = as_heads(q_), v = as_heads(v_);
+  OptTensor lengths;
+  if (lengths_) lengths = lengths_->contiguous();
+  c10::DeviceGuard guard(q.device());
+  if (at::GradMode::is_enabled() &&
+      (k.requires_grad() || q.requires_grad() || v.requires_grad() ||
+       lam.requires_grad()))
+    return DiffAttn::apply(k, q, v, lam, lengths, scale);
+  return attn_forward(q, k, v, lam, scale, lengths.value_or(Tensor()), false,
+                      nullptr, nullptr);
 }
 
 }  // namespace
 
 void npf_bind_diff_attn(pybind11::module_& m) {
-  m.def("diff_attn_fwd", &diff_attn_fwd,
-        "differential attention forward -> (out, o2, lse)");
-  m.def("diff_attn_bwd", &diff_attn_bwd,
-        "differential attention backward -> (dq, dk, dv, dlam)");
+  m.def("differential_attention", &differential_attention,
+        "difference of two softmax maps times the values");
 }

@@ -15,114 +15,163 @@ namespace {
 using torch::Tensor;
 using OptTensor = std::optional<Tensor>;
 
-void* ptr_of(const OptTensor& t) { return t ? t->data_ptr() : nullptr; }
+void* ptr_of(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
-void check_rows(const Tensor& t, const Tensor& like, const char* name) {
-  TORCH_CHECK_VALUE(t.dim() == 2 && t.sizes() == like.sizes(), name,
-                    " must have the shape ", like.sizes(), ", has ",
-                    t.sizes());
-  TORCH_CHECK_VALUE(t.device() == like.device(), name, " must be on ",
-                    like.device());
-  TORCH_CHECK_TYPE(t.scalar_type() == like.scalar_type(), name,
-                   " must have type ", like.scalar_type());
-  TORCH_CHECK_VALUE(t.size(1) < 2 || t.stride(1) == 1, name,
-                    " must have contiguous rows");
+OptTensor some(const Tensor& t) {
+  return t.defined() ? OptTensor(t) : OptTensor();
 }
 
-void check_columns(const OptTensor& t, const Tensor& x, const char* name) {
-  if (!t) return;
-  TORCH_CHECK_VALUE(t->dim() == 1 && t->size(0) == x.size(1) &&
-                        t->is_contiguous() && t->device() == x.device(),
-                    name, " must be a contiguous [", x.size(1), "] on ",
+// [..., D] as [rows, D] with contiguous rows; copied only where no stride
+// describes the rows
+Tensor rows_of(const Tensor& t) {
+  if (!t.defined()) return t;
+  Tensor r = t.dim() == 2 ? t : t.reshape({-1, t.size(-1)});
+  return r.size(1) == 1 || r.stride(1) == 1 ? r : r.contiguous();
+}
+
+void check_like(const Tensor& t, const Tensor& x, const char* name) {
+  TORCH_CHECK_VALUE(t.sizes() == x.sizes(), name, " must have the shape ",
+                    x.sizes(), ", has ", t.sizes());
+  TORCH_CHECK_VALUE(t.device() == x.device(), name, " must be on ",
+                    x.device());
+  TORCH_CHECK_TYPE(t.scalar_type() == x.scalar_type(), name,
+                   " must have type ", x.scalar_type());
+}
+
+void check_columns(const Tensor& t, const Tensor& x, const char* name) {
+  TORCH_CHECK_VALUE(t.dim() == 1 && t.size(0) == x.size(-1) &&
+                        t.device() == x.device(),
+                    name, " must have ", x.size(-1), " values on ",
                     x.device());
 }
 
-NpfLayerNormArgs norm_args(const Tensor& x, const OptTensor& residual,
-                           const OptTensor& weight, const OptTensor& bias) {
-  TORCH_CHECK_VALUE(x.is_cuda() && x.dim() == 2 && x.size(1) > 0,
-                    "layer_norm takes rows of at least one value on a GPU");
-  TORCH_CHECK_VALUE(x.size(1) <= std::numeric_limits<int>::max(),
-                    "layer_norm: rows are too wide");
-  check_rows(x, x, "x");
-  if (residual) check_rows(*residual, x, "residual");
-  check_columns(weight, x, "weight");
-  check_columns(bias, x, "bias");
-  TORCH_CHECK_TYPE(!weight || !bias ||
-                       weight->scalar_type() == bias->scalar_type(),
-                   "weight and bias must have the same type");
+// The rows (x, residual as rows_of leaves them), weight and bias contiguous;
+// residual, weight and bias may be undefined.
+NpfLayerNormArgs norm_args(const Tensor& x, const Tensor& residual,
+                           const Tensor& weight, const Tensor& bias) {
   NpfLayerNormArgs a{};
   a.x = x.data_ptr();
   a.residual = ptr_of(residual);
   a.weight = ptr_of(weight);
   a.bias = ptr_of(bias);
   a.x_stride = x.stride(0);
-  a.residual_stride = residual ? residual->stride(0) : 0;
+  a.residual_stride = residual.defined() ? residual.stride(0) : 0;
   a.rows = x.size(0);
   a.width = (int)x.size(1);
-  const OptTensor& w = weight ? weight : bias;
-  a.weight_type = w ? npf_type_code(*w, "weight", true) : (int)NPF_F32;
+  const Tensor& w = weight.defined() ? weight : bias;
+  a.weight_type = w.defined() ? npf_type_code(w, "weight", true) : (int)NPF_F32;
   return a;
 }
 
-// (y, mean, rstd); the last two are empty unless `save`
-std::tuple<Tensor, Tensor, Tensor> layer_norm_fwd(
-    const Tensor& x, const OptTensor& residual, const OptTensor& weight,
-    const OptTensor& bias, double eps, bool save) {
+// mean and rstd are filled where they are defined
+void layer_norm_forward(const Tensor& x, const Tensor& residual,
+                        const Tensor& weight, const Tensor& bias, double eps,
+                        Tensor& y, const Tensor& mean, const Tensor& rstd) {
   NpfLayerNormArgs a = norm_args(x, residual, weight, bias);
-  const int type = npf_type_code(x, "x");
-  c10::DeviceGuard guard(x.device());
-  Tensor y = torch::empty({x.size(0), x.size(1)}, x.options());
-  auto f32 = x.options().dtype(torch::kFloat32);
-  Tensor mean = torch::empty({save ? x.size(0) : 0}, f32);
-  Tensor rstd = torch::empty({save ? x.size(0) : 0}, f32);
-  if (a.rows == 0) return {y, mean, rstd};
+  if (a.rows == 0) return;
   a.y = y.data_ptr();
-  a.mean = save ? mean.data_ptr<float>() : nullptr;
-  a.rstd = save ? rstd.data_ptr<float>() : nullptr;
+  a.mean = static_cast<float*>(ptr_of(mean));
+  a.rstd = static_cast<float*>(ptr_of(rstd));
   a.eps = (float)eps;
-  npf_check(npf_layernorm_fwd(a, type, at::hip::getCurrentHIPStream()),
+  npf_check(npf_layernorm_fwd(a, npf_type_code(x, "x"),
+                              at::hip::getCurrentHIPStream()),
             "layer_norm");
-  return {y, mean, rstd};
 }
 
-// (dx, dweight, dbias); those that are not asked for are None
-std::tuple<OptTensor, OptTensor, OptTensor> layer_norm_bwd(
-    const Tensor& dy, const Tensor& x, const OptTensor& residual,
-    const OptTensor& weight, const OptTensor& bias, const Tensor& mean,
-    const Tensor& rstd, bool need_dx, bool need_dweight, bool need_dbias) {
-  NpfLayerNormArgs a = norm_args(x, residual, weight, bias);
-  const int type = npf_type_code(x, "x");
-  check_rows(dy, x, "dy");
-  TORCH_CHECK_VALUE(dy.is_contiguous(), "dy must be contiguous");
-  TORCH_CHECK_VALUE(mean.numel() == x.size(0) && rstd.numel() == x.size(0),
-                    "mean and rstd must hold one value a row");
-  need_dweight = need_dweight && weight;
-  need_dbias = need_dbias && bias;
+struct LayerNorm : torch::autograd::Function<LayerNorm> {
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x,
+                        const OptTensor& residual_, const OptTensor& weight_,
+                        const OptTensor& bias_, double eps) {
+    const Tensor residual = residual_.value_or(Tensor());
+    const Tensor weight = weight_.value_or(Tensor());
+    const Tensor bias = bias_.value_or(Tensor());
+    const Tensor xr = rows_of(x), rr = rows_of(residual);
+    Tensor y = torch::empty(x.sizes(), x.options());
+    auto f32 = x.options().dtype(torch::kFloat32);
+    const Tensor mean = torch::empty({xr.size(0)}, f32);
+    const Tensor rstd = torch::empty({xr.size(0)}, f32);
+    layer_norm_forward(xr, rr, weight, bias, eps, y, mean, rstd);
+    auto needs = [](const Tensor& t) { return t.defined() && t.requires_grad(); };
+    ctx->saved_data["needs"] =
+        (int64_t)(needs(x) + 2 * needs(residual) + 4 * needs(weight) +
+                  8 * needs(bias));
+    ctx->save_for_backward({xr, rr, weight, bias, mean, rstd});
+    return y;
+  }
+
+  static torch::autograd::variable_list backward(
+      torch::autograd::AutogradContext* ctx,
+      torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const int64_t needs = ctx->saved_data["needs"].toInt();
+    const Tensor &x = saved[0], &residual = saved[1], &weight = saved[2],
+                 &bias = saved[3], &mean = saved[4], &rstd = saved[5];
+    c10::DeviceGuard guard(x.device());
+    NpfLayerNormArgs a = norm_args(x, residual, weight, bias);
+    const Tensor dy = grads[0].contiguous();
+    Tensor dx, dweight, dbias, partial;
+    if (needs & 3) dx = torch::empty(dy.sizes(), dy.options());
+    if (needs & 4) dweight = torch::empty_like(weight);
+    if (needs & 8) dbias = torch::empty_like(bias);
+    if (a.rows == 0) {
+      if (dweight.defined()) dweight.zero_();
+      if (dbias.defined()) dbias.zero_();
+    } else {
+      const int type = npf_type_code(x, "x");
+      if (needs & 12) {
+        a.parts = npf_layernorm_parts(a, type);
+        partial = torch::empty({a.parts, 2, x.size(1)}, mean.options());
+        a.partial = partial.data_ptr<float>();
+      }
+      a.dy = dy.data_ptr();
+      a.y = ptr_of(dx);
+      a.mean = mean.data_ptr<float>();
+      a.rstd = rstd.data_ptr<float>();
+      a.dweight = ptr_of(dweight);
+      a.dbias = ptr_of(dbias);
+      npf_check(npf_layernorm_bwd(a, type, at::hip::getCurrentHIPStream()),
+                "layer_norm backward");
+    }
+    return npf_once(
+        {needs & 1 ? dx : Tensor(), needs & 2 ? dx : Tensor(), dweight, dbias,
+         Tensor()},
+        "layer_norm");
+  }
+};
+
+Tensor layer_norm(const Tensor& x, const OptTensor& residual_,
+                  const OptTensor& weight_, const OptTensor& bias_,
+                  double eps) {
+  TORCH_CHECK_VALUE(x.is_cuda() && x.dim() >= 1 && x.size(-1) > 0,
+                    "layer_norm takes rows of at least one value on a GPU");
+  TORCH_CHECK_VALUE(x.size(-1) <= std::numeric_limits<int>::max() / 2,
+                    "layer_norm: rows are too wide");
+  npf_type_code(x, "x");
+  const Tensor residual = residual_.value_or(Tensor());
+  Tensor weight = weight_.value_or(Tensor()), bias = bias_.value_or(Tensor());
+  if (residual.defined()) check_like(residual, x, "residual");
+  if (weight.defined()) {
+    check_columns(weight, x, "weight");
+    weight = weight.contiguous();
+  }
+  if (bias.defined()) {
+    check_columns(bias, x, "bias");
+    bias = bias.contiguous();
+  }
+  TORCH_CHECK_TYPE(!weight.defined() || !bias.defined() ||
+                       weight.scalar_type() == bias.scalar_type(),
+                   "weight and bias must have the same type");
   c10::DeviceGuard guard(x.device());
-  OptTensor dx, dweight, dbias, partial;
-  if (need_dx) dx = torch::empty({x.size(0), x.size(1)}, x.options());
-  if (a.rows == 0) {
-    if (need_dweight) dweight = torch::zeros_like(*weight);
-    if (need_dbias) dbias = torch::zeros_like(*bias);
-    return {dx, dweight, dbias};
-  }
-  if (need_dweight) dweight = torch::empty_like(*weight);
-  if (need_dbias) dbias = torch::empty_like(*bias);
-  if (need_dweight || need_dbias) {
-    a.parts = npf_layernorm_parts(a, type);
-    partial = torch::empty({a.parts, 2, x.size(1)},
-                           x.options().dtype(torch::kFloat32));
-    a.partial = partial->data_ptr<float>();
-  }
-  a.dy = dy.data_ptr();
-  a.y = ptr_of(dx);
-  a.mean = mean.data_ptr<float>();
-  a.rstd = rstd.data_ptr<float>();
-  a.dweight = ptr_of(dweight);
-  a.dbias = ptr_of(dbias);
-  npf_check(npf_layernorm_bwd(a, type, at::hip::getCurrentHIPStream()),
-            "layer_norm backward");
-  return {dx, dweight, dbias};
+  if (at::GradMode::is_enabled())
+    for (const Tensor* t : {&x, &residual, (const Tensor*)&weight,
+                            (const Tensor*)&bias})
+      if (t->defined() && t->requires_grad())
+        return LayerNorm::apply(x, some(residual), some(weight), some(bias),
+                                eps);
+  Tensor y = torch::empty(x.sizes(), x.options());
+  layer_norm_forward(rows_of(x), rows_of(residual), weight, bias, eps, y,
+                     Tensor(), Tensor());
+  return y;
 }
 
 int norm_code(double p) {
@@ -236,9 +285,7 @@ Tensor grad_norm(const std::vector<Tensor>& grads, double norm_type,
 }  // namespace
 
 void npf_bind_norms(pybind11::module_& m) {
-  m.def("layer_norm_fwd", &layer_norm_fwd, "layer norm forward");
-  m.def("layer_norm_bwd", &layer_norm_bwd,
-        "layer norm backward -> (dx, dweight, dbias)");
+  m.def("layer_norm", &layer_norm, "layer norm over the last axis");
   m.def("grad_norm", &grad_norm,
         "norm of many gradients; max_norm >= 0 clips them in place");
 }
