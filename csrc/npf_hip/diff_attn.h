@@ -15,11 +15,14 @@ struct NpfDiffAttnArgs {
   NpfHeads dq, dk, dv;    // backward; null where not asked for
   float* lse;             // [B, H, Q, 2]: log2 of each map's sum of exponents
   float* stats;           // backward: [B, H, Q, 4]: lse_1, lse_2, delta_1, _2
-  float* dlam_rows;       // backward: [B, H, Q]
+  float* dlam_rows;       // backward: [dq_splits, B, H, Q]
   void* dlam;             // backward: [lam_heads], or null
   const void* lam;
   const void* lengths;    // [B] int32 or int64, or null
   void* split;            // forward: workspace of a split key axis
+  float* dq_part;         // backward: parts of a split sum, [dq_splits, B, H,
+  float* dk_part;         // Q, 2D] and [dkv_splits, B, Hk, K, 2D or Dv], where
+  float* dv_part;         // there are several
   float scale;
   int B, H, Hk, Q, K, D, Dv;
   int type, lam_type, lam_stride;
@@ -28,12 +31,14 @@ struct NpfDiffAttnArgs {
   // the plan
   int pad;     // D and Dv / 2 are padded to this
   int waves;   // of a forward block
-  int splits;  // parts of the key axis
+  int splits;  // parts of the key axis, forward
+  int dq_splits;   // parts of the key axis, and of the query axis, backward
+  int dkv_splits;
 };
 
 // fills the plan; false where no kernel covers the sizes
 bool npf_diff_attn_plan(NpfDiffAttnArgs&);
-// bytes of `split`
-size_t npf_diff_attn_workspace(const NpfDiffAttnArgs&);
+// floats of `split`
+long npf_diff_attn_workspace(const NpfDiffAttnArgs&);
 hipError_t npf_diff_attn_fwd(const NpfDiffAttnArgs&, hipStream_t);
 hipError_t npf_diff_attn_bwd(const NpfDiffAttnArgs&, hipStream_t);

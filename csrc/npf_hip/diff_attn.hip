@@ -14,7 +14,8 @@ namespace {
 
 using namespace npf_attn;
 
-// one block a row: 4 slices of the splits, each over both maps' values
+// Join of a split forward pass.  Many splits (few rows): one block a row, 4
+// slices of the splits, each over both maps' values.
 constexpr int kJoinThreads = 1024;
 
 template <typename T>
@@ -69,6 +70,87 @@ __global__ void __launch_bounds__(kJoinThreads) join(NpfDiffAttnArgs a) {
         any ? top[t] + __log2f(weight_sum[t]) : 0.f;
 }
 
+// Few splits (many rows): kLanes lanes of 4 values a row.
+template <typename T, int kLanes>
+__global__ void __launch_bounds__(256) join_rows(NpfDiffAttnArgs a) {
+  const unsigned rows = (unsigned)a.B * a.H * a.Q;
+  const unsigned r = blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
+  if (r >= rows) return;
+  const unsigned each = (unsigned)(a.H / a.Hk) * a.Q;
+  const int row = (int)(r % each), bh = (int)(r / each);
+  const int b = bh / a.Hk;
+  const int h = bh % a.Hk * (a.H / a.Hk) + row / a.Q, q = row % a.Q;
+  const int c = (threadIdx.x % kLanes) * 4;
+  const int count = a.Dv - c < 4 ? a.Dv - c : 4;
+  const long step = split_row_floats(a.Dv);
+  const float* w = static_cast<const float*>(a.split) + (long)r * a.splits * step;
+  float mx[2] = {kLowest, kLowest}, l[2] = {0.f, 0.f}, o[2][4] = {};
+  for (int s = 0; s < a.splits; ++s)
+    for (int m = 0; m < 2; ++m) mx[m] = fmaxf(mx[m], w[s * step + 2 * m]);
+  for (int s = 0; s < a.splits; ++s)
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      const float* p = w + s * step;
+      const float f = exp2f(p[2 * m] - mx[m]);
+      l[m] += f * p[2 * m + 1];
+      float v[4] = {};
+      if (count == 4)
+        load_pack(v, p + 4 + m * a.Dv + c);
+      else
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (i < count) v[i] = p[4 + m * a.Dv + c + i];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[m][i] += f * v[i];
+    }
+  const bool any = keys_of(a, b) > 0;
+  const float lam = lam_of(a, h);
+  float x[4], y[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    y[i] = any ? o[1][i] / l[1] : 0.f;
+    x[i] = any ? o[0][i] / l[0] - lam * y[i] : 0.f;
+  }
+  if (count > 0) {
+    store4(row_of<T>(a.out, b, h, q) + c, count, x[0], x[1], x[2], x[3]);
+    if (a.o2.p)
+      store4(row_of<T>(a.o2, b, h, q) + c, count, y[0], y[1], y[2], y[3]);
+  }
+  if (a.lse && c == 0) {
+    float* p = a.lse + (((long)b * a.H + h) * a.Q + q) * 2;
+    for (int m = 0; m < 2; ++m) p[m] = any ? mx[m] + __log2f(l[m]) : 0.f;
+  }
+}
+
+// Sum of the parts of a split gradient, in their order: rows of `size` values.
+template <typename T, int kLanes>
+__global__ void __launch_bounds__(256)
+    join_grads(NpfHeads out, const float* part, int B, int H, int L, int size,
+               int splits) {
+  const unsigned rows = (unsigned)B * H * L;
+  const unsigned r = blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
+  if (r >= rows) return;
+  const int l = (int)(r % (unsigned)L), bh = (int)(r / (unsigned)L);
+  const int c = (threadIdx.x % kLanes) * 4;
+  const int count = size - c < 4 ? size - c : 4;
+  if (count <= 0) return;
+  float x[4] = {};
+#pragma unroll 4
+  for (int s = 0; s < splits; ++s) {
+    const float* p = part + ((long)s * rows + r) * size + c;
+    float v[4] = {};
+    if (count == 4)
+      load_pack(v, p);
+    else
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (i < count) v[i] = p[i];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] += v[i];
+  }
+  store4(row_of<T>(out, bh / H, bh % H, l) + c, count, x[0], x[1], x[2], x[3]);
+}
+
 // delta_i of each row, beside its lse: kLanes lanes of 4 values a row
 template <typename T, int kLanes>
 __global__ void __launch_bounds__(256) row_stats(NpfDiffAttnArgs a) {
@@ -92,11 +174,13 @@ __global__ void __launch_bounds__(256) row_stats(NpfDiffAttnArgs a) {
       load_pack(o, op);
       load_pack(s, sp);
     } else {
-      for (int i = 0; c + i < a.Dv; ++i) {
-        g[i] = gp[i];
-        o[i] = op[i];
-        s[i] = sp[i];
-      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (c + i < a.Dv) {
+          g[i] = gp[i];
+          o[i] = op[i];
+          s[i] = sp[i];
+        }
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -119,10 +203,12 @@ __global__ void __launch_bounds__(1024) sum_dlam(NpfDiffAttnArgs a,
                                                  int heads) {
   __shared__ double smem[1024];
   double s = 0.;
-  const long per = (long)heads * a.Q;
+  // (sizes are checked to fit 31 bits)
+  const unsigned per = (unsigned)heads * a.Q;
+  const unsigned all = (unsigned)a.dq_splits * a.B * per;
 #pragma unroll 4
-  for (long i = threadIdx.x; i < a.B * per; i += 1024)
-    s += a.dlam_rows[(i / per * a.H + blockIdx.x * heads) * a.Q + i % per];
+  for (unsigned i = threadIdx.x; i < all; i += 1024)
+    s += a.dlam_rows[(long)(i / per * a.H + blockIdx.x * heads) * a.Q + i % per];
   smem[threadIdx.x] = s;
   __syncthreads();
   for (int n = 512; n > 0; n >>= 1) {
@@ -132,20 +218,72 @@ __global__ void __launch_bounds__(1024) sum_dlam(NpfDiffAttnArgs a,
   if (threadIdx.x == 0) store_coded(a.dlam, a.lam_type, blockIdx.x, -smem[0]);
 }
 
-template <typename T>
-void launch_row_stats(const NpfDiffAttnArgs& a, hipStream_t stream) {
-  const long rows = (long)a.B * a.H * a.Q;
-  auto blocks = [&](int lanes) {
-    return (unsigned)((rows * lanes + 255) / 256);
-  };
-  if (a.Dv <= 32)
-    row_stats<T, 8><<<blocks(8), 256, 0, stream>>>(a);
-  else if (a.Dv <= 64)
-    row_stats<T, 16><<<blocks(16), 256, 0, stream>>>(a);
-  else if (a.Dv <= 128)
-    row_stats<T, 32><<<blocks(32), 256, 0, stream>>>(a);
+// lanes of 4 values for a row of `size`, as a compile-time number
+template <typename F>
+void with_lanes(int size, F f) {
+  if (size <= 32)
+    f(std::integral_constant<int, 8>{});
+  else if (size <= 64)
+    f(std::integral_constant<int, 16>{});
+  else if (size <= 128)
+    f(std::integral_constant<int, 32>{});
   else
-    row_stats<T, 64><<<blocks(64), 256, 0, stream>>>(a);
+    f(std::integral_constant<int, 64>{});
+}
+
+unsigned row_blocks(long rows, int lanes) {
+  return (unsigned)((rows * lanes + 255) / 256);
+}
+
+// whether a split pass has so many parts that a block joins one row
+bool many(int splits) { return splits > 8; }
+
+template <typename T>
+hipError_t join_forward(const NpfDiffAttnArgs& a, hipStream_t stream) {
+  const long rows = (long)a.B * a.H * a.Q;
+  if (many(a.splits))
+    join<T><<<(unsigned)rows, kJoinThreads, 0, stream>>>(a);
+  else
+    with_lanes(a.Dv, [&](auto lanes) {
+      join_rows<T, lanes()>
+          <<<row_blocks(rows, lanes()), 256, 0, stream>>>(a);
+    });
+  return hipGetLastError();
+}
+
+template <typename T>
+void stats(const NpfDiffAttnArgs& a, hipStream_t stream) {
+  with_lanes(a.Dv, [&](auto lanes) {
+    row_stats<T, lanes()>
+        <<<row_blocks((long)a.B * a.H * a.Q, lanes()), 256, 0, stream>>>(a);
+  });
+}
+
+template <typename T>
+void join_one(const NpfHeads& out, const float* part, int B, int H, int L,
+              int size, int splits, hipStream_t stream) {
+  if (!out.p || splits == 1) return;
+  with_lanes(size, [&](auto lanes) {
+    join_grads<T, lanes()><<<row_blocks((long)B * H * L, lanes()), 256, 0,
+                             stream>>>(out, part, B, H, L, size, splits);
+  });
+}
+
+template <typename T>
+hipError_t join_backward(const NpfDiffAttnArgs& a, hipStream_t stream) {
+  join_one<T>(a.dq, a.dq_part, a.B, a.H, a.Q, 2 * a.D, a.dq_splits, stream);
+  join_one<T>(a.dk, a.dk_part, a.B, a.Hk, a.K, 2 * a.D, a.dkv_splits, stream);
+  join_one<T>(a.dv, a.dv_part, a.B, a.Hk, a.K, a.Dv, a.dkv_splits, stream);
+  return hipGetLastError();
+}
+
+// Parts of an axis of `length` so that `blocks` of 4 waves become two a CU;
+// none shorter than `least`, whose work would not pay for the join.
+int parts_for(long blocks, long wanted, int length, int least) {
+  if (blocks <= 0 || 2 * blocks > wanted) return 1;
+  const long most = length / least;
+  const long n = wanted / blocks;
+  return (int)(n < most ? (n < 1 ? 1 : n) : (most < 1 ? 1 : most));
 }
 
 }  // namespace
@@ -155,23 +293,25 @@ bool npf_diff_attn_plan(NpfDiffAttnArgs& a) {
     if (a.pad == 128) return false;
   const long rows = (long)(a.H / a.Hk) * a.Q;
   const long heads = (long)a.B * a.Hk;
-  a.waves = heads * ((rows + 127) / 128) >= kManyBlocks ? 4 : 1;
-  // Few rows: the key axis is split until every SIMD has a wave, no part
-  // below 256 keys.
-  const long waves = heads * ((rows + 31) / 32);
-  const long most = (a.K + 255) / 256;
-  long splits = a.waves == 1 && waves > 0 && waves < 512 ? 1280 / waves : 1;
-  splits = splits > most ? most : splits;
-  a.splits = (int)(splits < 1 ? 1 : splits);
+  // Rows that fit one wave get a block of one wave, the others share tiles
+  // between four.
+  a.waves = rows <= 32 ? 1 : 4;
+  const long row_blocks4 = heads * ((rows + 127) / 128);
+  a.splits = a.waves == 1 ? parts_for(heads, 1280, a.K, 256)
+                          : parts_for(row_blocks4, 512, a.K, 512);
+  a.dq_splits = parts_for(row_blocks4, 512, a.K, 256);
+  a.dkv_splits =
+      parts_for(heads * ((a.K + 127) / 128), 512, (int)rows, 256);
   return true;
 }
 
-size_t npf_diff_attn_workspace(const NpfDiffAttnArgs& a) {
+long npf_diff_attn_workspace(const NpfDiffAttnArgs& a) {
   if (a.splits <= 1) return 0;
-  return sizeof(float) * a.splits * split_row_floats(a.Dv) * a.B * a.H * a.Q;
+  return split_row_floats(a.Dv) * a.splits * a.B * a.H * a.Q;
 }
 
 hipError_t npf_diff_attn_fwd(const NpfDiffAttnArgs& a, hipStream_t stream) {
+  if ((long)a.B * a.H * a.Q > 0x7fffffffL) return hipErrorInvalidConfiguration;
   hipError_t e = hipErrorInvalidValue;
   switch (a.type) {
     case NPF_F32: e = npf_diff_attn_fwd_f32(a, stream); break;
@@ -179,31 +319,33 @@ hipError_t npf_diff_attn_fwd(const NpfDiffAttnArgs& a, hipStream_t stream) {
     case NPF_F16: e = npf_diff_attn_fwd_f16(a, stream); break;
   }
   if (e != hipSuccess || a.splits <= 1) return e;
-  const long rows = (long)a.B * a.H * a.Q;
-  if (rows > 0x7fffffffL) return hipErrorInvalidConfiguration;
   switch (a.type) {
-    case NPF_F32: join<float><<<(unsigned)rows, kJoinThreads, 0, stream>>>(a); break;
-    case NPF_BF16: join<npf_bf16><<<(unsigned)rows, kJoinThreads, 0, stream>>>(a); break;
-    default: join<npf_f16><<<(unsigned)rows, kJoinThreads, 0, stream>>>(a);
+    case NPF_F32: return join_forward<float>(a, stream);
+    case NPF_BF16: return join_forward<npf_bf16>(a, stream);
+    default: return join_forward<npf_f16>(a, stream);
   }
-  return hipGetLastError();
 }
 
 hipError_t npf_diff_attn_bwd(const NpfDiffAttnArgs& a, hipStream_t stream) {
-  if ((long)a.B * a.H * a.Q > 0x7fffffffL) return hipErrorInvalidConfiguration;
+  if ((long)a.dq_splits * a.B * a.H * a.Q > 0x7fffffffL ||
+      (long)a.B * a.Hk * a.K > 0x7fffffffL)
+    return hipErrorInvalidConfiguration;
   hipError_t e = hipErrorInvalidValue;
   switch (a.type) {
     case NPF_F32:
-      launch_row_stats<float>(a, stream);
+      stats<float>(a, stream);
       e = npf_diff_attn_bwd_f32(a, stream);
+      if (e == hipSuccess) e = join_backward<float>(a, stream);
       break;
     case NPF_BF16:
-      launch_row_stats<npf_bf16>(a, stream);
+      stats<npf_bf16>(a, stream);
       e = npf_diff_attn_bwd_bf16(a, stream);
+      if (e == hipSuccess) e = join_backward<npf_bf16>(a, stream);
       break;
     case NPF_F16:
-      launch_row_stats<npf_f16>(a, stream);
+      stats<npf_f16>(a, stream);
       e = npf_diff_attn_bwd_f16(a, stream);
+      if (e == hipSuccess) e = join_backward<npf_f16>(a, stream);
       break;
   }
   if (e != hipSuccess || !a.dlam) return e;

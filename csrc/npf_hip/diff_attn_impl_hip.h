@@ -26,6 +26,12 @@ struct Shape {
   static constexpr int kTile = kRowBytes <= 256 ? 64 : 32;
   // tiles of 32 that a wave takes through a pass at once
   static constexpr int kSubs = kPad <= 32 ? 2 : 1;
+  // whether a wave's registers hold both gradients of its keys; else each has
+  // a launch of its own, at two waves a SIMD rather than one (bf16, 2 x 16 x
+  // 4096 x 4096, maps of 64: see the table of measurements)
+  static constexpr bool kBothGrads = kPad * (int)sizeof(T) < 128;
+  // whether the dq kernel keeps its queries in LDS rather than in registers
+  static constexpr bool kQueriesInLds = sizeof(T) == 2 && kPad == 64;
   // parts of the values' columns that forward blocks take: the sums of 256
   // columns for two maps would fill a wave's registers by themselves
   static constexpr int kParts = kPad == 128 ? 2 : 1;
@@ -37,7 +43,7 @@ struct Shape {
 // Waves a SIMD is to hold: two, in half of the registers each and with every
 // matrix result in ordinary registers, where a kernel fits; else one.
 template <typename T, int kPad>
-constexpr int kResident = kPad * (int)sizeof(T) <= 64 ? 2 : 1;
+constexpr int kResident = kPad * (int)sizeof(T) <= 128 ? 2 : 1;
 
 // Columns that block n of map m starts at.  Maps of 16 share one block: each
 // accumulates it whole and keeps its half.
@@ -110,7 +116,7 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, kPad>))
       const ChunkOf c =
           chunk_of_maps<T, kPad>((m * S::kSteps + u) * 2 + half, a.D);
       qf[m][u] = u32x4{0, 0, 0, 0};
-      if (live) qf[m][u] = load_chunk<kDirect>(row_of<T>(a.q, b, h, q), c);
+      if (live) qf[m][u] = load_chunk(row_of<T>(a.q, b, h, q), c);
     }
 
   f32x16 o[2][kCols];
@@ -124,10 +130,14 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, kPad>))
   Stage<T, S::kWidth, kTile, 64 * kWaves, kDirect> stage;
   const T* kp = row_of<T>(a.k, b, hk, 0);
   const T* vp = row_of<T>(a.v, b, hk, 0);
+  // the columns that this block's part begins with, in bytes of a row
+  const int part_cols = part * kCols * 32 * (int)sizeof(T);
   // one tile from LDS; kEdge: it may reach behind the last key
+  const int rows_base = Lds::rows_base(lane), cols_base = Lds::cols_base(lane);
   auto pass = [&](auto edge, int k0, const char* kt) {
     constexpr bool kEdge = decltype(edge)::value;
     const char* vt = kt + kTileBytes;
+    const int rb = fresh(rows_base), cb = fresh(cols_base);
 #pragma unroll
     for (int sub0 = 0; sub0 < kTile; sub0 += 32 * kSubs) {
       if (kEdge && k0 + sub0 >= end) break;
@@ -140,9 +150,8 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, kPad>))
 #pragma unroll
           for (int u = 0; u < S::kSteps; ++u)
             s[m][t] = mma_chunk<T>(
-                Lds::rows(kt, sub0 + 32 * t + col,
-                          (m * S::kSteps + u) * 2 + half),
-                qf[m][u], s[m][t]);
+                Lds::rows(kt, rb, sub0 + 32 * t, m * S::kSteps + u), qf[m][u],
+                s[m][t]);
         }
       if constexpr (kEdge) {
 #pragma unroll
@@ -180,8 +189,8 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, kPad>))
 #pragma unroll
         for (int j = 0; j < kCols; ++j) {
           f32x16* const acc[2] = {&o[0][j], &o[1][j]};
-          Lds::template transposed<2>(vt, sub0 + 32 * t,
-                                      32 * (part * kCols + j), lane, p, acc);
+          Lds::template transposed<2>(vt, cb ^ part_cols, sub0 + 32 * t, 32 * j,
+                                      p, acc);
         }
       }
     }
@@ -195,6 +204,9 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, kPad>))
     if (next < end) stage.store(end - next, then, then + kTileBytes);
     __syncthreads();
   };
+  stage.clear(a.D, a.Dv, even);
+  stage.clear(a.D, a.Dv, odd);
+  __syncthreads();
   if (begin < end) {
     stage.load(kp, a.k.l, vp, a.v.l, a.D, a.Dv, begin, end, even,
                even + kTileBytes);
@@ -275,38 +287,54 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, kPad>))
     diff_bwd_dq(NpfDiffAttnArgs a) {
   using S = Shape<T, kPad>;
   using Lds = Tile<T, S::kWidth>;
-  constexpr int kTile = kWaves == 1 ? 32 * S::kSubs : S::kTile;
+  constexpr bool kInLds = S::kQueriesInLds;
+  constexpr int kTile = kWaves == 1 || kInLds ? 32 * S::kSubs : S::kTile;
   constexpr int kSubs = S::kSubs;
   constexpr int kTileBytes = kTile * S::kRowBytes;
   // two objects, so that it shows that the next tiles' loads do not touch
   // what is being read
   __shared__ __attribute__((aligned(16))) char even[2 * kTileBytes];
   __shared__ __attribute__((aligned(16))) char odd[2 * kTileBytes];
+  __shared__ __attribute__((
+      aligned(16))) char held[kInLds ? 32 * kWaves * S::kRowBytes : 16];
 
   const int group = a.H / a.Hk, rows = group * a.Q;
   const int row_tiles = (rows + 32 * kWaves - 1) / (32 * kWaves);
-  const int row_tile = blockIdx.x % row_tiles, bh = blockIdx.x / row_tiles;
+  int id = blockIdx.x;
+  const int split = id % a.dq_splits;
+  id /= a.dq_splits;
+  const int row_tile = id % row_tiles, bh = id / row_tiles;
   const int b = bh / a.Hk, hk = bh % a.Hk;
   const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
   const int row = (row_tile * kWaves + (threadIdx.x >> 6)) * 32 + col;
   const bool live = row < rows;
   const int h = hk * group + (live ? row / a.Q : 0);
   const int q = live ? row % a.Q : 0;
-  const int n = keys_of(a, b);
+  int begin = 0, n = keys_of(a, b);  // this split's keys
+  if (a.dq_splits > 1) {
+    const int per = split_keys(n, a.dq_splits, kTile);
+    begin = split * per < n ? split * per : n;
+    n = n - begin < per ? n : begin + per;
+  }
   const long stat = ((long)b * a.H + h) * a.Q + q;
 
-  u32x4 qf[2][S::kSteps], gf[2 * S::kSteps];
+  const int rows_base = Lds::rows_base(lane), cols_base = Lds::cols_base(lane);
+  char* own = held + (kInLds ? (threadIdx.x >> 6) * 32 * S::kRowBytes : 0);
+  u32x4 qf[kInLds ? 1 : 2 * S::kSteps], gf[2 * S::kSteps];
 #pragma unroll
   for (int u = 0; u < 2 * S::kSteps; ++u) {
     u32x4 x{0, 0, 0, 0};
     gf[u] = x;
     if (live) {
-      x = load_chunk<kDirect>(row_of<T>(a.q, b, h, q),
+      x = load_chunk(row_of<T>(a.q, b, h, q),
                      chunk_of_maps<T, kPad>(u * 2 + half, a.D));
-      gf[u] = load_chunk<kDirect>(row_of<T>(a.dout, b, h, q),
+      gf[u] = load_chunk(row_of<T>(a.dout, b, h, q),
                          chunk_of_row<T>(u * 2 + half, a.Dv));
     }
-    qf[u / S::kSteps][u % S::kSteps] = x;
+    if constexpr (kInLds)  // read by the lanes that write it alone
+      *reinterpret_cast<u32x4*>(own + (rows_base ^ (u << 5))) = x;
+    else
+      qf[u] = x;
   }
   float4 st = {0.f, 0.f, 0.f, 0.f};
   if (live) st = reinterpret_cast<const float4*>(a.stats)[stat];
@@ -325,59 +353,56 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, kPad>))
   auto pass = [&](auto edge, int k0, const char* kt) {
     constexpr bool kEdge = decltype(edge)::value;
     const char* vt = kt + kTileBytes;
+    const int rb = fresh(rows_base), cb = fresh(cols_base);
 #pragma unroll
     for (int sub0 = 0; sub0 < kTile; sub0 += 32 * kSubs) {
       if (kEdge && k0 + sub0 >= n) break;
-      f32x16 s[2][kSubs], g[kSubs];
+      f32x16 g[kSubs];
 #pragma unroll
       for (int t = 0; t < kSubs; ++t) {
-        const int sub = sub0 + 32 * t;
-#pragma unroll
-        for (int m = 0; m < 2; ++m) {
-          s[m][t] = f32x16{};
-#pragma unroll
-          for (int u = 0; u < S::kSteps; ++u)
-            s[m][t] = mma_chunk<T>(
-                Lds::rows(kt, sub + col, (m * S::kSteps + u) * 2 + half),
-                qf[m][u], s[m][t]);
-        }
         g[t] = f32x16{};
 #pragma unroll
         for (int u = 0; u < 2 * S::kSteps; ++u)
-          g[t] = mma_chunk<T>(Lds::rows(vt, sub + col, u * 2 + half), gf[u],
-                              g[t]);
+          g[t] = mma_chunk<T>(Lds::rows(vt, rb, sub0 + 32 * t, u), gf[u], g[t]);
       }
-      if constexpr (kEdge) {
+      if (kSubs == 1) __builtin_amdgcn_sched_barrier(0);
+      // one map after the other: a second tile of scores would not fit
 #pragma unroll
-        for (int t = 0; t < kSubs; ++t)
+      for (int m = 0; m < 2; ++m) {
+        f32x16 s[kSubs];
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (k0 + sub0 + 32 * t + reg_row(i) + 4 * half >= n)
-              s[0][t][i] = s[1][t][i] = -INFINITY;
-      }
+        for (int t = 0; t < kSubs; ++t) {
+          s[t] = f32x16{};
 #pragma unroll
-      for (int t = 0; t < kSubs; ++t) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float gi = g[t][i];
-          const float p1 = __builtin_amdgcn_exp2f(
-              __builtin_fmaf(s[0][t][i], c, -st.x));
-          const float p2 = __builtin_amdgcn_exp2f(
-              __builtin_fmaf(s[1][t][i], c, -st.y));
-          dlam = __builtin_fmaf(p2, gi, dlam);
-          s[0][t][i] = p1 * (gi - st.z);
-          s[1][t][i] = p2 * (gi - st.w) * -lam;
+          for (int u = m * S::kSteps; u < (m + 1) * S::kSteps; ++u) {
+            u32x4 x;
+            if constexpr (kInLds)
+              x = Lds::rows(own, rb, 0, u);
+            else
+              x = qf[u];
+            s[t] = mma_chunk<T>(Lds::rows(kt, rb, sub0 + 32 * t, u), x, s[t]);
+          }
         }
+        const float lse = m ? st.y : st.x, delta = m ? st.w : st.z;
 #pragma unroll
-        for (int m = 0; m < 2; ++m) {
-          const Operand<T> ds[1] = {Operand<T>(s[m][t])};
+        for (int t = 0; t < kSubs; ++t) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i], c, -lse));
+            if (kEdge && k0 + sub0 + 32 * t + reg_row(i) + 4 * half >= n)
+              p = 0.f;
+            if (m) dlam = __builtin_fmaf(p, g[t][i], dlam);
+            s[t][i] = p * (g[t][i] - delta);
+          }
+          const Operand<T> ds[1] = {Operand<T>(s[t])};
 #pragma unroll
           for (int j = 0; j < S::kMapBlocks; ++j) {
             f32x16* const acc[1] = {&dq[m][j]};
-            Lds::template transposed<1>(kt, sub0 + 32 * t, map_col<kPad>(m, j),
-                                        lane, ds, acc);
+            Lds::template transposed<1>(kt, cb, sub0 + 32 * t,
+                                        map_col<kPad>(m, j), ds, acc);
           }
         }
+        if (kSubs == 1) __builtin_amdgcn_sched_barrier(0);
       }
     }
   };
@@ -390,14 +415,17 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, kPad>))
     if (next < n) stage.store(n - next, then, then + kTileBytes);
     __syncthreads();
   };
-  if (0 < n) {
-    stage.load(kp, a.k.l, vp, a.v.l, a.D, a.Dv, 0, n, even,
+  stage.clear(a.D, a.Dv, even);
+  stage.clear(a.D, a.Dv, odd);
+  __syncthreads();
+  if (begin < n) {
+    stage.load(kp, a.k.l, vp, a.v.l, a.D, a.Dv, begin, n, even,
                even + kTileBytes);
-    stage.store(n, even, even + kTileBytes);
+    stage.store(n - begin, even, even + kTileBytes);
   }
   __syncthreads();
-  const int full = (n) / kTile;
-  int k0 = 0;
+  const int full = (n - begin) / kTile;
+  int k0 = begin;
   for (int t = 0; t < full;) {
     step(k0, even, odd);
     k0 += kTile;
@@ -410,9 +438,11 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, kPad>))
 
   dlam = both_sum(dlam);
   if (!live) return;
-  if (half == 0) a.dlam_rows[stat] = dlam;
+  const long part = (long)split * a.B * a.H * a.Q + stat;
+  if (half == 0) a.dlam_rows[part] = dlam;
   if (!a.dq.p) return;
   T* out = row_of<T>(a.dq, b, h, q);
+  float* sum = a.dq_part + part * 2 * a.D;
 #pragma unroll
   for (int m = 0; m < 2; ++m)
 #pragma unroll
@@ -421,9 +451,13 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, kPad>))
       for (int g = 0; g < 4; ++g) {
         if (kPad == 16 && g / 2 != m) continue;
         const int d = (kPad == 16 ? 8 * (g % 2) : 32 * j + 8 * g) + 4 * half;
-        const f32x16 x = dq[m][j] * a.scale;
-        store4(out + m * a.D + d, a.D - d, x[4 * g], x[4 * g + 1],
-               x[4 * g + 2], x[4 * g + 3]);
+        const f32x16 x = dq[m][j] * (m ? -lam * a.scale : a.scale);
+        if (a.dq_splits > 1)
+          store4(sum + m * a.D + d, a.D - d, x[4 * g], x[4 * g + 1],
+                 x[4 * g + 2], x[4 * g + 3]);
+        else
+          store4(out + m * a.D + d, a.D - d, x[4 * g], x[4 * g + 1],
+                 x[4 * g + 2], x[4 * g + 3]);
       }
 }
 
@@ -434,7 +468,7 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, kPad>))
     diff_bwd_dkv(NpfDiffAttnArgs a) {
   using S = Shape<T, kPad>;
   using Lds = Tile<T, S::kWidth>;
-  constexpr int kTile = kWaves == 1 ? 32 : S::kTile;
+  constexpr int kTile = kDk && !S::kBothGrads ? 32 : S::kTile;
   constexpr int kTileBytes = kTile * S::kRowBytes;
   // two objects, so that it shows that the next tiles' loads do not touch
   // what is being read
@@ -446,27 +480,31 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, kPad>))
 
   const int group = a.H / a.Hk;
   const int key_tiles = (a.K + 32 * kWaves - 1) / (32 * kWaves);
-  const int key_tile = blockIdx.x % key_tiles, bh = blockIdx.x / key_tiles;
+  int id = blockIdx.x;
+  const int split = id % a.dkv_splits;
+  id /= a.dkv_splits;
+  const int key_tile = id % key_tiles, bh = id / key_tiles;
   const int b = bh / a.Hk, hk = bh % a.Hk;
   const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
   const int key = (key_tile * kWaves + (threadIdx.x >> 6)) * 32 + col;
   const int n = keys_of(a, b);
   const bool live = key < n;
   const float c = a.scale * kLog2e;
+  const int rows_base = Lds::rows_base(lane), cols_base = Lds::cols_base(lane);
 
   u32x4 kf[2][S::kSteps], vf[2 * S::kSteps];
 #pragma unroll
   for (int u = 0; u < 2 * S::kSteps; ++u) {
-    u32x4 x{0, 0, 0, 0};
-    vf[u] = x;
+    u32x4 x{0, 0, 0, 0}, y{0, 0, 0, 0};
     if (live) {
-      x = load_chunk<kDirect>(row_of<T>(a.k, b, hk, key),
-                     chunk_of_maps<T, kPad>(u * 2 + half, a.D));
+      x = load_chunk(row_of<T>(a.k, b, hk, key),
+                              chunk_of_maps<T, kPad>(u * 2 + half, a.D));
       if (kDk)
-        vf[u] = load_chunk<kDirect>(row_of<T>(a.v, b, hk, key),
-                           chunk_of_row<T>(u * 2 + half, a.Dv));
+        y = load_chunk(row_of<T>(a.v, b, hk, key),
+                                chunk_of_row<T>(u * 2 + half, a.Dv));
     }
     kf[u / S::kSteps][u % S::kSteps] = x;
+    vf[u] = y;
   }
   f32x16 dk[2][S::kMapBlocks], dv[S::kBlocks];
 #pragma unroll
@@ -474,14 +512,20 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, kPad>))
 #pragma unroll
   for (int j = 0; j < S::kBlocks; ++j) dv[j] = f32x16{};
 
-  // (head, tile) pairs in one sequence; none where the block has no keys
+  // (head, tile) pairs in one sequence, this split's part of it; none where
+  // the block has no keys
   const int q_tiles = (a.Q + kTile - 1) / kTile;
-  const int steps =
-      key_tile * 32 * kWaves < n ? group * q_tiles : 0;
+  const int per = (group * q_tiles + a.dkv_splits - 1) / a.dkv_splits;
+  const int step0 = split * per;
+  int steps = group * q_tiles;
+  steps = steps - step0 < per ? steps : step0 + per;
+  if (key_tile * 32 * kWaves >= n) steps = 0;
   Stage<T, S::kWidth, kTile, 64 * kWaves, kDirect> stage;
   float4 st;
+  float lam = 0.f, next_lam = 0.f;
   auto load = [&](int step, char* to) {
     const int h = hk * group + step / q_tiles;
+    next_lam = lam_of(a, h);
     const int q0 = step % q_tiles * kTile;
     stage.load(row_of<T>(a.q, b, h, 0), a.q.l, row_of<T>(a.dout, b, h, 0),
                a.dout.l, a.D, a.Dv, q0, a.Q, to, to + kTileBytes);
@@ -501,63 +545,63 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, kPad>))
       to_stats[3][threadIdx.x] = st.w;
     }
   };
-  auto pass = [&](int step, const char* qt, const float (*stats)[kTile]) {
-    const float lam = lam_of(a, hk * group + step / q_tiles);
+  auto pass = [&](const char* qt, const float (*stats)[kTile]) {
     const char* gt = qt + kTileBytes;
+    const int rb = fresh(rows_base), cb = fresh(cols_base);
 #pragma unroll
     for (int sub = 0; sub < kTile; sub += 32) {
-      f32x16 s[2], g{};
+      f32x16 p[2], x;
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
-        s[m] = f32x16{};
+        p[m] = f32x16{};
 #pragma unroll
         for (int u = 0; u < S::kSteps; ++u)
-          s[m] = mma_chunk<T>(
-              Lds::rows(qt, sub + col, (m * S::kSteps + u) * 2 + half),
-              kf[m][u], s[m]);
-      }
-      if (kDk) {
+          p[m] = mma_chunk<T>(Lds::rows(qt, rb, sub, m * S::kSteps + u),
+                              kf[m][u], p[m]);
 #pragma unroll
-        for (int u = 0; u < 2 * S::kSteps; ++u)
-          g = mma_chunk<T>(Lds::rows(gt, sub + col, u * 2 + half), vf[u], g);
-      }
-      f32x16 map;
+        for (int r = 0; r < 4; ++r) {
+          const f32x4 lse = *(const f32x4*)&stats[m][sub + 8 * r + 4 * half];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int at = sub + 8 * r + 4 * half;
-        const f32x4 lse1 = *(const f32x4*)&stats[0][at];
-        const f32x4 lse2 = *(const f32x4*)&stats[1][at];
-        const f32x4 d1 = *(const f32x4*)&stats[2][at];
-        const f32x4 d2 = *(const f32x4*)&stats[3][at];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int i = 4 * r + e;
-          const float p1 =
-              __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][i], c, -lse1[e]));
-          const float p2 =
-              __builtin_amdgcn_exp2f(__builtin_fmaf(s[1][i], c, -lse2[e])) *
-              lam;
-          map[i] = p1 - p2;
-          s[0][i] = p1 * (g[i] - d1[e]);
-          s[1][i] = p2 * (d2[e] - g[i]);
+          for (int e = 0; e < 4; ++e) {
+            float y = __builtin_amdgcn_exp2f(
+                __builtin_fmaf(p[m][4 * r + e], c, -lse[e]));
+            if (m) y *= lam;
+            p[m][4 * r + e] = y;
+          }
         }
       }
       if (kDv) {
-        const Operand<T> p[1] = {Operand<T>(map)};
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] = p[0][i] - p[1][i];
+        const Operand<T> map[1] = {Operand<T>(x)};
 #pragma unroll
         for (int j = 0; j < S::kBlocks; ++j) {
           f32x16* const acc[1] = {&dv[j]};
-          Lds::template transposed<1>(gt, sub, 32 * j, lane, p, acc);
+          Lds::template transposed<1>(gt, cb, sub, 32 * j, map, acc);
         }
       }
       if (kDk) {
+        x = f32x16{};
+#pragma unroll
+        for (int u = 0; u < 2 * S::kSteps; ++u)
+          x = mma_chunk<T>(Lds::rows(gt, rb, sub, u), vf[u], x);
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
-          const Operand<T> ds[1] = {Operand<T>(s[m])};
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const f32x4 d =
+                *(const f32x4*)&stats[2 + m][sub + 8 * r + 4 * half];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int i = 4 * r + e;
+              p[m][i] *= m ? d[e] - x[i] : x[i] - d[e];
+            }
+          }
+          const Operand<T> ds[1] = {Operand<T>(p[m])};
 #pragma unroll
           for (int j = 0; j < S::kMapBlocks; ++j) {
             f32x16* const acc[1] = {&dk[m][j]};
-            Lds::template transposed<1>(qt, sub, map_col<kPad>(m, j), lane, ds,
+            Lds::template transposed<1>(qt, cb, sub, map_col<kPad>(m, j), ds,
                                         acc);
           }
         }
@@ -567,17 +611,21 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, kPad>))
   auto turn = [&](int step, const char* now, const float (*now_stats)[kTile],
                   char* then, float (*then_stats)[kTile]) {
     const bool more = step + 1 < steps;
+    lam = next_lam;
     if (more) load(step + 1, then);
-    pass(step, now, now_stats);
+    pass(now, now_stats);
     if (more) store(step + 1, then, then_stats);
     __syncthreads();
   };
-  if (steps > 0) {
-    load(0, even);
-    store(0, even, even_stats);
+  stage.clear(a.D, a.Dv, even);
+  stage.clear(a.D, a.Dv, odd);
+  __syncthreads();
+  if (step0 < steps) {
+    load(step0, even);
+    store(step0, even, even_stats);
   }
   __syncthreads();
-  for (int step = 0; step < steps;) {
+  for (int step = step0; step < steps;) {
     turn(step, even, even_stats, odd, odd_stats);
     if (++step == steps) break;
     turn(step, odd, odd_stats, even, even_stats);
@@ -586,8 +634,10 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, kPad>))
 
   if (key >= a.K) return;
   // keys behind the last one take no part, whatever their lanes hold
+  const long part = ((long)split * a.B * a.Hk + bh) * a.K + key;
   if (kDk && a.dk.p) {
     T* out = row_of<T>(a.dk, b, hk, key);
+    float* sum = a.dk_part + part * 2 * a.D;
 #pragma unroll
     for (int m = 0; m < 2; ++m)
 #pragma unroll
@@ -600,11 +650,15 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, kPad>))
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             x[e] = live ? dk[m][j][4 * g + e] * a.scale : 0.f;
-          store4(out + m * a.D + d, a.D - d, x[0], x[1], x[2], x[3]);
+          if (a.dkv_splits > 1)
+            store4(sum + m * a.D + d, a.D - d, x[0], x[1], x[2], x[3]);
+          else
+            store4(out + m * a.D + d, a.D - d, x[0], x[1], x[2], x[3]);
         }
   }
   if (kDv && a.dv.p) {
     T* out = row_of<T>(a.dv, b, hk, key);
+    float* sum = a.dv_part + part * a.Dv;
 #pragma unroll
     for (int j = 0; j < S::kBlocks; ++j)
 #pragma unroll
@@ -613,13 +667,13 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, kPad>))
         float x[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) x[e] = live ? dv[j][4 * g + e] : 0.f;
-        store4(out + d, a.Dv - d, x[0], x[1], x[2], x[3]);
+        if (a.dkv_splits > 1)
+          store4(sum + d, a.Dv - d, x[0], x[1], x[2], x[3]);
+        else
+          store4(out + d, a.Dv - d, x[0], x[1], x[2], x[3]);
       }
   }
 }
-
-// blocks of 4 waves that reach every CU
-constexpr long kManyBlocks = 256;
 
 // -------------------------------- launches -------------------------------- //
 
@@ -631,8 +685,6 @@ hipError_t launch(K kernel, long blocks, int threads, const NpfDiffAttnArgs& a,
   return hipGetLastError();
 }
 
-// Blocks of 4 waves share their tiles; where they would not reach every CU,
-// blocks of one wave do.
 template <typename T, int kPad, bool kDirect>
 hipError_t fwd_sized(const NpfDiffAttnArgs& a, hipStream_t stream) {
   using S = Shape<T, kPad>;
@@ -645,60 +697,40 @@ hipError_t fwd_sized(const NpfDiffAttnArgs& a, hipStream_t stream) {
                 256, a, stream);
 }
 
-template <typename T, int kPad, int kWaves, bool kDirect, bool kDk, bool kDv>
-hipError_t dkv_launch(const NpfDiffAttnArgs& a, hipStream_t stream) {
-  const long heads = (long)a.B * a.Hk;
-  return launch(diff_bwd_dkv<T, kPad, kWaves, kDirect, kDk, kDv>,
-                heads * ((a.K + 32 * kWaves - 1) / (32 * kWaves)), 64 * kWaves,
-                a, stream);
-}
-
-template <typename T, int kPad, int kWaves, bool kDirect>
-hipError_t dkv_sized(const NpfDiffAttnArgs& a, hipStream_t stream) {
-  if constexpr (kPad == 128) {
-    // both gradients at once would not fit a wave's registers
-    if (a.dk.p) {
-      const hipError_t e =
-          dkv_launch<T, kPad, kWaves, kDirect, true, false>(a, stream);
-      if (e != hipSuccess) return e;
-    }
-    if (a.dv.p)
-      return dkv_launch<T, kPad, kWaves, kDirect, false, true>(a, stream);
-    return hipSuccess;
-  } else {
-    if (!a.dk.p && !a.dv.p) return hipSuccess;
-    return dkv_launch<T, kPad, kWaves, kDirect, true, true>(a, stream);
-  }
-}
-
 template <typename T, int kPad, bool kDirect>
 hipError_t bwd_sized(const NpfDiffAttnArgs& a, hipStream_t stream) {
   const long heads = (long)a.B * a.Hk, rows = (long)(a.H / a.Hk) * a.Q;
-  if (a.dq.p || a.dlam) {
-    const hipError_t e =
-        heads * ((rows + 127) / 128) >= kManyBlocks
-            ? launch(diff_bwd_dq<T, kPad, 4, kDirect>,
-                     heads * ((rows + 127) / 128), 256, a, stream)
-            : launch(diff_bwd_dq<T, kPad, 1, kDirect>, heads * ((rows + 31) / 32),
-                     64, a, stream);
-    if (e != hipSuccess) return e;
+  hipError_t e = hipSuccess;
+  if (a.dq.p || a.dlam)
+    e = launch(diff_bwd_dq<T, kPad, 4, kDirect>,
+               heads * a.dq_splits * ((rows + 127) / 128), 256, a, stream);
+  const long blocks = heads * a.dkv_splits * ((a.K + 127) / 128);
+  if constexpr (Shape<T, kPad>::kBothGrads) {
+    if (e == hipSuccess && (a.dk.p || a.dv.p))
+      e = launch(diff_bwd_dkv<T, kPad, 4, kDirect, true, true>, blocks, 256, a,
+                 stream);
+  } else {
+    if (e == hipSuccess && a.dk.p)
+      e = launch(diff_bwd_dkv<T, kPad, 4, kDirect, true, false>, blocks, 256, a,
+                 stream);
+    if (e == hipSuccess && a.dv.p)
+      e = launch(diff_bwd_dkv<T, kPad, 4, kDirect, false, true>, blocks, 256, a,
+                 stream);
   }
-  return heads * ((a.K + 127) / 128) >= kManyBlocks
-             ? dkv_sized<T, kPad, 4, kDirect>(a, stream)
-             : dkv_sized<T, kPad, 1, kDirect>(a, stream);
+  return e;
 }
 
-// whether rows can move to LDS by themselves: no padding, 16-byte aligned
+// whether rows can move to LDS by themselves: 16-byte aligned
 template <typename T>
 bool direct(const NpfHeads& t) {
   const long n = kChunk<T>;
   return reinterpret_cast<size_t>(t.p) % 16 == 0 && t.b % n == 0 &&
-         t.h % n == 0 && t.l % n == 0;
+         t.h % n == 0 && t.l % n == 0 && t.l < (1 << 24);
 }
 
 template <typename T, int kPad>
 hipError_t sized(const NpfDiffAttnArgs& a, bool bwd, hipStream_t stream) {
-  if (a.D == kPad && a.Dv == 2 * kPad && direct<T>(a.k) && direct<T>(a.v) &&
+  if (a.D % kChunk<T> == 0 && a.Dv % kChunk<T> == 0 && direct<T>(a.k) && direct<T>(a.v) &&
       (!bwd || (direct<T>(a.q) && direct<T>(a.dout))))
     return bwd ? bwd_sized<T, kPad, true>(a, stream)
                : fwd_sized<T, kPad, true>(a, stream);

@@ -97,6 +97,13 @@ struct Operand<float> {
 
 // -------------------------------- tiles ---------------------------------- //
 
+// A value the compiler is to compute with anew: the many addresses that follow
+// from it would otherwise be kept over a loop, each in a register.
+__device__ __forceinline__ int fresh(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
 template <typename T, int kWidth>
 struct Tile {
   static constexpr int kRowBytes = kWidth * (int)sizeof(T);
@@ -112,30 +119,48 @@ struct Tile {
     return row * kRowBytes + ((chunk ^ permute(row)) << 4);
   }
 
-  // one chunk a lane: row `row0 + lane % 32`, chunk `chunk`
-  __device__ static __forceinline__ u32x4 rows(const char* tile, int row,
-                                               int chunk) {
-    return *reinterpret_cast<const u32x4*>(tile + at(row, chunk));
+  // Where a lane reads along rows: its row of 32, its half's chunk 0.  The
+  // chunks of a row, and the 32-row blocks of a tile, are then constants away
+  // (XOR for the former).
+  __device__ static __forceinline__ int rows_base(int lane) {
+    return at(lane & 31, lane >> 5);
+  }
+  // chunk 2 pair + half of row row0 + lane % 32
+  __device__ static __forceinline__ u32x4 rows(const char* tile, int base,
+                                               int row0, int pair) {
+    return *reinterpret_cast<const u32x4*>(tile + row0 * kRowBytes +
+                                           (base ^ (pair << 5)));
+  }
+
+  // where a lane reads against rows
+  __device__ static __forceinline__ int cols_base(int lane) {
+    const int half = lane >> 5;
+    if constexpr (sizeof(T) == 2) {
+      // lane j of 16 names 4 values of row j / 4, and gets 4 rows of column j
+      const int j = lane & 15;
+      return at(4 * half + (j >> 2), 2 * ((lane >> 4) & 1) + ((j & 3) >> 1)) +
+             (j & 1) * 8;
+    } else {
+      const int col = lane & 31;
+      return at(4 * half, col >> 2) + (col & 3) * 4;
+    }
   }
 
   // acc[lane % 32 of columns col0 ..][column of p] += tile^T p over the 32
   // rows from row0 on, for both maps' p at once
   template <int kMaps>
   __device__ static __forceinline__ void transposed(
-      const char* tile, int row0, int col0, int lane,
-      const Operand<T> (&p)[kMaps], f32x16* const (&acc)[kMaps]) {
-    const int half = lane >> 5;
+      const char* tile, int base, int row0, int col0, const Operand<T> (&p)[kMaps],
+      f32x16* const (&acc)[kMaps]) {
     if constexpr (sizeof(T) == 2) {
-      const int j = lane & 15;
-      // lane j of 16 names 4 values of row j / 4, and gets 4 rows of column j
-      const int chunk = col0 / 8 + 2 * ((lane >> 4) & 1) + ((j & 3) >> 1);
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         s16x4 part[2];
 #pragma unroll
         for (int a = 0; a < 2; ++a) {
-          const int row = row0 + 16 * t + 8 * a + 4 * half + (j >> 2);
-          const char* src = tile + at(row, chunk) + (j & 1) * 8;
+          // rows 16 t + 8 a + ...: 8 rows on, bit 1 of the permutation flips
+          const char* src = tile + (row0 + 16 * t + 8 * a) * kRowBytes +
+                            (base ^ (permute(8 * a) << 4) ^ (col0 << 1));
           part[a] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
               (__attribute__((address_space(3))) s16x4*)(src));
         }
@@ -146,12 +171,11 @@ struct Tile {
         for (int m = 0; m < kMaps; ++m) *acc[m] = mma(v, p[m].v[t], *acc[m]);
       }
     } else {
-      const int col = col0 + (lane & 31);
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const int row = row0 + reg_row(i) + 4 * half;
         const float v = *reinterpret_cast<const float*>(
-            tile + at(row, col >> 2) + (col & 3) * 4);
+            tile + (row0 + reg_row(i)) * kRowBytes +
+            (base ^ (permute(reg_row(i)) << 4) ^ (col0 << 2)));
 #pragma unroll
         for (int m = 0; m < kMaps; ++m) *acc[m] = mma(v, p[m].v[i], *acc[m]);
       }
@@ -182,11 +206,10 @@ __device__ __forceinline__ ChunkOf chunk_of_row(int chunk, int size) {
           left < 0 ? 0 : left > kChunk<T> ? kChunk<T> : left};
 }
 
-// kFull: no chunk has padding
-template <bool kFull, typename T>
+template <typename T>
 __device__ __forceinline__ u32x4 load_chunk(const T* row, ChunkOf c) {
   T v[kChunk<T>];
-  if (kFull || c.count == kChunk<T>) {
+  if (c.count == kChunk<T>) {
     load_pack(v, row + c.offset);
   } else {
 #pragma unroll
@@ -201,11 +224,12 @@ __device__ __forceinline__ u32x4 load_chunk(const T* row, ChunkOf c) {
 // Two tiles of kRows rows each on their way from memory to LDS, the next pair
 // under the products of this one.
 //
-// kDirect: rows without padding, 16-byte aligned.  The loads write LDS
+// kDirect: 16-byte aligned rows of whole chunks.  The loads write LDS
 // themselves and hold no registers; a wave's 64 chunks land side by side, so
-// the permutation is in what each lane reads.  Rows behind the end read the
-// last one again: no weight meets them, and what they hold has met a weight
-// where it counts.
+// the permutation is in what each lane reads.  Chunks of padding are never
+// written (`clear` makes them zeros once).  Rows behind the end read the last
+// one again: no weight meets them, and what they hold has met a weight where it
+// counts.
 //
 // Otherwise the chunks come through registers, each lane testing its own, and
 // rows behind the end become zeros.
@@ -218,29 +242,55 @@ struct Stage<T, kWidth, kRows, kThreads, true> {
   static constexpr int kCount = kRows * Lds::kChunks / kThreads;
   static_assert(kRows * Lds::kChunks % kThreads == 0 && Lds::kChunks <= 64);
 
-  __device__ __forceinline__ static void one(const T* p, long l, int row0,
-                                             int end, char* tile) {
+  // Row pairs of the permutation repeat after 16 rows: where a step of all
+  // threads is a multiple of that, one offset a lane serves every step.
+  static constexpr int kStep = kThreads / Lds::kChunks;
+
+  // `per`: chunks of a part of the row (a map, or the whole), of which `size`
+  // values are there
+  __device__ __forceinline__ static void one(const T* p, int l, int rows,
+                                             int per, int size, char* tile) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lane = threadIdx.x & 63;
 #pragma unroll
     for (int j = 0; j < kCount; ++j) {
-      const int first = j * kThreads + wave * 64;  // chunk of lane 0
-      const int row = first / Lds::kChunks + lane / Lds::kChunks;
-      const int chunk = lane % Lds::kChunks ^ Lds::permute(row);
-      const int at = row0 + row < end ? row0 + row : end - 1;
-      __builtin_amdgcn_global_load_lds(
-          (__attribute__((address_space(1))) void*)(p + at * l +
-                                                    chunk * kChunk<T>),
-          (__attribute__((address_space(3))) void*)(tile + first * 16), 16, 0,
-          0);
+      // chunk of lane 0 within the step, and its row
+      const int first = wave * 64;
+      int row = first / Lds::kChunks + lane / Lds::kChunks;
+      const int chunk =
+          lane % Lds::kChunks ^ Lds::permute(row + (kStep % 16 ? j * kStep : 0));
+      if (rows < kRows) {  // the last tile alone
+        row += j * kStep;
+        row = (row < rows ? row : rows - 1) - j * kStep;
+      }
+      const T* src = p + (long)j * kStep * l;  // the same for all lanes
+      const int within = chunk % per * kChunk<T>;
+      if (within < size)
+        __builtin_amdgcn_global_load_lds(
+            (__attribute__((address_space(1))) void*)(src +
+                                                      (row * l +
+                                                       chunk / per * size +
+                                                       within)),
+            (__attribute__((address_space(3))) void*)(tile +
+                                                      (j * kThreads + first) *
+                                                          16),
+            16, 0, 0);
     }
   }
 
   __device__ __forceinline__ void load(const T* xp, long xl, const T* yp,
-                                       long yl, int, int, int row0, int end,
-                                       char* xt, char* yt) {
-    one(xp, xl, row0, end, xt);
-    one(yp, yl, row0, end, yt);
+                                       long yl, int map_size, int row_size,
+                                       int row0, int end, char* xt, char* yt) {
+    one(xp + row0 * xl, (int)xl, end - row0, Lds::kChunks / 2, map_size, xt);
+    one(yp + row0 * yl, (int)yl, end - row0, Lds::kChunks, row_size, yt);
+  }
+
+  // both tiles of a buffer become zeros, where some chunks will not be loaded
+  __device__ __forceinline__ static void clear(int map_size, int row_size,
+                                               char* tiles) {
+    if (2 * map_size == kWidth && row_size == kWidth) return;
+    for (int i = threadIdx.x; i < 2 * kRows * Lds::kChunks; i += kThreads)
+      reinterpret_cast<u32x4*>(tiles)[i] = u32x4{0, 0, 0, 0};
   }
 
   // before the barrier that shows the tiles to every wave
@@ -258,6 +308,8 @@ struct Stage<T, kWidth, kRows, kThreads, false> {
 
   u32x4 x[kCount], y[kCount];
 
+  __device__ __forceinline__ static void clear(int, int, char*) {}
+
   __device__ __forceinline__ void load(const T* xp, long xl, const T* yp,
                                        long yl, int map_size, int row_size,
                                        int row0, int end, char*, char*) {
@@ -269,8 +321,8 @@ struct Stage<T, kWidth, kRows, kThreads, false> {
     for (int j = 0; j < kCount; ++j) {
       const int row = first + j * kStep;
       const int at = row < end ? row : end - 1;
-      x[j] = load_chunk<false>(xp + at * xl, xc);
-      y[j] = load_chunk<false>(yp + at * yl, yc);
+      x[j] = load_chunk(xp + at * xl, xc);
+      y[j] = load_chunk(yp + at * yl, yc);
     }
   }
 

@@ -108,8 +108,8 @@ Tensor attn_forward(const Tensor& q, const Tensor& k, const Tensor& v,
   }
   if (out.numel() == 0) return out;
   Tensor split;
-  if (const size_t bytes = npf_diff_attn_workspace(a)) {
-    split = torch::empty({(long)bytes}, q.options().dtype(torch::kUInt8));
+  if (const long floats = npf_diff_attn_workspace(a)) {
+    split = torch::empty({floats}, q.options().dtype(torch::kFloat32));
     a.split = split.data_ptr();
   }
   npf_check(npf_diff_attn_fwd(a, at::hip::getCurrentHIPStream()),
@@ -163,7 +163,17 @@ struct DiffAttn : torch::autograd::Function<DiffAttn> {
     } else {
       const long rows = (long)a.B * a.H * a.Q;
       Tensor stats = torch::empty({rows, 4}, lse.options());
-      Tensor dlam_rows = torch::empty({rows}, lse.options());
+      Tensor dlam_rows = torch::empty({a.dq_splits * rows}, lse.options());
+      // parts of split sums
+      Tensor dq_part, dk_part, dv_part;
+      auto parts = [&](Tensor& part, const Tensor& grad, int splits) {
+        if (!grad.defined() || splits == 1) return (float*)nullptr;
+        part = torch::empty({splits * grad.numel()}, lse.options());
+        return part.data_ptr<float>();
+      };
+      a.dq_part = parts(dq_part, dq, a.dq_splits);
+      a.dk_part = parts(dk_part, dk, a.dkv_splits);
+      a.dv_part = parts(dv_part, dv, a.dkv_splits);
       a.out = heads_of(out);
       a.o2 = heads_of(o2);
       a.dout = heads_of(dout);
