@@ -151,7 +151,8 @@ __global__ void __launch_bounds__(256)
   store4(row_of<T>(out, bh / H, bh % H, l) + c, count, x[0], x[1], x[2], x[3]);
 }
 
-// delta_i of each row, beside its lse: kLanes lanes of 4 values a row
+// For gradients of keys and values alone, without the dq kernel that would
+// leave them: delta_i of each row, beside its lse: kLanes lanes of 4 values a row
 template <typename T, int kLanes>
 __global__ void __launch_bounds__(256) row_stats(NpfDiffAttnArgs a) {
   // (rows are checked to fit 31 bits; divisions of 64 bits would cost more
@@ -253,6 +254,7 @@ hipError_t join_forward(const NpfDiffAttnArgs& a, hipStream_t stream) {
 
 template <typename T>
 void stats(const NpfDiffAttnArgs& a, hipStream_t stream) {
+  if (a.dq.p || a.dlam) return;
   with_lanes(a.Dv, [&](auto lanes) {
     row_stats<T, lanes()>
         <<<row_blocks((long)a.B * a.H * a.Q, lanes()), 256, 0, stream>>>(a);

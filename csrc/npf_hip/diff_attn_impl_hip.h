@@ -336,9 +336,33 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, kPad>))
     else
       qf[u] = x;
   }
-  float4 st = {0.f, 0.f, 0.f, 0.f};
-  if (live) st = reinterpret_cast<const float4*>(a.stats)[stat];
   const float lam = lam_of(a, h), c = a.scale * kLog2e;
+  // the row's statistics; the dk/dv kernel finds them in a.stats
+  float4 st = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int u = 0; u < 2 * S::kSteps; ++u) {
+    if (!live) break;
+    const ChunkOf at = chunk_of_row<T>(u * 2 + half, a.Dv);
+    T g[kChunk<T>], o[kChunk<T>], o2[kChunk<T>];
+    const u32x4 x = load_chunk(row_of<T>(a.out, b, h, q), at);
+    const u32x4 y = load_chunk(row_of<T>(a.o2, b, h, q), at);
+    __builtin_memcpy(g, &gf[u], 16);
+    __builtin_memcpy(o, &x, 16);
+    __builtin_memcpy(o2, &y, 16);
+#pragma unroll
+    for (int i = 0; i < kChunk<T>; ++i) {
+      st.z += (float)g[i] * ((float)o[i] + lam * (float)o2[i]);
+      st.w += (float)g[i] * (float)o2[i];
+    }
+  }
+  st.z = both_sum(st.z);
+  st.w = both_sum(st.w);
+  if (live) {
+    st.x = a.lse[2 * stat];
+    st.y = a.lse[2 * stat + 1];
+    if (half == 0 && split == 0)
+      reinterpret_cast<float4*>(a.stats)[stat] = st;
+  }
 
   f32x16 dq[2][S::kMapBlocks];
 #pragma unroll
@@ -523,26 +547,32 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, kPad>))
   Stage<T, S::kWidth, kTile, 64 * kWaves, kDirect> stage;
   float4 st;
   float lam = 0.f, next_lam = 0.f;
-  auto load = [&](int step, char* to) {
-    const int h = hk * group + step / q_tiles;
-    next_lam = lam_of(a, h);
-    const int q0 = step % q_tiles * kTile;
-    stage.load(row_of<T>(a.q, b, h, 0), a.q.l, row_of<T>(a.dout, b, h, 0),
-               a.dout.l, a.D, a.Dv, q0, a.Q, to, to + kTileBytes);
-    const int q = q0 + (int)threadIdx.x;
+  // the tile that is being loaded
+  int next_h = hk * group + step0 / q_tiles, next_q = step0 % q_tiles * kTile;
+  auto load = [&](char* to) {
+    next_lam = lam_of(a, next_h);
+    stage.load(row_of<T>(a.q, b, next_h, 0), a.q.l,
+               row_of<T>(a.dout, b, next_h, 0), a.dout.l, a.D, a.Dv, next_q,
+               a.Q, to, to + kTileBytes);
+    const int q = next_q + (int)threadIdx.x;
     // rows that are not there have no weight
     st = float4{-kLowest, -kLowest, 0.f, 0.f};
     if (threadIdx.x < kTile && q < a.Q)
       st = reinterpret_cast<const float4*>(
-          a.stats)[((long)b * a.H + h) * a.Q + q];
+          a.stats)[((long)b * a.H + next_h) * a.Q + q];
   };
-  auto store = [&](int step, char* to, float (*to_stats)[kTile]) {
-    stage.store(a.Q - step % q_tiles * kTile, to, to + kTileBytes);
+  auto store = [&](char* to, float (*to_stats)[kTile]) {
+    stage.store(a.Q - next_q, to, to + kTileBytes);
     if (threadIdx.x < kTile) {
       to_stats[0][threadIdx.x] = st.x;
       to_stats[1][threadIdx.x] = st.y;
       to_stats[2][threadIdx.x] = st.z;
       to_stats[3][threadIdx.x] = st.w;
+    }
+    next_q += kTile;
+    if (next_q >= a.Q) {
+      next_q = 0;
+      ++next_h;
     }
   };
   auto pass = [&](const char* qt, const float (*stats)[kTile]) {
@@ -612,17 +642,17 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, kPad>))
                   char* then, float (*then_stats)[kTile]) {
     const bool more = step + 1 < steps;
     lam = next_lam;
-    if (more) load(step + 1, then);
+    if (more) load(then);
     pass(now, now_stats);
-    if (more) store(step + 1, then, then_stats);
+    if (more) store(then, then_stats);
     __syncthreads();
   };
   stage.clear(a.D, a.Dv, even);
   stage.clear(a.D, a.Dv, odd);
   __syncthreads();
   if (step0 < steps) {
-    load(step0, even);
-    store(step0, even, even_stats);
+    load(even);
+    store(even, even_stats);
   }
   __syncthreads();
   for (int step = step0; step < steps;) {

@@ -242,10 +242,20 @@ void check_apart(const std::vector<NpfGradSpans>& all) {
                       "clipped gradients must not share memory");
 }
 
-// norm of all gradients; max_norm >= 0 also scales them in place
-Tensor grad_norm(const std::vector<Tensor>& grads, double norm_type,
+// norm of the gradients of all parameters that have one; max_norm >= 0 also
+// scales them in place
+Tensor grad_norm(const std::vector<Tensor>& params, double norm_type,
                  double max_norm) {
   const int norm = norm_code(norm_type);
+  std::vector<Tensor> grads;
+  grads.reserve(params.size());
+  for (const Tensor& p : params) {
+    const Tensor& g = p.grad();
+    if (!g.defined()) continue;
+    TORCH_CHECK_TYPE(g.layout() == torch::kStrided,
+                     "gradients must be dense floating tensors");
+    grads.push_back(g);
+  }
   TORCH_CHECK_VALUE(!grads.empty(), "no gradients");
   std::vector<NpfGradSpans> all = spans_of(grads);
   const bool clip = max_norm >= 0.;
@@ -287,5 +297,5 @@ Tensor grad_norm(const std::vector<Tensor>& grads, double norm_type,
 void npf_bind_norms(pybind11::module_& m) {
   m.def("layer_norm", &layer_norm, "layer norm over the last axis");
   m.def("grad_norm", &grad_norm,
-        "norm of many gradients; max_norm >= 0 clips them in place");
+        "norm of the parameters' gradients; max_norm >= 0 clips them in place");
 }

@@ -9,7 +9,6 @@ SURVEY.md §2.3; reference call-sites cited per op.
 import math
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _backend
 
@@ -849,38 +848,6 @@ def _layer_norm_ref(x, weight, bias, eps, residual):
     return y.to(x.dtype)
 
 
-def _as_rows(t):
-    """[..., D] as [rows, D] with contiguous rows, copied only where no
-    stride describes them."""
-    rows = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
-    return rows if rows.stride(1) == 1 or rows.shape[1] == 1 else rows.contiguous()
-
-
-class _LayerNormFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, residual, weight, bias, eps):
-        ext = _backend.extension()
-        xr = _as_rows(x)
-        rr = None if residual is None else _as_rows(residual)
-        y, mean, rstd = ext.layer_norm_fwd(xr, rr, weight, bias, eps, True)
-        ctx.save_for_backward(xr, rr, weight, bias, mean, rstd)
-        return y.view(x.shape)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        ext = _backend.extension()
-        xr, rr, weight, bias, mean, rstd = ctx.saved_tensors
-        need_x, need_r, need_w, need_b = ctx.needs_input_grad[:4]
-        dx, dw, db = ext.layer_norm_bwd(
-            dy.reshape(xr.shape).contiguous(), xr, rr, weight, bias, mean, rstd,
-            need_x or need_r, need_w, need_b,
-        )
-        if dx is not None:
-            dx = dx.view(dy.shape)
-        return dx if need_x else None, dx if need_r else None, dw, db, None
-
-
 def layer_norm(x, weight=None, bias=None, eps=1e-5, residual=None):
     """Layer norm of `x` (or of ``x + residual``) over the last axis.
 
@@ -915,17 +882,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, residual=None):
     ext = _backend.require_extension("layer_norm")
     if ext is None:
         return _layer_norm_ref(x, weight, bias, eps, residual)
-    if weight is not None:
-        weight = weight.contiguous()
-    if bias is not None:
-        bias = bias.contiguous()
-    if torch.is_grad_enabled() and any(
-        t is not None and t.requires_grad for t in (x, residual, weight, bias)
-    ):
-        return _LayerNormFn.apply(x, residual, weight, bias, eps)
-    xr = _as_rows(x)
-    rr = None if residual is None else _as_rows(residual)
-    return ext.layer_norm_fwd(xr, rr, weight, bias, eps, False)[0].view(x.shape)
+    return ext.layer_norm(x, residual, weight, bias, eps)
 
 
 # --------------------------------------------------------------------------- #
@@ -960,34 +917,6 @@ def _differential_attention_ref(keys, queries, values, lam, scale, key_lengths):
             maps.append(logits.masked_fill(~row, low).softmax(-1) * row)
     lam = lam.to(maps[0].dtype).reshape(-1, 1, 1)
     return torch.matmul(maps[0] - lam * maps[1], values.contiguous()).to(dtype)
-
-
-def _as_heads(t):
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
-
-
-class _DifferentialAttentionFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, keys, queries, values, lam, scale, key_lengths):
-        ext = _backend.extension()
-        out, o2, lse = ext.diff_attn_fwd(
-            queries, keys, values, lam, scale, key_lengths, True
-        )
-        ctx.save_for_backward(keys, queries, values, lam, out, o2, lse, key_lengths)
-        ctx.scale = scale
-        return out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dout):
-        ext = _backend.extension()
-        keys, queries, values, lam, out, o2, lse, key_lengths = ctx.saved_tensors
-        need_k, need_q, need_v, need_lam = ctx.needs_input_grad[:4]
-        dq, dk, dv, dlam = ext.diff_attn_bwd(
-            _as_heads(dout), queries, keys, values, lam, out, o2, lse, ctx.scale,
-            key_lengths, need_q, need_k, need_v, need_lam,
-        )
-        return dk, dq, dv, dlam, None, None
 
 
 def differential_attention(keys, queries, values, lam, scale=None, key_lengths=None):
@@ -1050,19 +979,7 @@ def differential_attention(keys, queries, values, lam, scale=None, key_lengths=N
         return _differential_attention_ref(
             keys, queries, values, lam, scale, key_lengths
         )
-    keys, queries, values = _as_heads(keys), _as_heads(queries), _as_heads(values)
-    if key_lengths is not None:
-        key_lengths = key_lengths.contiguous()
-    if torch.is_grad_enabled() and (
-        keys.requires_grad or queries.requires_grad
-        or values.requires_grad or lam.requires_grad
-    ):
-        return _DifferentialAttentionFn.apply(
-            keys, queries, values, lam, scale, key_lengths
-        )
-    return ext.diff_attn_fwd(
-        queries, keys, values, lam, scale, key_lengths, False
-    )[0]
+    return ext.differential_attention(keys, queries, values, lam, scale, key_lengths)
 
 
 # --------------------------------------------------------------------------- #
@@ -1070,16 +987,20 @@ def differential_attention(keys, queries, values, lam, scale=None, key_lengths=N
 # --------------------------------------------------------------------------- #
 
 
-def _gradients(parameters, norm_type):
+def _with_gradients(parameters, norm_type):
+    """The parameters as a list, and their gradients if those are the composed
+    path's to take (not on a GPU, or none)."""
     if norm_type not in (1, 2, math.inf):
         raise ValueError(f"norm_type must be 1, 2 or inf, got {norm_type}")
-    if torch.is_tensor(parameters):
-        parameters = [parameters]
-    grads = [p.grad for p in parameters if p.grad is not None]
+    params = [parameters] if torch.is_tensor(parameters) else list(parameters)
+    first = next((g for p in params if (g := p.grad) is not None), None)
+    if first is not None and first.is_cuda and _backend.require_extension("grad_norm"):
+        return params, None
+    grads = [p.grad for p in params if p.grad is not None]
     for g in grads:
         if g.layout != torch.strided or not g.is_floating_point():
             raise TypeError("gradients must be dense floating tensors")
-    return grads
+    return params, grads
 
 
 def _grad_norm_ref(grads, norm_type):
@@ -1096,13 +1017,10 @@ def grad_norm(parameters, norm_type=2.0):
     are left out.  norm_type: 1, 2 or inf.  Returns a 0-d tensor on the
     gradients' device (fp32 on a GPU, fp64 where a gradient is); no host wait.
     """
-    grads = _gradients(parameters, norm_type)
-    if not grads or not grads[0].is_cuda:
+    params, grads = _with_gradients(parameters, norm_type)
+    if grads is not None:
         return _grad_norm_ref(grads, norm_type)
-    ext = _backend.require_extension("grad_norm")
-    if ext is None:
-        return _grad_norm_ref(grads, norm_type)
-    return ext.grad_norm(grads, norm_type, -1.0)
+    return _backend.extension().grad_norm(params, norm_type, -1.0)
 
 
 def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
@@ -1119,23 +1037,21 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError(f"max_norm must not be negative, got {max_norm}")
-    grads = _gradients(parameters, norm_type)
-    ext = None
-    if grads and grads[0].is_cuda:
-        ext = _backend.require_extension("grad_norm")
-    if error_if_nonfinite or ext is None:
+    params, grads = _with_gradients(parameters, norm_type)
+    ext = _backend.extension()
+    if error_if_nonfinite or grads is not None:
         total = (
-            _grad_norm_ref(grads, norm_type) if ext is None
-            else ext.grad_norm(grads, norm_type, -1.0)
+            ext.grad_norm(params, norm_type, -1.0) if grads is None
+            else _grad_norm_ref(grads, norm_type)
         )
         if error_if_nonfinite and not bool(torch.isfinite(total)):
             raise RuntimeError(
                 f"the norm of order {norm_type} of the gradients is {float(total)}, "
                 "so they cannot be clipped"
             )
-        if ext is None:
+        if grads is not None:
             c = torch.clamp(max_norm / (total + 1e-6), max=1.0)
             for g in grads:
                 g.mul_(c.to(g.device))
             return total
-    return ext.grad_norm(grads, norm_type, max_norm)
+    return ext.grad_norm(params, norm_type, max_norm)
