@@ -300,7 +300,7 @@ bool npf_diff_attn_plan(NpfDiffAttnArgs& a) {
   a.waves = rows <= 32 ? 1 : 4;
   const long row_blocks4 = heads * ((rows + 127) / 128);
   a.splits = a.waves == 1 ? parts_for(heads, 1280, a.K, 256)
-                          : parts_for(row_blocks4, 512, a.K, 512);
+                          : parts_for(row_blocks4, 512, a.K, 256);
   a.dq_splits = parts_for(row_blocks4, 512, a.K, 256);
   a.dkv_splits =
       parts_for(heads * ((a.K + 127) / 128), 512, (int)rows, 256);

@@ -85,12 +85,23 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, kPad>))
 
   const int group = a.H / a.Hk, rows = group * a.Q;
   const int row_tiles = (rows + 32 * kWaves - 1) / (32 * kWaves);
-  int id = blockIdx.x;
-  const int part = id % S::kParts;
-  id /= S::kParts;
-  const int split = id % a.splits;
-  id /= a.splits;
-  const int row_tile = id % row_tiles, bh = id / row_tiles;
+  // Neighbouring blocks take different batch entries and heads: long and short
+  // contexts spread over the chip, and as blocks are dealt to the 8 XCDs in
+  // turn, those of one head mostly share an L2.  With few rows nothing is
+  // shared, and neighbours in memory are read at a time (single queries
+  // against 32768 keys: 52 us rather than 66).
+  const int heads = a.B * a.Hk;
+  const int part = blockIdx.x % S::kParts, id = blockIdx.x / S::kParts;
+  int bh, row_tile, split;
+  if (kWaves == 1) {
+    split = id % a.splits;
+    row_tile = id / a.splits % row_tiles;
+    bh = id / a.splits / row_tiles;
+  } else {
+    bh = id % heads;
+    row_tile = id / heads % row_tiles;
+    split = id / heads / row_tiles;
+  }
   const int b = bh / a.Hk, hk = bh % a.Hk;
   const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
   const int row = (row_tile * kWaves + (threadIdx.x >> 6)) * 32 + col;
@@ -298,10 +309,9 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, kPad>))
 
   const int group = a.H / a.Hk, rows = group * a.Q;
   const int row_tiles = (rows + 32 * kWaves - 1) / (32 * kWaves);
-  int id = blockIdx.x;
-  const int split = id % a.dq_splits;
-  id /= a.dq_splits;
-  const int row_tile = id % row_tiles, bh = id / row_tiles;
+  const int heads = a.B * a.Hk, bh = blockIdx.x % heads;
+  const int row_tile = blockIdx.x / heads % row_tiles;
+  const int split = blockIdx.x / heads / row_tiles;
   const int b = bh / a.Hk, hk = bh % a.Hk;
   const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
   const int row = (row_tile * kWaves + (threadIdx.x >> 6)) * 32 + col;
@@ -502,10 +512,9 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, kPad>))
 
   const int group = a.H / a.Hk;
   const int key_tiles = (a.K + 32 * kWaves - 1) / (32 * kWaves);
-  int id = blockIdx.x;
-  const int split = id % a.dkv_splits;
-  id /= a.dkv_splits;
-  const int key_tile = id % key_tiles, bh = id / key_tiles;
+  const int heads = a.B * a.Hk, bh = blockIdx.x % heads;
+  const int key_tile = blockIdx.x / heads % key_tiles;
+  const int split = blockIdx.x / heads / key_tiles;
   const int b = bh / a.Hk, hk = bh % a.Hk;
   const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
   const int key = (key_tile * kWaves + (threadIdx.x >> 6)) * 32 + col;
