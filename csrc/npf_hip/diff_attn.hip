@@ -298,12 +298,18 @@ bool npf_diff_attn_plan(NpfDiffAttnArgs& a) {
   // Rows that fit one wave get a block of one wave, the others share tiles
   // between four.
   a.waves = rows <= 32 ? 1 : 4;
+  // Blocks that the chip holds at once: of one wave by their LDS (4 tiles of
+  // 32 or 64 rows), of four by their registers (see kResident).
+  const int row_bytes = 2 * a.pad * (a.type == NPF_F32 ? 4 : 2);
+  const long wanted1 = row_bytes <= 256 ? 1280 : row_bytes == 512 ? 512 : 256;
+  const long wanted = row_bytes <= 256 ? 512 : 256;
   const long row_blocks4 = heads * ((rows + 127) / 128);
-  a.splits = a.waves == 1 ? parts_for(heads, 1280, a.K, 256)
-                          : parts_for(row_blocks4, 512, a.K, 256);
-  a.dq_splits = parts_for(row_blocks4, 512, a.K, 256);
+  const long parts = a.pad == 128 ? 2 : 1;
+  a.splits = a.waves == 1 ? parts_for(heads * parts, wanted1, a.K, 64)
+                          : parts_for(row_blocks4 * parts, wanted, a.K, 256);
+  a.dq_splits = parts_for(row_blocks4, wanted, a.K, 256);
   a.dkv_splits =
-      parts_for(heads * ((a.K + 127) / 128), 512, (int)rows, 256);
+      parts_for(heads * ((a.K + 127) / 128), wanted, (int)rows, 256);
   return true;
 }
 

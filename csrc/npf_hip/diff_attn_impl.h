@@ -23,11 +23,14 @@ struct Shape {
   // keys (or queries) a tile: two buffers of two tiles in 64 KiB
   static constexpr int kTile = kRowBytes <= 256 ? 64 : 32;
   // tiles of 32 that a wave takes through a pass at once
-  static constexpr int kSubs = kPad <= 32 ? 2 : 1;
-  // whether a wave's registers hold both gradients of its keys; else each has
-  // a launch of its own, at two waves a SIMD rather than one (bf16, 2 x 16 x
-  // 4096 x 4096, maps of 64: see the table of measurements)
+  static constexpr int kSubs = sizeof(T) == 2 ? (kPad <= 32 ? 2 : 1)
+                                              : (kPad <= 16 ? 2 : 1);
+  // What a wave's registers hold decides how the gradients share launches: of
+  // the keys both at once, else dk and dv apart, else dk of each map apart; of
+  // the queries both maps at once, else apart.
   static constexpr bool kBothGrads = kPad * (int)sizeof(T) < 128;
+  static constexpr bool kDkMapsApart = kPad == 128;
+  static constexpr bool kDqMapsApart = kPad * (int)sizeof(T) > 256;
   // whether the dq kernel keeps its queries in LDS rather than in registers
   static constexpr bool kQueriesInLds = sizeof(T) == 2 && kPad == 64;
   // parts of the values' columns that forward blocks take: the sums of 256
@@ -289,9 +292,9 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, kPad>))
   }
 }
 
-// dq, and each row's part of dlam: a wave holds 32 query rows and passes over
-// the keys
-template <typename T, int kPad, int kWaves, bool kDirect>
+// dq of the maps in kMaps (bits), and with the second map each row's part of
+// dlam: a wave holds 32 query rows and passes over the keys
+template <typename T, int kPad, int kWaves, bool kDirect, int kMaps>
 __global__ void __launch_bounds__(64 * kWaves, (kResident<T, kPad>))
     diff_bwd_dq(NpfDiffAttnArgs a) {
   using S = Shape<T, kPad>;
@@ -368,7 +371,7 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, kPad>))
   if (live) {
     st.x = a.lse[2 * stat];
     st.y = a.lse[2 * stat + 1];
-    if (half == 0 && split == 0)
+    if ((kMaps & 1) && half == 0 && split == 0)
       reinterpret_cast<float4*>(a.stats)[stat] = st;
   }
 
@@ -401,6 +404,7 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, kPad>))
       // one map after the other: a second tile of scores would not fit
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
+        if (!(kMaps >> m & 1)) continue;
         f32x16 s[kSubs];
 #pragma unroll
         for (int t = 0; t < kSubs; ++t) {
@@ -471,14 +475,14 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, kPad>))
   dlam = both_sum(dlam);
   if (!live) return;
   const long part = (long)split * a.B * a.H * a.Q + stat;
-  if (half == 0) a.dlam_rows[part] = dlam;
+  if ((kMaps & 2) && half == 0) a.dlam_rows[part] = dlam;
   if (!a.dq.p) return;
   T* out = row_of<T>(a.dq, b, h, q);
   float* sum = a.dq_part + part * 2 * a.D;
 #pragma unroll
   for (int m = 0; m < 2; ++m)
 #pragma unroll
-    for (int j = 0; j < S::kMapBlocks; ++j)
+    for (int j = 0; j < (kMaps >> m & 1 ? S::kMapBlocks : 0); ++j)
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         if (kPad == 16 && g / 2 != m) continue;
@@ -493,13 +497,14 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, kPad>))
       }
 }
 
-// dk and dv: a wave holds 32 keys and passes over the queries of the heads
-// that share them
-template <typename T, int kPad, int kWaves, bool kDirect, bool kDk, bool kDv>
+// dk of the maps in kMaps (bits) and, with kDv, dv: a wave holds 32 keys and
+// passes over the queries of the heads that share them
+template <typename T, int kPad, int kWaves, bool kDirect, int kMaps, bool kDv>
 __global__ void __launch_bounds__(64 * kWaves, (kResident<T, kPad>))
     diff_bwd_dkv(NpfDiffAttnArgs a) {
   using S = Shape<T, kPad>;
   using Lds = Tile<T, S::kWidth>;
+  constexpr bool kDk = kMaps != 0;
   constexpr int kTile = kDk && !S::kBothGrads ? 32 : S::kTile;
   constexpr int kTileBytes = kTile * S::kRowBytes;
   // two objects, so that it shows that the next tiles' loads do not touch
@@ -590,6 +595,7 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, kPad>))
       f32x16 p[2], x;
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
+        if (!kDv && !(kMaps >> m & 1)) continue;
         p[m] = f32x16{};
 #pragma unroll
         for (int u = 0; u < S::kSteps; ++u)
@@ -615,6 +621,9 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, kPad>))
         for (int j = 0; j < S::kBlocks; ++j) {
           f32x16* const acc[1] = {&dv[j]};
           Lds::template transposed<1>(gt, cb, sub, 32 * j, map, acc);
+          // (reads of later columns would be taken ahead into registers that
+          // are not there)
+          if (kPad * (int)sizeof(T) > 256) __builtin_amdgcn_sched_barrier(0);
         }
       }
       if (kDk) {
@@ -624,6 +633,7 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, kPad>))
           x = mma_chunk<T>(Lds::rows(gt, rb, sub, u), vf[u], x);
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
+          if (!(kMaps >> m & 1)) continue;
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const f32x4 d =
@@ -678,7 +688,7 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, kPad>))
 #pragma unroll
     for (int m = 0; m < 2; ++m)
 #pragma unroll
-      for (int j = 0; j < S::kMapBlocks; ++j)
+      for (int j = 0; j < (kMaps >> m & 1 ? S::kMapBlocks : 0); ++j)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           if (kPad == 16 && g / 2 != m) continue;
@@ -737,22 +747,43 @@ hipError_t fwd_sized(const NpfDiffAttnArgs& a, hipStream_t stream) {
 template <typename T, int kPad, bool kDirect>
 hipError_t bwd_sized(const NpfDiffAttnArgs& a, hipStream_t stream) {
   const long heads = (long)a.B * a.Hk, rows = (long)(a.H / a.Hk) * a.Q;
+  using S = Shape<T, kPad>;
   hipError_t e = hipSuccess;
-  if (a.dq.p || a.dlam)
-    e = launch(diff_bwd_dq<T, kPad, 4, kDirect>,
-               heads * a.dq_splits * ((rows + 127) / 128), 256, a, stream);
-  const long blocks = heads * a.dkv_splits * ((a.K + 127) / 128);
-  if constexpr (Shape<T, kPad>::kBothGrads) {
-    if (e == hipSuccess && (a.dk.p || a.dv.p))
-      e = launch(diff_bwd_dkv<T, kPad, 4, kDirect, true, true>, blocks, 256, a,
-                 stream);
+  auto dq = [&](auto maps) {
+    if (e == hipSuccess)
+      e = launch(diff_bwd_dq<T, kPad, 4, kDirect, decltype(maps)::value>,
+                 heads * a.dq_splits * ((rows + 127) / 128), 256, a, stream);
+  };
+  auto dkv = [&](auto maps, auto with_dv) {
+    if (e == hipSuccess)
+      e = launch(diff_bwd_dkv<T, kPad, 4, kDirect, decltype(maps)::value,
+                              decltype(with_dv)::value>,
+                 heads * a.dkv_splits * ((a.K + 127) / 128), 256, a, stream);
+  };
+  using None = std::integral_constant<int, 0>;
+  using First = std::integral_constant<int, 1>;
+  using Second = std::integral_constant<int, 2>;
+  using Both = std::integral_constant<int, 3>;
+  if (a.dq.p || a.dlam) {
+    if constexpr (S::kDqMapsApart) {
+      dq(First{});
+      dq(Second{});
+    } else {
+      dq(Both{});
+    }
+  }
+  if constexpr (S::kBothGrads) {
+    if (a.dk.p || a.dv.p) dkv(Both{}, std::true_type{});
   } else {
-    if (e == hipSuccess && a.dk.p)
-      e = launch(diff_bwd_dkv<T, kPad, 4, kDirect, true, false>, blocks, 256, a,
-                 stream);
-    if (e == hipSuccess && a.dv.p)
-      e = launch(diff_bwd_dkv<T, kPad, 4, kDirect, false, true>, blocks, 256, a,
-                 stream);
+    if (a.dk.p) {
+      if constexpr (S::kDkMapsApart) {
+        dkv(First{}, std::false_type{});
+        dkv(Second{}, std::false_type{});
+      } else {
+        dkv(Both{}, std::false_type{});
+      }
+    }
+    if (a.dv.p) dkv(None{}, std::true_type{});
   }
   return e;
 }
