@@ -380,7 +380,10 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, kPad>))
   for (int m = 0; m < 2; ++m)
 #pragma unroll
     for (int j = 0; j < S::kMapBlocks; ++j) dq[m][j] = f32x16{};
+  // sum of P_2 (G - delta_2), which is zero but for the rounding that delta_2
+  // has seen: with delta_2 it makes the exact sum of P_2 G
   float dlam = 0.f;
+  const float apart = st.z - st.w;
 
   Stage<T, S::kWidth, kTile, 64 * kWaves, kDirect> stage;
   const T* kp = row_of<T>(a.k, b, hk, 0);
@@ -395,7 +398,9 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, kPad>))
       f32x16 g[kSubs];
 #pragma unroll
       for (int t = 0; t < kSubs; ++t) {
-        g[t] = f32x16{};
+        // the products start from -delta_1, which costs what zeros would
+#pragma unroll
+        for (int i = 0; i < 16; ++i) g[t][i] = -st.z;
 #pragma unroll
         for (int u = 0; u < 2 * S::kSteps; ++u)
           g[t] = mma_chunk<T>(Lds::rows(vt, rb, sub0 + 32 * t, u), gf[u], g[t]);
@@ -419,7 +424,7 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, kPad>))
             s[t] = mma_chunk<T>(Lds::rows(kt, rb, sub0 + 32 * t, u), x, s[t]);
           }
         }
-        const float lse = m ? st.y : st.x, delta = m ? st.w : st.z;
+        const float lse = m ? st.y : st.x;
 #pragma unroll
         for (int t = 0; t < kSubs; ++t) {
 #pragma unroll
@@ -427,8 +432,8 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, kPad>))
             float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i], c, -lse));
             if (kEdge && k0 + sub0 + 32 * t + reg_row(i) + 4 * half >= n)
               p = 0.f;
-            if (m) dlam = __builtin_fmaf(p, g[t][i], dlam);
-            s[t][i] = p * (g[t][i] - delta);
+            s[t][i] = p * (m ? g[t][i] + apart : g[t][i]);
+            if (m) dlam += s[t][i];
           }
           const Operand<T> ds[1] = {Operand<T>(s[t])};
 #pragma unroll
@@ -472,7 +477,7 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, kPad>))
   }
   if (k0 < n) pass(std::true_type{}, k0, full & 1 ? odd : even);
 
-  dlam = both_sum(dlam);
+  dlam = both_sum(dlam) + (split == 0 ? st.w : 0.f);
   if (!live) return;
   const long part = (long)split * a.B * a.H * a.Q + stat;
   if ((kMaps & 2) && half == 0) a.dlam_rows[part] = dlam;
@@ -511,7 +516,11 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, kPad>))
   // what is being read
   __shared__ __attribute__((aligned(16))) char even[2 * kTileBytes];
   __shared__ __attribute__((aligned(16))) char odd[2 * kTileBytes];
-  // of each tile's queries: lse_1, lse_2, delta_1, delta_2
+  // Of each tile's queries what the products start from, and what parts the
+  // two maps: the scores' -lse_i / c in 16 bits, where the maps' rounding hides
+  // that they are summed at that size (lse_i in 32 bits); -delta_1 and
+  // delta_2 - delta_1.
+  constexpr bool kFromLse = sizeof(T) == 2;
   __shared__ __attribute__((aligned(16))) float even_stats[4][kTile];
   __shared__ __attribute__((aligned(16))) float odd_stats[4][kTile];
 
@@ -568,7 +577,7 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, kPad>))
                a.Q, to, to + kTileBytes);
     const int q = next_q + (int)threadIdx.x;
     // rows that are not there have no weight
-    st = float4{-kLowest, -kLowest, 0.f, 0.f};
+    st = float4{INFINITY, INFINITY, 0.f, 0.f};
     if (threadIdx.x < kTile && q < a.Q)
       st = reinterpret_cast<const float4*>(
           a.stats)[((long)b * a.H + next_h) * a.Q + q];
@@ -576,10 +585,10 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, kPad>))
   auto store = [&](char* to, float (*to_stats)[kTile]) {
     stage.store(a.Q - next_q, to, to + kTileBytes);
     if (threadIdx.x < kTile) {
-      to_stats[0][threadIdx.x] = st.x;
-      to_stats[1][threadIdx.x] = st.y;
-      to_stats[2][threadIdx.x] = st.z;
-      to_stats[3][threadIdx.x] = st.w;
+      to_stats[0][threadIdx.x] = kFromLse ? -st.x / c : st.x;
+      to_stats[1][threadIdx.x] = kFromLse ? -st.y / c : st.y;
+      to_stats[2][threadIdx.x] = -st.z;
+      to_stats[3][threadIdx.x] = st.w - st.z;
     }
     next_q += kTile;
     if (next_q >= a.Q) {
@@ -596,22 +605,23 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, kPad>))
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
         if (!kDv && !(kMaps >> m & 1)) continue;
-        p[m] = f32x16{};
+        p[m] = kFromLse ? rows16(stats[m], sub, half) : f32x16{};
 #pragma unroll
         for (int u = 0; u < S::kSteps; ++u)
           p[m] = mma_chunk<T>(Lds::rows(qt, rb, sub, m * S::kSteps + u),
                               kf[m][u], p[m]);
+        if constexpr (kFromLse) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const f32x4 lse = *(const f32x4*)&stats[m][sub + 8 * r + 4 * half];
+          for (int i = 0; i < 16; ++i)
+            p[m][i] = __builtin_amdgcn_exp2f(p[m][i] * c);
+        } else {
+          const f32x16 lse = rows16(stats[m], sub, half);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float y = __builtin_amdgcn_exp2f(
-                __builtin_fmaf(p[m][4 * r + e], c, -lse[e]));
-            if (m) y *= lam;
-            p[m][4 * r + e] = y;
-          }
+          for (int i = 0; i < 16; ++i)
+            p[m][i] =
+                __builtin_amdgcn_exp2f(__builtin_fmaf(p[m][i], c, -lse[i]));
         }
+        if (m) p[m] *= lam;
       }
       if (kDv) {
 #pragma unroll
@@ -627,23 +637,17 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, kPad>))
         }
       }
       if (kDk) {
-        x = f32x16{};
+        x = rows16(stats[2], sub, half);
 #pragma unroll
         for (int u = 0; u < 2 * S::kSteps; ++u)
           x = mma_chunk<T>(Lds::rows(gt, rb, sub, u), vf[u], x);
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
           if (!(kMaps >> m & 1)) continue;
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const f32x4 d =
-                *(const f32x4*)&stats[2 + m][sub + 8 * r + 4 * half];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int i = 4 * r + e;
-              p[m][i] *= m ? d[e] - x[i] : x[i] - d[e];
-            }
-          }
+          if (m == 0)
+            p[m] *= x;
+          else
+            p[m] *= rows16(stats[3], sub, half) - x;
           const Operand<T> ds[1] = {Operand<T>(p[m])};
 #pragma unroll
           for (int j = 0; j < S::kMapBlocks; ++j) {
@@ -653,6 +657,8 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, kPad>))
           }
         }
       }
+      // (the next tile's reads, taken ahead, would not fit the registers)
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
   auto turn = [&](int step, const char* now, const float (*now_stats)[kTile],

@@ -381,6 +381,20 @@ __device__ __forceinline__ float both_sum(float x) {
   return h.low + h.high;
 }
 
+// one value a row of a 32-row block, in the order of a tile's registers
+__device__ __forceinline__ f32x16 rows16(const float* of_row, int row0,
+                                         int half) {
+  f32x16 x;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const f32x4 y =
+        *reinterpret_cast<const f32x4*>(of_row + row0 + 8 * r + 4 * half);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[4 * r + i] = y[i];
+  }
+  return x;
+}
+
 // 4 consecutive values of a row, of which `count` exist
 template <typename T>
 __device__ __forceinline__ void store4(T* p, int count, float a, float b,

@@ -930,7 +930,7 @@ def differential_attention(keys, queries, values, lam, scale=None, key_lengths=N
     Dv <= 2 * max(D, 16) rounded up to the next of 32, 64, 128, 256.
 
     lam: 0-d, or [H] for one weight a head, any floating type.
-    scale: positive; 1 / sqrt(D) by default.
+    scale: from 1e-20 to 1e20; 1 / sqrt(D) by default.
     key_lengths: int [B] on the same device; batch entry b attends to its
     first key_lengths[b] keys (values outside 0..K count as the nearest of the
     two) and later keys are not read.  Rows without keys give zeros, and take
@@ -967,8 +967,8 @@ def differential_attention(keys, queries, values, lam, scale=None, key_lengths=N
         raise TypeError(f"lam must be floating, got {lam.dtype}")
     if scale is None:
         scale = 1.0 / math.sqrt(D2 // 2)
-    if not 0.0 < scale < math.inf:
-        raise ValueError(f"scale must be positive, got {scale}")
+    if not 1e-20 <= scale <= 1e20:
+        raise ValueError(f"scale must be from 1e-20 to 1e20, got {scale}")
     if key_lengths is not None:
         if tuple(key_lengths.shape) != (B,):
             raise ValueError(f"key_lengths has shape {tuple(key_lengths.shape)}, needs ({B},)")
