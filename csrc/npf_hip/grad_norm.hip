@@ -15,7 +15,9 @@
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kMostBlocks = 2048;
+// 492 MB of bf16, both passes with 512, 1024, 2048, 4096 blocks: 280, 268, 278,
+// 286 us.
+constexpr int kMostBlocks = 1024;
 
 __device__ __forceinline__ double join(double a, double b, int norm) {
   if (norm != NPF_NORM_INF) return a + b;
@@ -160,7 +162,9 @@ __global__ void __launch_bounds__(kThreads)
   // a norm that is no number makes every gradient none
   const float scale = ratio >= 1. ? 1.f : (float)ratio;
   if (scale == 1.f) return;  // nothing to change
-  for (int c = blockIdx.x; c < s.first_chunk[s.n]; c += gridDim.x) {
+  // from the last chunk back: what the first pass read last is still cached
+  for (int c = s.first_chunk[s.n] - 1 - (int)blockIdx.x; c >= 0;
+       c -= gridDim.x) {
     const int i = span_of(s, c);
     const long per = kGradChunkBytes / size_of(s.type[i]);
     const long at = (long)(c - s.first_chunk[i]) * per;
