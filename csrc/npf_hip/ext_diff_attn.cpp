@@ -40,9 +40,11 @@ NpfDiffAttnArgs common_args(const Tensor& q, const Tensor& k, const Tensor& v,
   check_heads(k, q, "keys");
   check_heads(v, q, "values");
   NpfDiffAttnArgs a{};
-  const int64_t most = std::numeric_limits<int>::max() / 2;
-  TORCH_CHECK_VALUE(q.size(0) <= 65535 && q.size(1) <= 65535 &&
-                        q.size(1) * q.size(2) <= most && k.size(2) <= most,
+  // rows are counted in 31 bits; offsets in memory are not
+  const int64_t most = std::numeric_limits<int>::max();
+  TORCH_CHECK_VALUE(q.size(0) * q.size(1) * q.size(2) <= most &&
+                        q.size(0) * k.size(1) * k.size(2) <= most &&
+                        k.size(2) <= most / 2 && q.size(2) <= most / 2,
                     "differential_attention: too many rows");
   a.B = (int)q.size(0);
   a.H = (int)q.size(1);

@@ -926,8 +926,8 @@ def differential_attention(keys, queries, values, lam, scale=None, key_lengths=N
     first map's in the first half; values [B, Hk, K, Dv]; result
     [B, H, Q, Dv].  Query head h reads key head h // (H // Hk), so Hk < H
     shares keys between heads.  All three of one type (fp32, bf16, fp16), any
-    strides with a contiguous last axis (others are copied), D <= 128,
-    Dv <= 2 * max(D, 16) rounded up to the next of 32, 64, 128, 256.
+    strides with a contiguous last axis (others are copied), D <= 128 and
+    Dv <= 256 on a GPU.
 
     lam: 0-d, or [H] for one weight a head, any floating type.
     scale: from 1e-20 to 1e20; 1 / sqrt(D) by default.

@@ -191,6 +191,37 @@ class TestLayerNorm:
         check_norm(run_norm("cuda", x, r, None, None, dy), want)
 
     @pytest.mark.gpu
+    @pytest.mark.parametrize("width", [20, 700])
+    def test_weight_or_bias_alone(self, width):
+        x, r, w, b, dy = norm_inputs(30, width, torch.bfloat16, torch.bfloat16, False)
+        zero = torch.zeros_like(b)
+        want = norm_oracle(x, None, w, zero, 1e-5, dy, torch.bfloat16)
+        check_norm(run_norm("cuda", x, None, w, None, dy), want)
+        want = norm_oracle(x, None, None, b, 1e-5, dy, torch.bfloat16)
+        check_norm(run_norm("cuda", x, None, None, b, dy), want)
+
+    @pytest.mark.gpu
+    def test_weights_of_other_types(self):
+        for wtype in (torch.float16, torch.float64):
+            args = norm_inputs(30, 70, torch.float32, wtype, True)
+            check_norm(run_norm("cuda", *args),
+                       norm_oracle(*args[:4], 1e-5, args[4], torch.float32))
+
+    @pytest.mark.gpu
+    def test_residual_and_its_gradient(self):
+        x = torch.randn(6, 24, device="cuda", requires_grad=True)
+        r = torch.randn(6, 24, device="cuda", requires_grad=True)
+        dy = torch.randn(6, 24, device="cuda")
+        ops.layer_norm(x, residual=r).backward(dy)
+        assert torch.equal(x.grad, r.grad) and x.grad.data_ptr() != r.grad.data_ptr()
+        # the same tensor twice: its gradients add up
+        z = x.detach().clone().requires_grad_(True)
+        ops.layer_norm(z, residual=z).backward(dy)
+        one = x.detach().clone().requires_grad_(True)
+        ops.layer_norm(one, residual=x.detach()).backward(dy)
+        assert torch.equal(z.grad, 2 * one.grad)
+
+    @pytest.mark.gpu
     @pytest.mark.parametrize("width", [8, 96, 2000])
     def test_one_of_the_gradients(self, width):
         x, r, w, b, dy = (None if t is None else t.cuda() for t in norm_inputs(
@@ -203,6 +234,16 @@ class TestLayerNorm:
             (grad,) = torch.autograd.grad(y, leaves[at], dy)
             assert torch.equal(grad, full[name]), name
             leaves[at].requires_grad_(False)
+
+    @pytest.mark.gpu
+    def test_differentiable_once(self):
+        x = torch.randn(3, 8, device="cuda", requires_grad=True)
+        w = torch.randn(8, device="cuda", requires_grad=True)
+        y = ops.layer_norm(x, w)
+        (dx,) = torch.autograd.grad(y.sum(), x, create_graph=True)
+        assert torch.equal(dx, torch.autograd.grad(ops.layer_norm(x, w).sum(), x)[0])
+        with pytest.raises(RuntimeError, match="layer_norm is differentiable once"):
+            dx.square().sum().backward()
 
     @pytest.mark.gpu
     def test_no_rows(self):
@@ -385,6 +426,15 @@ SIZES = [
     (1, 1, 1, 130, 260, 128, 256),
     (1, 2, 1, 3, 515, 128, 100),
     (2, 8, 1, 1, 300, 24, 48),
+    # values wider or narrower than two maps
+    (1, 2, 2, 40, 50, 16, 100),
+    (1, 2, 1, 40, 50, 48, 16),
+    (2, 2, 1, 50, 90, 96, 192),
+    # one block of rows or keys: sums over a split axis
+    (1, 2, 1, 600, 700, 16, 32),
+    (1, 1, 1, 300, 1100, 64, 128),
+    (1, 3, 1, 400, 530, 128, 256),
+    (1, 2, 2, 257, 513, 20, 40),
 ]
 
 
@@ -404,6 +454,12 @@ class TestDifferentialAttention:
             a = attn_inputs(3, 2, 1, 4, 7, 4, 8, torch.float32)
         check_attn(run_attn("cpu", a, lengths=lengths),
                    attn_oracle(a, lengths=lens))
+
+    def test_composed_empty(self):
+        for B, Q, K in ((0, 3, 4), (2, 0, 4), (2, 3, 0)):
+            got = run_attn("cpu", attn_inputs(B, 2, 1, Q, K, 4, 8, torch.float32))
+            assert got["out"].shape == (B, 2, Q, 8)
+            assert not any(t.any() for t in got.values())
 
     def test_gradient_against_differences(self):
         a = attn_inputs(2, 2, 1, 3, 4, 2, 3, torch.float64)
@@ -443,6 +499,7 @@ class TestDifferentialAttention:
             (ValueError, (k, q, v, lam), dict(scale=0.0)),
             (ValueError, (k, q, v, lam), dict(scale=-1.0)),
             (ValueError, (k, q, v, lam), dict(scale=math.nan)),
+            (ValueError, (k, q, v, lam), dict(scale=1e-30)),
             (ValueError, (k, q, v, lam), dict(key_lengths=torch.tensor([1]))),
             (TypeError, (k, q, v, lam), dict(key_lengths=torch.tensor([1.0, 2.0]))),
         ]
@@ -519,6 +576,37 @@ class TestDifferentialAttention:
                 assert torch.equal(x1, x2)
 
     @pytest.mark.gpu
+    @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+    def test_aligned_and_not(self, dtype):
+        # whole chunks at an odd place in memory take the loads that test each
+        # lane's; the same products in the same order
+        a = {n: t.cuda() for n, t in
+             attn_inputs(1, 2, 1, 70, 150, 64, 128, dtype).items()}
+        want = run_attn("cuda", a)
+
+        def moved(t):
+            room = torch.empty(t.numel() + 1, dtype=t.dtype, device="cuda")
+            return room[1:].view(t.shape).copy_(t)
+
+        got = run_attn("cuda", {n: t if n == "lam" else moved(t) for n, t in a.items()})
+        for n in want:
+            assert torch.equal(want[n], got[n]), n
+
+    @pytest.mark.gpu
+    @pytest.mark.parametrize("far", ["batch", "row"])
+    def test_offsets_over_32_bits(self, far):
+        # a cache whose entries stand more than 2^31 values apart
+        a = attn_inputs(2, 2, 1, 3, 130, 16, 32, torch.bfloat16)
+        step = {"batch": (2 ** 31 + 64, 32), "row": (64, 2 ** 24 + 32)}[far]
+        room = torch.empty(step[0] + 260 * step[1] + 64, dtype=torch.bfloat16, device="cuda")
+        t = {n: x.cuda() for n, x in a.items()}
+        for i, n in enumerate(("keys", "values")):
+            view = room.as_strided((2, 1, 130, 32), (step[0], 32, step[1], 1), 32 * i
+                                   if far == "row" else 130 * 32 * i)
+            t[n] = view.copy_(t[n])
+        check_attn(run_attn("cuda", t), attn_oracle(a))
+
+    @pytest.mark.gpu
     def test_broadcast_inputs(self):
         # one context set for a whole batch: gradients sum over it
         a = attn_inputs(3, 2, 2, 10, 20, 8, 16, torch.float32)
@@ -554,6 +642,15 @@ class TestDifferentialAttention:
             out = ops.differential_attention(t["keys"], t["queries"], t["values"], t["lam"])
             for w, g in zip(want, torch.autograd.grad(out, [t[names[w]] for w in want], t["dout"])):
                 assert torch.equal(g, full[w]), w
+
+    @pytest.mark.gpu
+    def test_differentiable_once(self):
+        a = {n: t.cuda().requires_grad_(True) for n, t in
+             attn_inputs(1, 1, 1, 3, 5, 4, 8, torch.float32).items()}
+        out = ops.differential_attention(a["keys"], a["queries"], a["values"], a["lam"])
+        (dq,) = torch.autograd.grad(out.sum(), a["queries"], create_graph=True)
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            dq.sum().backward()
 
     @pytest.mark.gpu
     def test_empty(self):
@@ -943,6 +1040,62 @@ class TestTogether:
             for _, call, _, out in runs:
                 with torch.no_grad():
                     assert torch.equal(out, call())
+
+    @pytest.mark.gpu
+    def test_captured_training_call(self):
+        """Forward and backward of both operators in one graph, replayed on new
+        inputs between eager work."""
+        a = {n: t.cuda() for n, t in
+             attn_inputs(2, 4, 2, 140, 600, 16, 32, torch.bfloat16).items()}
+        w = torch.randn(32, device="cuda")
+
+        def call():
+            t = {n: x.detach().requires_grad_(n != "dout") for n, x in a.items()}
+            wg = w.detach().requires_grad_(True)
+            out = ops.differential_attention(t["keys"], t["queries"], t["values"], t["lam"])
+            out = ops.layer_norm(out, wg)
+            leaves = [t[n] for n in ("keys", "queries", "values", "lam")] + [wg]
+            return (out.detach(), *torch.autograd.grad(out, leaves, t["dout"]))
+
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            call()
+        torch.cuda.current_stream().wait_stream(side)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            static = call()
+        for i in range(4):
+            for n in ("queries", "keys", "dout"):
+                a[n].normal_()
+            g.replay()
+            torch.cuda.synchronize()
+            for x, y in zip(static, call()):
+                assert torch.equal(x, y)
+
+    @pytest.mark.gpu
+    def test_captured_clipping(self):
+        params = params_of(SHAPES, torch.float32, "cuda")
+        grads = [p.grad.clone() for p in params]
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            ops.clip_grad_norm_(params, 0.5)
+        torch.cuda.current_stream().wait_stream(side)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            total = ops.clip_grad_norm_(params, 0.5)
+        for i in range(4):
+            for p, x in zip(params, grads):
+                p.grad.copy_(x * (i + 1))
+            eager = params_of(SHAPES, torch.float32, "cuda")
+            for p, x in zip(eager, grads):
+                p.grad.copy_(x * (i + 1))
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(total, ops.clip_grad_norm_(eager, 0.5))
+            for p, q in zip(params, eager):
+                assert torch.equal(p.grad, q.grad)
 
     @pytest.mark.gpu
     def test_own_stream(self):
