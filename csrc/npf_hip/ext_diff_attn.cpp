@@ -30,7 +30,8 @@ void check_heads(const Tensor& t, const Tensor& q, const char* name) {
 // memory [B, length, heads, size], as the projection that follows wants it
 Tensor heads_like(const Tensor& q, int64_t B, int64_t H, int64_t L,
                   int64_t size) {
-  return torch::empty({B, L, H, size}, q.options()).transpose(1, 2);
+  return torch::empty_strided({B, H, L, size},
+                              {L * H * size, size, H * size, 1}, q.options());
 }
 
 NpfDiffAttnArgs common_args(const Tensor& q, const Tensor& k, const Tensor& v,
@@ -164,8 +165,7 @@ struct DiffAttn : torch::autograd::Function<DiffAttn> {
         if (t->defined()) t->zero_();
     } else {
       const long rows = (long)a.B * a.H * a.Q;
-      Tensor stats = torch::empty({rows, 4}, lse.options());
-      Tensor dlam_rows = torch::empty({a.dq_splits * rows}, lse.options());
+      Tensor stats = torch::empty({(4 + a.dq_splits) * rows}, lse.options());
       // parts of split sums
       Tensor dq_part, dk_part, dv_part;
       auto parts = [&](Tensor& part, const Tensor& grad, int splits) {
@@ -181,7 +181,7 @@ struct DiffAttn : torch::autograd::Function<DiffAttn> {
       a.dout = heads_of(dout);
       a.lse = lse.data_ptr<float>();
       a.stats = stats.data_ptr<float>();
-      a.dlam_rows = dlam_rows.data_ptr<float>();
+      a.dlam_rows = a.stats + 4 * rows;
       if (dq.defined()) a.dq = heads_of(dq);
       if (dk.defined()) a.dk = heads_of(dk);
       if (dv.defined()) a.dv = heads_of(dv);
