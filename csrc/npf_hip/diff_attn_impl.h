@@ -27,11 +27,14 @@ struct Shape {
                                               : (kPad <= 16 ? 2 : 1);
   // What a wave's registers hold decides how the gradients share launches: of
   // the keys both at once, else dk and dv apart, else dk of each map apart; of
-  // the queries both maps at once, else apart.
+  // the queries both maps at once, else apart.  (Long: dk and dv apart 988 us,
+  // together 1260; heads of 128, 2 x 8 x 1024 x 1024, a whole step with dk of
+  // each map apart: bf16 299 us, together 517.)
   static constexpr bool kBothGrads = kPad * (int)sizeof(T) < 128;
   static constexpr bool kDkMapsApart = kPad == 128;
   static constexpr bool kDqMapsApart = kPad * (int)sizeof(T) > 256;
   // whether the dq kernel keeps its queries in LDS rather than in registers
+  // (long: 529 us, 704 with one wave a SIMD, 814 with two that spill)
   static constexpr bool kQueriesInLds = sizeof(T) == 2 && kPad == 64;
   // parts of the values' columns that forward blocks take: the sums of 256
   // columns for two maps would fill a wave's registers by themselves
@@ -42,7 +45,8 @@ struct Shape {
 };
 
 // Waves a SIMD is to hold: two, in half of the registers each and with every
-// matrix result in ordinary registers, where a kernel fits; else one.
+// matrix result in ordinary registers, where a kernel fits; else one.  (Long
+// training bf16, forward: 794 us with one, 475 with two; two that spill, 1384.)
 template <typename T, int kPad>
 constexpr int kResident = kPad * (int)sizeof(T) <= 128 ? 2 : 1;
 
@@ -73,6 +77,23 @@ __device__ __forceinline__ float exp_tile(f32x16& s, float c, float m) {
   return sum;
 }
 
+// Measured (one MI355X; "long": 2 x 16 heads on 4, 4096 x 4096, maps of 64,
+// bf16; "image": 16 x 4 heads, 1024 x 1024, maps of 16):
+//
+//            long bf16               image bf16   bound by
+//   forward  475 us, 0.58 PFLOP/s      36 us      vector unit 66% (image 88%)
+//   dq       529 us                    42 us      and matrix unit 49% of the
+//   dk, dv   582 + 406 us              51 us      time, at 1.9 GHz
+//
+// A pair of scores costs two exponents (8 clocks a 64-lane wave each) and about
+// 9 other vector operations a lane; the matrix unit works beside them as long
+// as a SIMD has a second wave.  LDS is read at less than half of its rate, and
+// without bank conflicts.
+
+// Forward: a wave holds 32 query rows and passes over the keys.  Blocks of four
+// waves share the tiles; with up to 32 rows a head, blocks of one wave split
+// the keys between them (single queries against 32768 keys, 200 MB of bf16: 52
+// us, 3.9 TB/s, and 8 us to join).
 template <typename T, int kPad, int kWaves, bool kDirect>
 __global__ void __launch_bounds__(64 * kWaves, (kResident<T, kPad>))
     diff_fwd(NpfDiffAttnArgs a) {
@@ -292,15 +313,18 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, kPad>))
   }
 }
 
+constexpr int kBwdWaves = 4;  // of a backward block
+
 // dq of the maps in kMaps (bits), and with the second map each row's part of
 // dlam: a wave holds 32 query rows and passes over the keys
-template <typename T, int kPad, int kWaves, bool kDirect, int kMaps>
-__global__ void __launch_bounds__(64 * kWaves, (kResident<T, kPad>))
+template <typename T, int kPad, bool kDirect, int kMaps>
+__global__ void __launch_bounds__(64 * kBwdWaves, (kResident<T, kPad>))
     diff_bwd_dq(NpfDiffAttnArgs a) {
   using S = Shape<T, kPad>;
   using Lds = Tile<T, S::kWidth>;
+  constexpr int kWaves = kBwdWaves;
   constexpr bool kInLds = S::kQueriesInLds;
-  constexpr int kTile = kWaves == 1 || kInLds ? 32 * S::kSubs : S::kTile;
+  constexpr int kTile = kInLds ? 32 * S::kSubs : S::kTile;
   constexpr int kSubs = S::kSubs;
   constexpr int kTileBytes = kTile * S::kRowBytes;
   // two objects, so that it shows that the next tiles' loads do not touch
@@ -504,11 +528,12 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, kPad>))
 
 // dk of the maps in kMaps (bits) and, with kDv, dv: a wave holds 32 keys and
 // passes over the queries of the heads that share them
-template <typename T, int kPad, int kWaves, bool kDirect, int kMaps, bool kDv>
-__global__ void __launch_bounds__(64 * kWaves, (kResident<T, kPad>))
+template <typename T, int kPad, bool kDirect, int kMaps, bool kDv>
+__global__ void __launch_bounds__(64 * kBwdWaves, (kResident<T, kPad>))
     diff_bwd_dkv(NpfDiffAttnArgs a) {
   using S = Shape<T, kPad>;
   using Lds = Tile<T, S::kWidth>;
+  constexpr int kWaves = kBwdWaves;
   constexpr bool kDk = kMaps != 0;
   constexpr int kTile = kDk && !S::kBothGrads ? 32 : S::kTile;
   constexpr int kTileBytes = kTile * S::kRowBytes;
@@ -543,10 +568,10 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, kPad>))
     u32x4 x{0, 0, 0, 0}, y{0, 0, 0, 0};
     if (live) {
       x = load_chunk(row_of<T>(a.k, b, hk, key),
-                              chunk_of_maps<T, kPad>(u * 2 + half, a.D));
+                     chunk_of_maps<T, kPad>(u * 2 + half, a.D));
       if (kDk)
         y = load_chunk(row_of<T>(a.v, b, hk, key),
-                                chunk_of_row<T>(u * 2 + half, a.Dv));
+                       chunk_of_row<T>(u * 2 + half, a.Dv));
     }
     kf[u / S::kSteps][u % S::kSteps] = x;
     vf[u] = y;
@@ -757,12 +782,12 @@ hipError_t bwd_sized(const NpfDiffAttnArgs& a, hipStream_t stream) {
   hipError_t e = hipSuccess;
   auto dq = [&](auto maps) {
     if (e == hipSuccess)
-      e = launch(diff_bwd_dq<T, kPad, 4, kDirect, decltype(maps)::value>,
+      e = launch(diff_bwd_dq<T, kPad, kDirect, decltype(maps)::value>,
                  heads * a.dq_splits * ((rows + 127) / 128), 256, a, stream);
   };
   auto dkv = [&](auto maps, auto with_dv) {
     if (e == hipSuccess)
-      e = launch(diff_bwd_dkv<T, kPad, 4, kDirect, decltype(maps)::value,
+      e = launch(diff_bwd_dkv<T, kPad, kDirect, decltype(maps)::value,
                               decltype(with_dv)::value>,
                  heads * a.dkv_splits * ((a.K + 127) / 128), 256, a, stream);
   };

@@ -7,6 +7,11 @@
 // order (every block for itself: a few thousand values) and scales.  No
 // atomics, so the result does not change between runs.  Sums are held in 64
 // bits: squares of 32-bit values neither overflow nor lose small terms.
+//
+// Measured (one MI355X), 492 MB of bf16 in 48 tensors: norm 114 us (4.3 TB/s;
+// reading alone, a sum of 1 GiB reaches 4.0), scaling 154 us (6.4 TB/s, part
+// of it from the cache that the norm has filled): memory bounds both.  32
+// tensors of one small model (1 MB): 6 and 5 us, launches.
 
 #include "common.h"
 #include "grad_norm.h"
