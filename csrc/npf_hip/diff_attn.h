@@ -19,7 +19,7 @@ struct NpfDiffAttnArgs {
   void* dlam;             // backward: [lam_heads], or null
   const void* lam;
   const void* lengths;    // [B] int32 or int64, or null
-  void* split;            // forward: workspace of a split key axis
+  void* split;            // forward: the parts of a result that is joined
   float* dq_part;         // backward: parts of a split sum, [dq_splits, B, H,
   float* dk_part;         // Q, 2D] and [dkv_splits, B, Hk, K, 2D or Dv], where
   float* dv_part;         // there are several

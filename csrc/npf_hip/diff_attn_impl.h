@@ -29,17 +29,29 @@ struct Shape {
   // the keys both at once, else dk and dv apart, else dk of each map apart; of
   // the queries both maps at once, else apart.  (Long: dk and dv apart 988 us,
   // together 1260; heads of 128, 2 x 8 x 1024 x 1024, a whole step with dk of
-  // each map apart: bf16 299 us, together 517.)
+  // each map apart: bf16 313 us, together 517.)
   static constexpr bool kBothGrads = kPad * (int)sizeof(T) < 128;
   static constexpr bool kDkMapsApart = kPad == 128;
   static constexpr bool kDqMapsApart = kPad * (int)sizeof(T) > 256;
   // whether the dq kernel keeps its queries in LDS rather than in registers
   // (long: 529 us, 704 with one wave a SIMD, 814 with two that spill)
   static constexpr bool kQueriesInLds = sizeof(T) == 2 && kPad == 64;
-  // parts of the values' columns that forward blocks take: the sums of 256
-  // columns for two maps would fill a wave's registers by themselves
-  static constexpr int kParts = kPad == 128 ? 2 : 1;
+  // forward blocks of one map each, joined like parts of a split key axis: the
+  // sums of 256 columns for two maps would fill a wave's registers alone.
+  // (8 heads, bf16: 4096 x 4096 269 us, with half of the columns of both maps
+  // a block 479; 8 x 256 x 256, where the join counts most, a step 159 and 145.)
+  static constexpr bool kMapsApart = kPad == 128;
   static constexpr int kSteps = kPad / (2 * kChunk<T>);  // chunk pairs a map
+
+  // Whether value `at` of `all` padded ones, of which `size` are there, is to
+  // be computed: the widest fp32 products leave out a last quarter of pure
+  // padding (a step at heads of 96: 1178 us to 983); the others are taken
+  // whole (the same question at heads of 64: 516 us to 570).
+  __device__ static __forceinline__ bool counts(int at, int all, int size) {
+    if (sizeof(T) == 2 || kPad < 128 || 2 * at < all) return true;
+    return at / (all / 4) * (all / 4) < size;
+  }
+
   static constexpr int kBlocks = kWidth / 32;  // 32 columns of a whole row
   static constexpr int kMapBlocks = kPad / 32 > 0 ? kPad / 32 : 1;
 };
@@ -47,8 +59,10 @@ struct Shape {
 // Waves a SIMD is to hold: two, in half of the registers each and with every
 // matrix result in ordinary registers, where a kernel fits; else one.  (Long
 // training bf16, forward: 794 us with one, 475 with two; two that spill, 1384.)
-template <typename T, int kPad>
-constexpr int kResident = kPad * (int)sizeof(T) <= 128 ? 2 : 1;
+// Kernels of one map fit at twice the size.
+template <typename T, int kPad, bool kOneMap = false>
+constexpr int kResident =
+    kPad * (int)sizeof(T) <= (kOneMap && sizeof(T) == 2 ? 256 : 128) ? 2 : 1;
 
 // Columns that block n of map m starts at.  Maps of 16 share one block: each
 // accumulates it whole and keeps its half.
@@ -95,12 +109,13 @@ __device__ __forceinline__ float exp_tile(f32x16& s, float c, float m) {
 // the keys between them (single queries against 32768 keys, 200 MB of bf16: 52
 // us, 3.9 TB/s, and 8 us to join).
 template <typename T, int kPad, int kWaves, bool kDirect>
-__global__ void __launch_bounds__(64 * kWaves, (kResident<T, kPad>))
+__global__ void __launch_bounds__(
+    64 * kWaves, (kResident<T, kPad, Shape<T, kPad>::kMapsApart>))
     diff_fwd(NpfDiffAttnArgs a) {
   using S = Shape<T, kPad>;
   using Lds = Tile<T, S::kWidth>;
   constexpr int kTile = kWaves == 1 ? 32 * S::kSubs : S::kTile;
-  constexpr int kSubs = S::kSubs, kCols = S::kBlocks / S::kParts;
+  constexpr int kSubs = S::kSubs, kMaps = S::kMapsApart ? 1 : 2;
   constexpr int kTileBytes = kTile * S::kRowBytes;
   // two objects, so that it shows that the next tiles' loads do not touch
   // what is being read
@@ -115,7 +130,8 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, kPad>))
   // shared, and neighbours in memory are read at a time (single queries
   // against 32768 keys: 52 us rather than 66).
   const int heads = a.B * a.Hk;
-  const int part = blockIdx.x % S::kParts, id = blockIdx.x / S::kParts;
+  const int first = S::kMapsApart ? blockIdx.x % 2 : 0;  // of its maps
+  const int id = S::kMapsApart ? blockIdx.x / 2 : blockIdx.x;
   int bh, row_tile, split;
   if (kWaves == 1) {
     split = id % a.splits;
@@ -141,32 +157,34 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, kPad>))
     end = n - begin < per ? n : begin + per;
   }
 
-  u32x4 qf[2][S::kSteps];
+  u32x4 qf[kMaps][S::kSteps];
 #pragma unroll
-  for (int m = 0; m < 2; ++m)
+  for (int m = 0; m < kMaps; ++m)
 #pragma unroll
     for (int u = 0; u < S::kSteps; ++u) {
       const ChunkOf c =
-          chunk_of_maps<T, kPad>((m * S::kSteps + u) * 2 + half, a.D);
+          chunk_of_maps<T, kPad>(((first + m) * S::kSteps + u) * 2 + half, a.D);
       qf[m][u] = u32x4{0, 0, 0, 0};
       if (live) qf[m][u] = load_chunk(row_of<T>(a.q, b, h, q), c);
     }
 
-  f32x16 o[2][kCols];
+  f32x16 o[kMaps][S::kBlocks];
+  float mx[kMaps], l[kMaps];
 #pragma unroll
-  for (int m = 0; m < 2; ++m)
+  for (int m = 0; m < kMaps; ++m) {
+    mx[m] = kLowest;
+    l[m] = 0.f;
 #pragma unroll
-    for (int j = 0; j < kCols; ++j) o[m][j] = f32x16{};
-  float mx[2] = {kLowest, kLowest}, l[2] = {0.f, 0.f};
+    for (int j = 0; j < S::kBlocks; ++j) o[m][j] = f32x16{};
+  }
   const float c = a.scale * kLog2e;
 
   Stage<T, S::kWidth, kTile, 64 * kWaves, kDirect> stage;
   const T* kp = row_of<T>(a.k, b, hk, 0);
   const T* vp = row_of<T>(a.v, b, hk, 0);
-  // the columns that this block's part begins with, in bytes of a row
-  const int part_cols = part * kCols * 32 * (int)sizeof(T);
   // one tile from LDS; kEdge: it may reach behind the last key
-  const int rows_base = Lds::rows_base(lane), cols_base = Lds::cols_base(lane);
+  const int rows_base = Lds::rows_base(lane) ^ (first * S::kSteps << 5);
+  const int cols_base = Lds::cols_base(lane);
   auto pass = [&](auto edge, int k0, const char* kt) {
     constexpr bool kEdge = decltype(edge)::value;
     const char* vt = kt + kTileBytes;
@@ -174,17 +192,18 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, kPad>))
 #pragma unroll
     for (int sub0 = 0; sub0 < kTile; sub0 += 32 * kSubs) {
       if (kEdge && k0 + sub0 >= end) break;
-      f32x16 s[2][kSubs];
+      f32x16 s[kMaps][kSubs];
 #pragma unroll
-      for (int m = 0; m < 2; ++m)
+      for (int m = 0; m < kMaps; ++m)
 #pragma unroll
         for (int t = 0; t < kSubs; ++t) {
           s[m][t] = f32x16{};
 #pragma unroll
           for (int u = 0; u < S::kSteps; ++u)
-            s[m][t] = mma_chunk<T>(
-                Lds::rows(kt, rb, sub0 + 32 * t, m * S::kSteps + u), qf[m][u],
-                s[m][t]);
+            if (S::counts(u * 2 * kChunk<T>, kPad, a.D))
+              s[m][t] = mma_chunk<T>(
+                  Lds::rows(kt, rb, sub0 + 32 * t, m * S::kSteps + u),
+                  qf[m][u], s[m][t]);
         }
       if constexpr (kEdge) {
 #pragma unroll
@@ -192,10 +211,11 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, kPad>))
 #pragma unroll
           for (int i = 0; i < 16; ++i)
             if (k0 + sub0 + 32 * t + reg_row(i) + 4 * half >= end)
-              s[0][t][i] = s[1][t][i] = -INFINITY;
+#pragma unroll
+              for (int m = 0; m < kMaps; ++m) s[m][t][i] = -INFINITY;
       }
 #pragma unroll
-      for (int m = 0; m < 2; ++m) {
+      for (int m = 0; m < kMaps; ++m) {
         float top = s[m][0][0];
 #pragma unroll
         for (int t = 0; t < kSubs; ++t)
@@ -211,19 +231,32 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, kPad>))
           mx[m] = up;
           l[m] *= f;
 #pragma unroll
-          for (int j = 0; j < kCols; ++j) o[m][j] *= f;
+          for (int j = 0; j < S::kBlocks; ++j) o[m][j] *= f;
         }
       }
 #pragma unroll
       for (int t = 0; t < kSubs; ++t) {
-        l[0] += exp_tile(s[0][t], c, mx[0]);
-        l[1] += exp_tile(s[1][t], c, mx[1]);
-        const Operand<T> p[2] = {Operand<T>(s[0][t]), Operand<T>(s[1][t])};
 #pragma unroll
-        for (int j = 0; j < kCols; ++j) {
-          f32x16* const acc[2] = {&o[0][j], &o[1][j]};
-          Lds::template transposed<2>(vt, cb ^ part_cols, sub0 + 32 * t, 32 * j,
-                                      p, acc);
+        for (int m = 0; m < kMaps; ++m)
+          l[m] += exp_tile(s[m][t], c, mx[m]);
+        if constexpr (kMaps == 2) {
+          const Operand<T> p[2] = {Operand<T>(s[0][t]), Operand<T>(s[1][t])};
+#pragma unroll
+          for (int j = 0; j < S::kBlocks; ++j) {
+            f32x16* const acc[2] = {&o[0][j], &o[1][j]};
+            if (S::counts(32 * j, 2 * kPad, a.Dv))
+              Lds::template transposed<2>(vt, cb, sub0 + 32 * t, 32 * j, p,
+                                          acc);
+          }
+        } else {
+          const Operand<T> p[1] = {Operand<T>(s[0][t])};
+#pragma unroll
+          for (int j = 0; j < S::kBlocks; ++j) {
+            f32x16* const acc[1] = {&o[0][j]};
+            if (S::counts(32 * j, 2 * kPad, a.Dv))
+              Lds::template transposed<1>(vt, cb, sub0 + 32 * t, 32 * j, p,
+                                          acc);
+          }
         }
       }
     }
@@ -259,57 +292,56 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, kPad>))
   if (k0 < end) pass(std::true_type{}, k0, full & 1 ? odd : even);
 
 #pragma unroll
-  for (int m = 0; m < 2; ++m) l[m] = both_sum(l[m]);
+  for (int m = 0; m < kMaps; ++m) l[m] = both_sum(l[m]);
   if (!live) return;
-  if (a.splits > 1) {
+  if (S::kMapsApart || a.splits > 1) {
     float* w = static_cast<float*>(a.split) +
                ((long)bh * rows + row) * a.splits * split_row_floats(a.Dv) +
                split * split_row_floats(a.Dv);
-    if (half == 0 && part == 0) {
 #pragma unroll
-      for (int m = 0; m < 2; ++m) {
-        w[2 * m] = mx[m];
-        w[2 * m + 1] = l[m];
+    for (int m = 0; m < kMaps; ++m) {
+      if (half == 0) {
+        w[2 * (first + m)] = mx[m];
+        w[2 * (first + m) + 1] = l[m];
       }
-    }
-    w += 4;
 #pragma unroll
-    for (int m = 0; m < 2; ++m)
-#pragma unroll
-      for (int j = 0; j < kCols; ++j)
+      for (int j = 0; j < S::kBlocks; ++j)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          const int d = 32 * (part * kCols + j) + 8 * g + 4 * half;
+          const int d = 32 * j + 8 * g + 4 * half;
           const f32x16& x = o[m][j];
-          store4(w + m * a.Dv + d, a.Dv - d, x[4 * g], x[4 * g + 1],
-                 x[4 * g + 2], x[4 * g + 3]);
+          store4(w + 4 + (first + m) * a.Dv + d, a.Dv - d, x[4 * g],
+                 x[4 * g + 1], x[4 * g + 2], x[4 * g + 3]);
         }
+    }
     return;
   }
-  const float lam = lam_of(a, h);
-  // rows without keys: zeros; all else divides, so that sums that are no
-  // number show
-  const float i1 = n ? 1.f / l[0] : 0.f, i2 = n ? 1.f / l[1] : 0.f;
-  T* out = row_of<T>(a.out, b, h, q);
-  T* o2 = a.o2.p ? row_of<T>(a.o2, b, h, q) : nullptr;
+  if constexpr (!S::kMapsApart) {
+    const float lam = lam_of(a, h);
+    // rows without keys: zeros; all else divides, so that sums that are no
+    // number show
+    const float i1 = n ? 1.f / l[0] : 0.f, i2 = n ? 1.f / l[1] : 0.f;
+    T* out = row_of<T>(a.out, b, h, q);
+    T* o2 = a.o2.p ? row_of<T>(a.o2, b, h, q) : nullptr;
 #pragma unroll
-  for (int j = 0; j < kCols; ++j)
+    for (int j = 0; j < S::kBlocks; ++j)
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int d = 32 * (part * kCols + j) + 8 * g + 4 * half;
-      float x[4], y[4];
+      for (int g = 0; g < 4; ++g) {
+        const int d = 32 * j + 8 * g + 4 * half;
+        float x[4], y[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        y[e] = o[1][j][4 * g + e] * i2;
-        x[e] = o[0][j][4 * g + e] * i1 - lam * y[e];
+        for (int e = 0; e < 4; ++e) {
+          y[e] = o[1][j][4 * g + e] * i2;
+          x[e] = o[0][j][4 * g + e] * i1 - lam * y[e];
+        }
+        store4(out + d, a.Dv - d, x[0], x[1], x[2], x[3]);
+        if (o2) store4(o2 + d, a.Dv - d, y[0], y[1], y[2], y[3]);
       }
-      store4(out + d, a.Dv - d, x[0], x[1], x[2], x[3]);
-      if (o2) store4(o2 + d, a.Dv - d, y[0], y[1], y[2], y[3]);
-    }
-  if (a.lse && half == 0 && part == 0) {
-    float* p = a.lse + (((long)b * a.H + h) * a.Q + q) * 2;
+    if (a.lse && half == 0) {
+      float* p = a.lse + (((long)b * a.H + h) * a.Q + q) * 2;
 #pragma unroll
-    for (int m = 0; m < 2; ++m) p[m] = n ? mx[m] + __log2f(l[m]) : 0.f;
+      for (int m = 0; m < 2; ++m) p[m] = n ? mx[m] + __log2f(l[m]) : 0.f;
+    }
   }
 }
 
@@ -427,7 +459,9 @@ __global__ void __launch_bounds__(64 * kBwdWaves, (kResident<T, kPad>))
         for (int i = 0; i < 16; ++i) g[t][i] = -st.z;
 #pragma unroll
         for (int u = 0; u < 2 * S::kSteps; ++u)
-          g[t] = mma_chunk<T>(Lds::rows(vt, rb, sub0 + 32 * t, u), gf[u], g[t]);
+          if (S::counts(u * 2 * kChunk<T>, 2 * kPad, a.Dv))
+            g[t] =
+                mma_chunk<T>(Lds::rows(vt, rb, sub0 + 32 * t, u), gf[u], g[t]);
       }
       if (kSubs == 1) __builtin_amdgcn_sched_barrier(0);
       // one map after the other: a second tile of scores would not fit
@@ -440,6 +474,7 @@ __global__ void __launch_bounds__(64 * kBwdWaves, (kResident<T, kPad>))
           s[t] = f32x16{};
 #pragma unroll
           for (int u = m * S::kSteps; u < (m + 1) * S::kSteps; ++u) {
+            if (!S::counts(u % S::kSteps * 2 * kChunk<T>, kPad, a.D)) continue;
             u32x4 x;
             if constexpr (kInLds)
               x = Lds::rows(own, rb, 0, u);
@@ -463,6 +498,7 @@ __global__ void __launch_bounds__(64 * kBwdWaves, (kResident<T, kPad>))
 #pragma unroll
           for (int j = 0; j < S::kMapBlocks; ++j) {
             f32x16* const acc[1] = {&dq[m][j]};
+            if (!S::counts(32 * j, kPad, a.D)) continue;
             Lds::template transposed<1>(kt, cb, sub0 + 32 * t,
                                         map_col<kPad>(m, j), ds, acc);
           }
@@ -529,7 +565,8 @@ __global__ void __launch_bounds__(64 * kBwdWaves, (kResident<T, kPad>))
 // dk of the maps in kMaps (bits) and, with kDv, dv: a wave holds 32 keys and
 // passes over the queries of the heads that share them
 template <typename T, int kPad, bool kDirect, int kMaps, bool kDv>
-__global__ void __launch_bounds__(64 * kBwdWaves, (kResident<T, kPad>))
+__global__ void __launch_bounds__(64 * kBwdWaves,
+                                  (kResident<T, kPad, !kDv && kMaps != 3>))
     diff_bwd_dkv(NpfDiffAttnArgs a) {
   using S = Shape<T, kPad>;
   using Lds = Tile<T, S::kWidth>;
@@ -633,8 +670,9 @@ __global__ void __launch_bounds__(64 * kBwdWaves, (kResident<T, kPad>))
         p[m] = kFromLse ? rows16(stats[m], sub, half) : f32x16{};
 #pragma unroll
         for (int u = 0; u < S::kSteps; ++u)
-          p[m] = mma_chunk<T>(Lds::rows(qt, rb, sub, m * S::kSteps + u),
-                              kf[m][u], p[m]);
+          if (S::counts(u * 2 * kChunk<T>, kPad, a.D))
+            p[m] = mma_chunk<T>(Lds::rows(qt, rb, sub, m * S::kSteps + u),
+                                kf[m][u], p[m]);
         if constexpr (kFromLse) {
 #pragma unroll
           for (int i = 0; i < 16; ++i)
@@ -655,6 +693,7 @@ __global__ void __launch_bounds__(64 * kBwdWaves, (kResident<T, kPad>))
 #pragma unroll
         for (int j = 0; j < S::kBlocks; ++j) {
           f32x16* const acc[1] = {&dv[j]};
+          if (!S::counts(32 * j, 2 * kPad, a.Dv)) continue;
           Lds::template transposed<1>(gt, cb, sub, 32 * j, map, acc);
           // (reads of later columns would be taken ahead into registers that
           // are not there)
@@ -665,7 +704,8 @@ __global__ void __launch_bounds__(64 * kBwdWaves, (kResident<T, kPad>))
         x = rows16(stats[2], sub, half);
 #pragma unroll
         for (int u = 0; u < 2 * S::kSteps; ++u)
-          x = mma_chunk<T>(Lds::rows(gt, rb, sub, u), vf[u], x);
+          if (S::counts(u * 2 * kChunk<T>, 2 * kPad, a.Dv))
+            x = mma_chunk<T>(Lds::rows(gt, rb, sub, u), vf[u], x);
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
           if (!(kMaps >> m & 1)) continue;
@@ -677,6 +717,7 @@ __global__ void __launch_bounds__(64 * kBwdWaves, (kResident<T, kPad>))
 #pragma unroll
           for (int j = 0; j < S::kMapBlocks; ++j) {
             f32x16* const acc[1] = {&dk[m][j]};
+            if (!S::counts(32 * j, kPad, a.D)) continue;
             Lds::template transposed<1>(qt, cb, sub, map_col<kPad>(m, j), ds,
                                         acc);
           }
@@ -767,7 +808,7 @@ template <typename T, int kPad, bool kDirect>
 hipError_t fwd_sized(const NpfDiffAttnArgs& a, hipStream_t stream) {
   using S = Shape<T, kPad>;
   const long heads = (long)a.B * a.Hk, rows = (long)(a.H / a.Hk) * a.Q;
-  const long each = heads * a.splits * S::kParts;
+  const long each = heads * a.splits * (S::kMapsApart ? 2 : 1);
   if (a.waves == 1)
     return launch(diff_fwd<T, kPad, 1, kDirect>, each * ((rows + 31) / 32), 64,
                   a, stream);
