@@ -529,7 +529,8 @@ class DifferentialAttender(nn.Module):
     @staticmethod
     def _heads(x, n_heads):
         """[B, N, H*h] -> [B, H, N, h], a view."""
-        return x.view(*x.shape[:2], n_heads, -1).transpose(1, 2)
+        # (the size is given: with no contexts it would not follow)
+        return x.view(*x.shape[:2], n_heads, x.shape[-1] // n_heads).transpose(1, 2)
 
 
 @_register("differential_transformer")

@@ -884,6 +884,19 @@ class TestAttenders:
         # 64 roundings of values below 16
         assert (alone - out[1:2]).abs().max() <= 64 * 16 * E32
 
+    @pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+    @pytest.mark.parametrize("name", ["differential", "differential_transformer"])
+    @pytest.mark.parametrize("B, K, Q", [(2, 0, 3), (2, 3, 0), (0, 3, 2)])
+    def test_nothing_to_attend(self, device, name, B, K, Q):
+        att = get_attender(name, 16, 16, 16, n_heads=2).to(device)
+        keys, queries, values = (torch.randn(B, n, 16, device=device, requires_grad=True)
+                                 for n in (K, Q, K))
+        out = att(keys, queries, values)
+        assert out.shape == (B, Q, 16) and torch.isfinite(out).all()
+        out.sum().backward()
+        for p in (*att.parameters(), keys, queries, values):
+            assert p.grad is not None and torch.isfinite(p.grad).all()
+
     def test_permutation_of_contexts(self):
         torch.manual_seed(0)
         att = get_attender("differential", 16, 16, 16, n_heads=2, depth=3)
