@@ -25,7 +25,8 @@ struct NpfDiffAttnArgs {
   float* dv_part;         // there are several
   float scale;
   int B, H, Hk, Q, K, D, Dv;
-  int type, lam_type, lam_stride;
+  int type, lam_type;
+  long lam_stride;
   int lam_heads;          // values of lam: H or 1
   int lengths64;
   // the plan

@@ -359,7 +359,7 @@ __device__ __forceinline__ int keys_of(const NpfDiffAttnArgs& a, int b) {
 }
 
 __device__ __forceinline__ float lam_of(const NpfDiffAttnArgs& a, int h) {
-  return load_coded(a.lam, a.lam_type, (long)h * a.lam_stride);
+  return load_coded(a.lam, a.lam_type, h * a.lam_stride);
 }
 
 // x of the other lane half, for a reduction over both

@@ -41,8 +41,9 @@ NpfDiffAttnArgs common_args(const Tensor& q, const Tensor& k, const Tensor& v,
   check_heads(k, q, "keys");
   check_heads(v, q, "values");
   NpfDiffAttnArgs a{};
-  // rows are counted in 31 bits; offsets in memory are not
-  const int64_t most = std::numeric_limits<int>::max();
+  // rows are counted in 31 bits, up to a block's behind the last one; offsets
+  // in memory are not
+  const int64_t most = std::numeric_limits<int>::max() - 1024;
   TORCH_CHECK_VALUE(q.size(0) * q.size(1) * q.size(2) <= most &&
                         q.size(0) * k.size(1) * k.size(2) <= most &&
                         k.size(2) <= most / 2 && q.size(2) <= most / 2,
@@ -57,7 +58,7 @@ NpfDiffAttnArgs common_args(const Tensor& q, const Tensor& k, const Tensor& v,
   TORCH_CHECK_VALUE(q.size(3) == 2 * a.D && k.size(3) == 2 * a.D && a.D >= 1 &&
                         a.D <= 128,
                     "queries and keys must hold two maps of 1 to 128 values");
-  TORCH_CHECK_VALUE(a.Dv >= 1 && a.Dv <= 256,
+  TORCH_CHECK_VALUE(v.size(3) >= 1 && v.size(3) <= 256,
                     "values must have 1 to 256 values a head");
   TORCH_CHECK_VALUE(k.size(0) == a.B && v.size(0) == a.B &&
                         v.size(1) == a.Hk && v.size(2) == a.K,
@@ -71,7 +72,7 @@ NpfDiffAttnArgs common_args(const Tensor& q, const Tensor& k, const Tensor& v,
   a.lam = lam.data_ptr();
   a.lam_type = npf_type_code(lam, "lam", true);
   a.lam_heads = lam.dim() == 0 ? 1 : a.H;
-  a.lam_stride = lam.dim() == 0 ? 0 : (int)lam.stride(0);
+  a.lam_stride = lam.dim() == 0 ? 0 : lam.stride(0);
   if (lengths.defined()) {
     TORCH_CHECK_VALUE(lengths.dim() == 1 && lengths.size(0) == a.B &&
                           lengths.device() == q.device() &&

@@ -699,6 +699,24 @@ class TestDifferentialAttention:
         with pytest.raises(ValueError):
             f(k, q, torch.randn(2, 2, 5, 300, device="cuda"), lam)
 
+    @pytest.mark.gpu
+    def test_sizes_at_the_end_of_31_bits(self):
+        f = ops.differential_attention
+        k, lam = torch.zeros(1, 1, 1, 2, device="cuda"), torch.tensor(0.5, device="cuda")
+        with pytest.raises(ValueError, match="too many rows"):
+            f(k, k.expand(1, 1, 2 ** 31 - 64, 2), k, lam)
+        with pytest.raises(ValueError, match="too many rows"):
+            f(k.expand(1, 1, 2 ** 30, 2), k, k.expand(1, 1, 2 ** 30, 2), lam)
+        bf16 = dict(dtype=torch.bfloat16, device="cuda")
+        # a size whose low 32 bits would be one that is taken
+        with pytest.raises(ValueError, match="1 to 256"):
+            f(k.bfloat16(), k.bfloat16(), torch.empty(1, 1, 1, 2 ** 32 + 64, **bf16), lam)
+        a = attn_inputs(1, 2, 1, 5, 9, 8, 16, torch.float32)
+        room = torch.empty(2, 2 ** 31 + 8, **bf16)[:, 3]
+        a["lam"] = room.copy_(a["lam"])
+        want = attn_oracle({n: t.cpu() for n, t in a.items()})
+        check_attn(run_attn("cuda", a), want)
+
 
 # --------------------------------------------------------------------------- #
 # gradient norm and clipping
