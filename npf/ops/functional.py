@@ -1010,12 +1010,14 @@ def _grad_norm_ref(grads, norm_type):
     return torch.linalg.vector_norm(torch.stack(norms), norm_type)
 
 
+@torch.no_grad()
 def grad_norm(parameters, norm_type=2.0):
     """Norm of the gradients of `parameters` taken as one vector.
 
     parameters: a tensor or an iterable of tensors; those without a gradient
     are left out.  norm_type: 1, 2 or inf.  Returns a 0-d tensor on the
-    gradients' device (fp32 on a GPU, fp64 where a gradient is); no host wait.
+    gradients' device (fp32 on a GPU, fp64 where a gradient is), outside of any
+    autograd graph; no host wait.
     """
     params, grads = _with_gradients(parameters, norm_type)
     if grads is not None:
@@ -1023,6 +1025,7 @@ def grad_norm(parameters, norm_type=2.0):
     return _backend.extension().grad_norm(params, norm_type, -1.0)
 
 
+@torch.no_grad()
 def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
     """Scale the gradients of `parameters` in place so that their norm, taken
     as one vector, is at most `max_norm`; returns the norm before.

@@ -783,6 +783,17 @@ class TestGradClip:
             ops.clip_grad_norm_(params, 1.0, error_if_nonfinite=True)
         assert all(torch.equal(a, p.grad) for a, p in zip(before, params))
 
+    @pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+    def test_gradients_with_a_graph(self, device):
+        # of a backward pass that is itself differentiated
+        p = torch.tensor([3.0, 4.0], device=device, requires_grad=True)
+        p.pow(2).sum().backward(create_graph=True)
+        assert p.grad.requires_grad
+        assert not ops.grad_norm([p]).requires_grad
+        total = ops.clip_grad_norm_([p], 1.0)
+        assert not total.requires_grad and abs(total.item() - 10.0) <= 10 * 4 * E32
+        assert abs(p.grad.norm().item() - 1.0) <= 1e-6 + 16 * E32
+
     def test_nothing_to_clip(self):
         assert ops.clip_grad_norm_([], 1.0).item() == 0.0
         assert ops.grad_norm([torch.zeros(3, requires_grad=True)]).item() == 0.0
