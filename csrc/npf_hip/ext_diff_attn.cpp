@@ -30,8 +30,9 @@ void check_heads(const Tensor& t, const Tensor& q, const char* name) {
 // memory [B, length, heads, size], as the projection that follows wants it
 Tensor heads_like(const Tensor& q, int64_t B, int64_t H, int64_t L,
                   int64_t size) {
-  return torch::empty_strided({B, H, L, size},
-                              {L * H * size, size, H * size, 1}, q.options());
+  return torch::Tensor(at::detail::empty_strided_cuda(
+      {B, H, L, size}, {L * H * size, size, H * size, 1}, q.scalar_type(),
+      q.device()));
 }
 
 NpfDiffAttnArgs common_args(const Tensor& q, const Tensor& k, const Tensor& v,
@@ -105,15 +106,14 @@ Tensor attn_forward(const Tensor& q, const Tensor& k, const Tensor& v,
   a.out = heads_of(out);
   if (save) {
     *o2 = heads_like(q, a.B, a.H, a.Q, a.Dv);
-    *lse = torch::empty({(long)a.B * a.H * a.Q * 2},
-                        q.options().dtype(torch::kFloat32));
+    *lse = npf_empty({(long)a.B * a.H * a.Q * 2}, torch::kFloat32, q);
     a.o2 = heads_of(*o2);
     a.lse = lse->data_ptr<float>();
   }
   if (out.numel() == 0) return out;
   Tensor split;
   if (const long floats = npf_diff_attn_workspace(a)) {
-    split = torch::empty({floats}, q.options().dtype(torch::kFloat32));
+    split = npf_empty({floats}, torch::kFloat32, q);
     a.split = split.data_ptr();
   }
   npf_check(npf_diff_attn_fwd(a, at::hip::getCurrentHIPStream()),
@@ -160,18 +160,18 @@ struct DiffAttn : torch::autograd::Function<DiffAttn> {
     if (needs & 1) dk = heads_like(k, a.B, a.Hk, a.K, 2 * a.D);
     if (needs & 2) dq = heads_like(q, a.B, a.H, a.Q, 2 * a.D);
     if (needs & 4) dv = heads_like(v, a.B, a.Hk, a.K, a.Dv);
-    if (needs & 8) dlam = torch::empty(lam.sizes(), lam.options());
+    if (needs & 8) dlam = npf_empty(lam.sizes(), lam.scalar_type(), q);
     if (out.numel() == 0 || a.K == 0) {
       for (Tensor* t : {&dk, &dq, &dv, &dlam})
         if (t->defined()) t->zero_();
     } else {
       const long rows = (long)a.B * a.H * a.Q;
-      Tensor stats = torch::empty({(4 + a.dq_splits) * rows}, lse.options());
+      Tensor stats = npf_empty({(4 + a.dq_splits) * rows}, torch::kFloat32, q);
       // parts of split sums
       Tensor dq_part, dk_part, dv_part;
       auto parts = [&](Tensor& part, const Tensor& grad, int splits) {
         if (!grad.defined() || splits == 1) return (float*)nullptr;
-        part = torch::empty({splits * grad.numel()}, lse.options());
+        part = npf_empty({splits * grad.numel()}, torch::kFloat32, q);
         return part.data_ptr<float>();
       };
       a.dq_part = parts(dq_part, dq, a.dq_splits);

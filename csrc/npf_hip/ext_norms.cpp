@@ -63,15 +63,20 @@ NpfLayerNormArgs norm_args(const Tensor& x, const Tensor& residual,
   return a;
 }
 
-// mean and rstd are filled where they are defined
+// [2, rows]: means, and inverse deviations
+void set_stats(NpfLayerNormArgs& a, const Tensor& stats) {
+  a.mean = stats.data_ptr<float>();
+  a.rstd = a.mean + a.rows;
+}
+
+// `stats` are filled where they are defined
 void layer_norm_forward(const Tensor& x, const Tensor& residual,
                         const Tensor& weight, const Tensor& bias, double eps,
-                        Tensor& y, const Tensor& mean, const Tensor& rstd) {
+                        Tensor& y, const Tensor& stats) {
   NpfLayerNormArgs a = norm_args(x, residual, weight, bias);
   if (a.rows == 0) return;
   a.y = y.data_ptr();
-  a.mean = static_cast<float*>(ptr_of(mean));
-  a.rstd = static_cast<float*>(ptr_of(rstd));
+  if (stats.defined()) set_stats(a, stats);
   a.eps = (float)eps;
   npf_check(npf_layernorm_fwd(a, npf_type_code(x, "x"),
                               at::hip::getCurrentHIPStream()),
@@ -86,16 +91,14 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     const Tensor weight = weight_.value_or(Tensor());
     const Tensor bias = bias_.value_or(Tensor());
     const Tensor xr = rows_of(x), rr = rows_of(residual);
-    Tensor y = torch::empty(x.sizes(), x.options());
-    auto f32 = x.options().dtype(torch::kFloat32);
-    const Tensor mean = torch::empty({xr.size(0)}, f32);
-    const Tensor rstd = torch::empty({xr.size(0)}, f32);
-    layer_norm_forward(xr, rr, weight, bias, eps, y, mean, rstd);
+    Tensor y = npf_empty(x.sizes(), x.scalar_type(), x);
+    const Tensor stats = npf_empty({2, xr.size(0)}, torch::kFloat32, x);
+    layer_norm_forward(xr, rr, weight, bias, eps, y, stats);
     auto needs = [](const Tensor& t) { return t.defined() && t.requires_grad(); };
     ctx->saved_data["needs"] =
         (int64_t)(needs(x) + 2 * needs(residual) + 4 * needs(weight) +
                   8 * needs(bias));
-    ctx->save_for_backward({xr, rr, weight, bias, mean, rstd});
+    ctx->save_for_backward({xr, rr, weight, bias, stats});
     return y;
   }
 
@@ -105,14 +108,15 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     const auto saved = ctx->get_saved_variables();
     const int64_t needs = ctx->saved_data["needs"].toInt();
     const Tensor &x = saved[0], &residual = saved[1], &weight = saved[2],
-                 &bias = saved[3], &mean = saved[4], &rstd = saved[5];
+                 &bias = saved[3], &stats = saved[4];
     c10::DeviceGuard guard(x.device());
     NpfLayerNormArgs a = norm_args(x, residual, weight, bias);
     const Tensor dy = grads[0].contiguous();
     Tensor dx, dweight, dbias, partial;
-    if (needs & 3) dx = torch::empty(dy.sizes(), dy.options());
-    if (needs & 4) dweight = torch::empty_like(weight);
-    if (needs & 8) dbias = torch::empty_like(bias);
+    if (needs & 3) dx = npf_empty(dy.sizes(), dy.scalar_type(), dy);
+    if (needs & 4)
+      dweight = npf_empty(weight.sizes(), weight.scalar_type(), weight);
+    if (needs & 8) dbias = npf_empty(bias.sizes(), bias.scalar_type(), bias);
     if (a.rows == 0) {
       if (dweight.defined()) dweight.zero_();
       if (dbias.defined()) dbias.zero_();
@@ -120,13 +124,12 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
       const int type = npf_type_code(x, "x");
       if (needs & 12) {
         a.parts = npf_layernorm_parts(a, type);
-        partial = torch::empty({a.parts, 2, x.size(1)}, mean.options());
+        partial = npf_empty({a.parts, 2, x.size(1)}, torch::kFloat32, x);
         a.partial = partial.data_ptr<float>();
       }
       a.dy = dy.data_ptr();
       a.y = ptr_of(dx);
-      a.mean = mean.data_ptr<float>();
-      a.rstd = rstd.data_ptr<float>();
+      set_stats(a, stats);
       a.dweight = ptr_of(dweight);
       a.dbias = ptr_of(dbias);
       npf_check(npf_layernorm_bwd(a, type, at::hip::getCurrentHIPStream()),
@@ -168,9 +171,9 @@ Tensor layer_norm(const Tensor& x, const OptTensor& residual_,
       if (t->defined() && t->requires_grad())
         return LayerNorm::apply(x, some(residual), some(weight), some(bias),
                                 eps);
-  Tensor y = torch::empty(x.sizes(), x.options());
+  Tensor y = npf_empty(x.sizes(), x.scalar_type(), x);
   layer_norm_forward(rows_of(x), rows_of(residual), weight, bias, eps, y,
-                     Tensor(), Tensor());
+                     Tensor());
   return y;
 }
 
@@ -261,16 +264,15 @@ Tensor grad_norm(const std::vector<Tensor>& params, double norm_type,
   const bool clip = max_norm >= 0.;
   if (clip) check_apart(all);
   c10::DeviceGuard guard(grads[0].device());
-  auto options = torch::dtype(torch::kFloat32).device(grads[0].device());
   int type = NPF_F32;  // of the norm: as wide as the widest gradient
   for (const Tensor& g : grads)
     if (g.scalar_type() == torch::kFloat64) type = NPF_F64;
-  Tensor total = torch::empty(
-      {}, options.dtype(type == NPF_F64 ? torch::kFloat64 : torch::kFloat32));
+  Tensor total = npf_empty(
+      {}, type == NPF_F64 ? torch::kFloat64 : torch::kFloat32, grads[0]);
   if (all.empty()) return total.zero_();
   int n = 0;
   for (const NpfGradSpans& s : all) n += npf_grad_blocks(s.first_chunk[s.n]);
-  Tensor partial = torch::empty({n}, options.dtype(torch::kFloat64));
+  Tensor partial = npf_empty({n}, torch::kFloat64, grads[0]);
   auto stream = at::hip::getCurrentHIPStream();
   double* p = partial.data_ptr<double>();
   for (const NpfGradSpans& s : all) {
