@@ -288,9 +288,6 @@ int parts_for(long blocks, long wanted, int length, int least) {
   return (int)(n < most ? (n < 1 ? 1 : n) : (most < 1 ? 1 : most));
 }
 
-// whether forward blocks leave parts: of the key axis, or of one map each
-bool joined(const NpfDiffAttnArgs& a) { return a.splits > 1 || a.pad == 128; }
-
 }  // namespace
 
 bool npf_diff_attn_plan(NpfDiffAttnArgs& a) {
@@ -302,17 +299,13 @@ bool npf_diff_attn_plan(NpfDiffAttnArgs& a) {
   // between four.
   a.waves = rows <= 32 ? 1 : 4;
   // Blocks that the chip holds at once: of one wave by their LDS (4 tiles of
-  // 32 or 64 rows), of four by their registers (see kResident: 16-bit forward
-  // blocks of one map are two a SIMD).
+  // 32 or 64 rows), of four by their registers (see kResident).
   const int row_bytes = 2 * a.pad * (a.type == NPF_F32 ? 4 : 2);
   const long wanted1 = row_bytes <= 256 ? 1280 : row_bytes == 512 ? 512 : 256;
   const long wanted = row_bytes <= 256 ? 512 : 256;
-  const long wanted_fwd = a.pad == 128 && a.type != NPF_F32 ? 512 : wanted;
   const long row_blocks4 = heads * ((rows + 127) / 128);
-  const long parts = a.pad == 128 ? 2 : 1;
-  a.splits = a.waves == 1
-                 ? parts_for(heads * parts, wanted1, a.K, 64)
-                 : parts_for(row_blocks4 * parts, wanted_fwd, a.K, 256);
+  a.splits = a.waves == 1 ? parts_for(heads, wanted1, a.K, 64)
+                          : parts_for(row_blocks4, wanted, a.K, 256);
   a.dq_splits = parts_for(row_blocks4, wanted, a.K, 256);
   a.dkv_splits =
       parts_for(heads * ((a.K + 127) / 128), wanted, (int)rows, 256);
@@ -320,7 +313,7 @@ bool npf_diff_attn_plan(NpfDiffAttnArgs& a) {
 }
 
 long npf_diff_attn_workspace(const NpfDiffAttnArgs& a) {
-  if (!joined(a)) return 0;
+  if (a.splits <= 1) return 0;
   return split_row_floats(a.Dv) * a.splits * a.B * a.H * a.Q;
 }
 
@@ -332,7 +325,7 @@ hipError_t npf_diff_attn_fwd(const NpfDiffAttnArgs& a, hipStream_t stream) {
     case NPF_BF16: e = npf_diff_attn_fwd_bf16(a, stream); break;
     case NPF_F16: e = npf_diff_attn_fwd_f16(a, stream); break;
   }
-  if (e != hipSuccess || !joined(a)) return e;
+  if (e != hipSuccess || a.splits <= 1) return e;
   switch (a.type) {
     case NPF_F32: return join_forward<float>(a, stream);
     case NPF_BF16: return join_forward<npf_bf16>(a, stream);

@@ -36,11 +36,6 @@ struct Shape {
   // whether the dq kernel keeps its queries in LDS rather than in registers
   // (long: 529 us, 704 with one wave a SIMD, 814 with two that spill)
   static constexpr bool kQueriesInLds = sizeof(T) == 2 && kPad == 64;
-  // forward blocks of one map each, joined like parts of a split key axis: the
-  // sums of 256 columns for two maps would fill a wave's registers alone.
-  // (8 heads, bf16: 4096 x 4096 269 us, with half of the columns of both maps
-  // a block 479; 8 x 256 x 256, where the join counts most, a step 159 and 145.)
-  static constexpr bool kMapsApart = kPad == 128;
   static constexpr int kSteps = kPad / (2 * kChunk<T>);  // chunk pairs a map
 
   // Whether value `at` of `all` padded ones, of which `size` are there, is to
@@ -64,6 +59,13 @@ template <typename T, int kPad, bool kOneMap = false>
 constexpr int kResident =
     kPad * (int)sizeof(T) <= (kOneMap && sizeof(T) == 2 ? 256 : 128) ? 2 : 1;
 
+// The same of the forward kernel, whose waves hold one map; rows on their way
+// through registers (not kDirect) need room too.
+template <typename T, int kPad, bool kDirect>
+constexpr int kFwdResident =
+    kPad * (int)sizeof(T) <= (kDirect ? 128 : 64) ? 4
+    : kPad * (int)sizeof(T) <= (kDirect ? 512 : 256) ? 2 : 1;
+
 // Columns that block n of map m starts at.  Maps of 16 share one block: each
 // accumulates it whole and keeps its half.
 template <int kPad>
@@ -80,9 +82,10 @@ __host__ __device__ inline int split_keys(int n, int splits, int tile) {
 // maximum and sum, and both sums of values, all in fp32.
 __host__ __device__ inline long split_row_floats(int Dv) { return 2L * Dv + 4; }
 
-// exp2 of score * c - m over one tile, into s; returns the lane's sum
-__device__ __forceinline__ float exp_tile(f32x16& s, float c, float m) {
-  float sum = 0.f;
+// exp2 of score * c - m over one tile, into s; returns the lane's sum of them
+// and `sum`
+__device__ __forceinline__ float exp_tile(f32x16& s, float c, float m,
+                                          float sum) {
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -m));
@@ -104,18 +107,20 @@ __device__ __forceinline__ float exp_tile(f32x16& s, float c, float m) {
 // as a SIMD has a second wave.  LDS is read at less than half of its rate, and
 // without bank conflicts.
 
-// Forward: a wave holds 32 query rows and passes over the keys.  Blocks of four
-// waves share the tiles; with up to 32 rows a head, blocks of one wave split
-// the keys between them (single queries against 32768 keys, 200 MB of bf16: 52
-// us, 3.9 TB/s, and 8 us to join).
-template <typename T, int kPad, int kWaves, bool kDirect>
-__global__ void __launch_bounds__(
-    64 * kWaves, (kResident<T, kPad, Shape<T, kPad>::kMapsApart>))
+// Forward: a wave holds 32 query rows and one map, and passes over the keys; a
+// block has kRowWaves waves for each map, which share the tiles (the first
+// map's waves move the keys', the second's the values') and meet at the end.
+// With up to 32 rows a head, blocks of one wave a map split the keys between
+// them (single queries against 32768 keys, 200 MB of bf16: 52 us, 3.9 TB/s, and
+// 8 us to join).
+template <typename T, int kPad, int kRowWaves, bool kDirect>
+__global__ void __launch_bounds__(128 * kRowWaves,
+                                  (kFwdResident<T, kPad, kDirect>))
     diff_fwd(NpfDiffAttnArgs a) {
   using S = Shape<T, kPad>;
   using Lds = Tile<T, S::kWidth>;
-  constexpr int kTile = kWaves == 1 ? 32 * S::kSubs : S::kTile;
-  constexpr int kSubs = S::kSubs, kMaps = S::kMapsApart ? 1 : 2;
+  constexpr int kTile = kRowWaves == 1 ? 32 * S::kSubs : S::kTile;
+  constexpr int kSubs = S::kSubs;
   constexpr int kTileBytes = kTile * S::kRowBytes;
   // two objects, so that it shows that the next tiles' loads do not touch
   // what is being read
@@ -123,28 +128,28 @@ __global__ void __launch_bounds__(
   __shared__ __attribute__((aligned(16))) char odd[2 * kTileBytes];
 
   const int group = a.H / a.Hk, rows = group * a.Q;
-  const int row_tiles = (rows + 32 * kWaves - 1) / (32 * kWaves);
+  const int row_tiles = (rows + 32 * kRowWaves - 1) / (32 * kRowWaves);
   // Neighbouring blocks take different batch entries and heads: long and short
   // contexts spread over the chip, and as blocks are dealt to the 8 XCDs in
   // turn, those of one head mostly share an L2.  With few rows nothing is
   // shared, and neighbours in memory are read at a time (single queries
   // against 32768 keys: 52 us rather than 66).
   const int heads = a.B * a.Hk;
-  const int first = S::kMapsApart ? blockIdx.x % 2 : 0;  // of its maps
-  const int id = S::kMapsApart ? blockIdx.x / 2 : blockIdx.x;
   int bh, row_tile, split;
-  if (kWaves == 1) {
-    split = id % a.splits;
-    row_tile = id / a.splits % row_tiles;
-    bh = id / a.splits / row_tiles;
+  if (kRowWaves == 1) {
+    split = blockIdx.x % a.splits;
+    row_tile = blockIdx.x / a.splits % row_tiles;
+    bh = blockIdx.x / a.splits / row_tiles;
   } else {
-    bh = id % heads;
-    row_tile = id / heads % row_tiles;
-    split = id / heads / row_tiles;
+    bh = blockIdx.x % heads;
+    row_tile = blockIdx.x / heads % row_tiles;
+    split = blockIdx.x / heads / row_tiles;
   }
   const int b = bh / a.Hk, hk = bh % a.Hk;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int m = wave / kRowWaves, row_wave = wave % kRowWaves;
   const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
-  const int row = (row_tile * kWaves + (threadIdx.x >> 6)) * 32 + col;
+  const int row = (row_tile * kRowWaves + row_wave) * 32 + col;
   const bool live = row < rows;
   const int h = hk * group + (live ? row / a.Q : 0);
   const int q = live ? row % a.Q : 0;
@@ -157,33 +162,24 @@ __global__ void __launch_bounds__(
     end = n - begin < per ? n : begin + per;
   }
 
-  u32x4 qf[kMaps][S::kSteps];
+  u32x4 qf[S::kSteps];
 #pragma unroll
-  for (int m = 0; m < kMaps; ++m)
-#pragma unroll
-    for (int u = 0; u < S::kSteps; ++u) {
-      const ChunkOf c =
-          chunk_of_maps<T, kPad>(((first + m) * S::kSteps + u) * 2 + half, a.D);
-      qf[m][u] = u32x4{0, 0, 0, 0};
-      if (live) qf[m][u] = load_chunk(row_of<T>(a.q, b, h, q), c);
-    }
-
-  f32x16 o[kMaps][S::kBlocks];
-  float mx[kMaps], l[kMaps];
-#pragma unroll
-  for (int m = 0; m < kMaps; ++m) {
-    mx[m] = kLowest;
-    l[m] = 0.f;
-#pragma unroll
-    for (int j = 0; j < S::kBlocks; ++j) o[m][j] = f32x16{};
+  for (int u = 0; u < S::kSteps; ++u) {
+    qf[u] = u32x4{0, 0, 0, 0};
+    if (live)
+      qf[u] = load_chunk(
+          row_of<T>(a.q, b, h, q),
+          chunk_of_maps<T, kPad>((m * S::kSteps + u) * 2 + half, a.D));
   }
+
+  f32x16 o[S::kBlocks];
+#pragma unroll
+  for (int j = 0; j < S::kBlocks; ++j) o[j] = f32x16{};
+  float mx = kLowest, l = 0.f;
   const float c = a.scale * kLog2e;
 
-  Stage<T, S::kWidth, kTile, 64 * kWaves, kDirect> stage;
-  const T* kp = row_of<T>(a.k, b, hk, 0);
-  const T* vp = row_of<T>(a.v, b, hk, 0);
   // one tile from LDS; kEdge: it may reach behind the last key
-  const int rows_base = Lds::rows_base(lane) ^ (first * S::kSteps << 5);
+  const int rows_base = Lds::rows_base(lane) ^ (m * S::kSteps << 5);
   const int cols_base = Lds::cols_base(lane);
   auto pass = [&](auto edge, int k0, const char* kt) {
     constexpr bool kEdge = decltype(edge)::value;
@@ -192,91 +188,76 @@ __global__ void __launch_bounds__(
 #pragma unroll
     for (int sub0 = 0; sub0 < kTile; sub0 += 32 * kSubs) {
       if (kEdge && k0 + sub0 >= end) break;
-      f32x16 s[kMaps][kSubs];
+      f32x16 s[kSubs];
 #pragma unroll
-      for (int m = 0; m < kMaps; ++m)
+      for (int t = 0; t < kSubs; ++t) {
+        s[t] = f32x16{};
 #pragma unroll
-        for (int t = 0; t < kSubs; ++t) {
-          s[m][t] = f32x16{};
-#pragma unroll
-          for (int u = 0; u < S::kSteps; ++u)
-            if (S::counts(u * 2 * kChunk<T>, kPad, a.D))
-              s[m][t] = mma_chunk<T>(
-                  Lds::rows(kt, rb, sub0 + 32 * t, m * S::kSteps + u),
-                  qf[m][u], s[m][t]);
-        }
+        for (int u = 0; u < S::kSteps; ++u)
+          if (S::counts(u * 2 * kChunk<T>, kPad, a.D))
+            s[t] = mma_chunk<T>(Lds::rows(kt, rb, sub0 + 32 * t, u), qf[u],
+                                s[t]);
+      }
       if constexpr (kEdge) {
 #pragma unroll
         for (int t = 0; t < kSubs; ++t)
 #pragma unroll
           for (int i = 0; i < 16; ++i)
             if (k0 + sub0 + 32 * t + reg_row(i) + 4 * half >= end)
-#pragma unroll
-              for (int m = 0; m < kMaps; ++m) s[m][t][i] = -INFINITY;
+              s[t][i] = -INFINITY;
       }
+      float top = s[0][0];
 #pragma unroll
-      for (int m = 0; m < kMaps; ++m) {
-        float top = s[m][0][0];
+      for (int t = 0; t < kSubs; ++t)
 #pragma unroll
-        for (int t = 0; t < kSubs; ++t)
+        for (int i = 0; i < 16; ++i) top = larger(top, s[t][i]);
+      top = both_max(top) * c;
+      // The maximum is raised only where it is exceeded by 2^8: exponents stay
+      // below that, far from any type's end, and most tiles leave the sums as
+      // they are.
+      if (__any(top > mx + 8.f)) {
+        const float up = fmaxf(mx, top);
+        const float f = __builtin_amdgcn_exp2f(mx - up);
+        mx = up;
+        l *= f;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) top = fmaxf(top, s[m][t][i]);
-        top = both_max(top) * c;
-        // The maximum is raised only where it is exceeded by 2^8: exponents
-        // stay below that, far from any type's end, and most tiles leave the
-        // sums as they are.
-        if (__any(top > mx[m] + 8.f)) {
-          const float up = fmaxf(mx[m], top);
-          const float f = __builtin_amdgcn_exp2f(mx[m] - up);
-          mx[m] = up;
-          l[m] *= f;
-#pragma unroll
-          for (int j = 0; j < S::kBlocks; ++j) o[m][j] *= f;
-        }
+        for (int j = 0; j < S::kBlocks; ++j) o[j] *= f;
       }
 #pragma unroll
       for (int t = 0; t < kSubs; ++t) {
+        l = exp_tile(s[t], c, mx, l);
+        const Operand<T> p[1] = {Operand<T>(s[t])};
 #pragma unroll
-        for (int m = 0; m < kMaps; ++m)
-          l[m] += exp_tile(s[m][t], c, mx[m]);
-        if constexpr (kMaps == 2) {
-          const Operand<T> p[2] = {Operand<T>(s[0][t]), Operand<T>(s[1][t])};
-#pragma unroll
-          for (int j = 0; j < S::kBlocks; ++j) {
-            f32x16* const acc[2] = {&o[0][j], &o[1][j]};
-            if (S::counts(32 * j, 2 * kPad, a.Dv))
-              Lds::template transposed<2>(vt, cb, sub0 + 32 * t, 32 * j, p,
-                                          acc);
-          }
-        } else {
-          const Operand<T> p[1] = {Operand<T>(s[0][t])};
-#pragma unroll
-          for (int j = 0; j < S::kBlocks; ++j) {
-            f32x16* const acc[1] = {&o[0][j]};
-            if (S::counts(32 * j, 2 * kPad, a.Dv))
-              Lds::template transposed<1>(vt, cb, sub0 + 32 * t, 32 * j, p,
-                                          acc);
-          }
+        for (int j = 0; j < S::kBlocks; ++j) {
+          f32x16* const acc[1] = {&o[j]};
+          if (S::counts(32 * j, 2 * kPad, a.Dv))
+            Lds::template transposed<1>(vt, cb, sub0 + 32 * t, 32 * j, p, acc);
         }
       }
     }
   };
+
+  // what this wave's threads move
+  Stage<T, S::kWidth, kTile, 64 * kRowWaves, kDirect> stage;
+  const T* from = row_of<T>(m ? a.v : a.k, b, hk, 0);
+  const long from_l = m ? a.v.l : a.k.l;
+  const int per = m ? Lds::kChunks : Lds::kChunks / 2;
+  const int size = m ? a.Dv : a.D;
+  const int tid = row_wave * 64 + lane, to = m * kTileBytes;
   auto step = [&](int k0, const char* now, char* then) {
     const int next = k0 + kTile;
     if (next < end)
-      stage.load(kp, a.k.l, vp, a.v.l, a.D, a.Dv, next, end, then,
-                 then + kTileBytes);
+      stage.load(from, from_l, per, size, next, end, tid, then + to);
     pass(std::false_type{}, k0, now);
-    if (next < end) stage.store(end - next, then, then + kTileBytes);
+    if (next < end) stage.store(end - next, tid, then + to);
     __syncthreads();
   };
-  stage.clear(a.D, a.Dv, even);
-  stage.clear(a.D, a.Dv, odd);
+  stage.clear(per, size, tid, even + to);
+  stage.clear(per, size, tid, odd + to);
   __syncthreads();
   if (begin < end) {
-    stage.load(kp, a.k.l, vp, a.v.l, a.D, a.Dv, begin, end, even,
-               even + kTileBytes);
-    stage.store(end - begin, even, even + kTileBytes);
+    stage.load(from, from_l, per, size, begin, end, tid, even + to);
+    stage.store(end - begin, tid, even + to);
   }
   __syncthreads();
   const int full = (end - begin) / kTile;
@@ -291,56 +272,71 @@ __global__ void __launch_bounds__(
   }
   if (k0 < end) pass(std::true_type{}, k0, full & 1 ? odd : even);
 
-#pragma unroll
-  for (int m = 0; m < kMaps; ++m) l[m] = both_sum(l[m]);
-  if (!live) return;
-  if (S::kMapsApart || a.splits > 1) {
+  l = both_sum(l);
+  if (a.splits > 1) {
+    if (!live) return;
     float* w = static_cast<float*>(a.split) +
-               ((long)bh * rows + row) * a.splits * split_row_floats(a.Dv) +
-               split * split_row_floats(a.Dv);
-#pragma unroll
-    for (int m = 0; m < kMaps; ++m) {
-      if (half == 0) {
-        w[2 * (first + m)] = mx[m];
-        w[2 * (first + m) + 1] = l[m];
-      }
-#pragma unroll
-      for (int j = 0; j < S::kBlocks; ++j)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const int d = 32 * j + 8 * g + 4 * half;
-          const f32x16& x = o[m][j];
-          store4(w + 4 + (first + m) * a.Dv + d, a.Dv - d, x[4 * g],
-                 x[4 * g + 1], x[4 * g + 2], x[4 * g + 3]);
-        }
+               (((long)bh * rows + row) * a.splits + split) *
+                   split_row_floats(a.Dv);
+    if (half == 0) {
+      w[2 * m] = mx;
+      w[2 * m + 1] = l;
     }
-    return;
-  }
-  if constexpr (!S::kMapsApart) {
-    const float lam = lam_of(a, h);
-    // rows without keys: zeros; all else divides, so that sums that are no
-    // number show
-    const float i1 = n ? 1.f / l[0] : 0.f, i2 = n ? 1.f / l[1] : 0.f;
-    T* out = row_of<T>(a.out, b, h, q);
-    T* o2 = a.o2.p ? row_of<T>(a.o2, b, h, q) : nullptr;
+    w += 4 + m * a.Dv;
 #pragma unroll
     for (int j = 0; j < S::kBlocks; ++j)
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const int d = 32 * j + 8 * g + 4 * half;
-        float x[4], y[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          y[e] = o[1][j][4 * g + e] * i2;
-          x[e] = o[0][j][4 * g + e] * i1 - lam * y[e];
-        }
-        store4(out + d, a.Dv - d, x[0], x[1], x[2], x[3]);
-        if (o2) store4(o2 + d, a.Dv - d, y[0], y[1], y[2], y[3]);
+        store4(w + d, a.Dv - d, o[j][4 * g], o[j][4 * g + 1], o[j][4 * g + 2],
+               o[j][4 * g + 3]);
       }
-    if (a.lse && half == 0) {
-      float* p = a.lse + (((long)b * a.H + h) * a.Q + q) * 2;
+    return;
+  }
+  // rows without keys: zeros; all else divides, so that sums that are no
+  // number show
+  const float inv = n ? 1.f / l : 0.f;
+  if (a.lse && half == 0 && live)
+    a.lse[(((long)b * a.H + h) * a.Q + q) * 2 + m] =
+        n ? mx + __log2f(l) : 0.f;
+  // The second map's results go to the first map's wave of the same rows, four
+  // registers of all lanes (a piece) at a time, through what the tiles held.
+  constexpr int kPieces = 2 * kTileBytes / (1024 * kRowWaves);  // of each array
+  static_assert(kPieces * 1024 * kRowWaves == 2 * kTileBytes);
+  auto piece = [&](int i) {
+    char* at = i / kPieces % 2 ? odd : even;
+    return reinterpret_cast<f32x4*>(
+        at + ((i % kPieces * kRowWaves + row_wave) * 64 + lane) * 16);
+  };
+  const float lam = lam_of(a, h);
+  T* out = row_of<T>(m ? a.o2 : a.out, b, h, q);
+  const bool stores = live && (m == 0 || a.o2.p);
 #pragma unroll
-      for (int m = 0; m < 2; ++m) p[m] = n ? mx[m] + __log2f(l[m]) : 0.f;
+  for (int i0 = 0; i0 < 4 * S::kBlocks; i0 += 2 * kPieces) {
+    __syncthreads();
+    if (m) {
+#pragma unroll
+      for (int i = i0; i < i0 + 2 * kPieces && i < 4 * S::kBlocks; ++i) {
+        f32x4 y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = o[i / 4][i % 4 * 4 + e] * inv;
+        *piece(i) = y;
+        const int d = 8 * i + 4 * half;
+        if (stores) store4(out + d, a.Dv - d, y[0], y[1], y[2], y[3]);
+      }
+    }
+    __syncthreads();
+    if (m == 0) {
+#pragma unroll
+      for (int i = i0; i < i0 + 2 * kPieces && i < 4 * S::kBlocks; ++i) {
+        const f32x4 y = *piece(i);
+        float x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          x[e] = o[i / 4][i % 4 * 4 + e] * inv - lam * y[e];
+        const int d = 8 * i + 4 * half;
+        if (stores) store4(out + d, a.Dv - d, x[0], x[1], x[2], x[3]);
+      }
     }
   }
 }
@@ -396,7 +392,7 @@ __global__ void __launch_bounds__(64 * kBwdWaves, (kResident<T, kPad>))
       x = load_chunk(row_of<T>(a.q, b, h, q),
                      chunk_of_maps<T, kPad>(u * 2 + half, a.D));
       gf[u] = load_chunk(row_of<T>(a.dout, b, h, q),
-                         chunk_of_row<T>(u * 2 + half, a.Dv));
+                         chunk_of_row<T, kPad>(u * 2 + half, a.Dv));
     }
     if constexpr (kInLds)  // read by the lanes that write it alone
       *reinterpret_cast<u32x4*>(own + (rows_base ^ (u << 5))) = x;
@@ -409,7 +405,7 @@ __global__ void __launch_bounds__(64 * kBwdWaves, (kResident<T, kPad>))
 #pragma unroll
   for (int u = 0; u < 2 * S::kSteps; ++u) {
     if (!live) break;
-    const ChunkOf at = chunk_of_row<T>(u * 2 + half, a.Dv);
+    const ChunkOf at = chunk_of_row<T, kPad>(u * 2 + half, a.Dv);
     T g[kChunk<T>], o[kChunk<T>], o2[kChunk<T>];
     const u32x4 x = load_chunk(row_of<T>(a.out, b, h, q), at);
     const u32x4 y = load_chunk(row_of<T>(a.o2, b, h, q), at);
@@ -441,7 +437,7 @@ __global__ void __launch_bounds__(64 * kBwdWaves, (kResident<T, kPad>))
   float dlam = 0.f;
   const float apart = st.z - st.w;
 
-  Stage<T, S::kWidth, kTile, 64 * kWaves, kDirect> stage;
+  StagePair<T, S::kWidth, kTile, 64 * kWaves, kDirect> stage;
   const T* kp = row_of<T>(a.k, b, hk, 0);
   const T* vp = row_of<T>(a.v, b, hk, 0);
   auto pass = [&](auto edge, int k0, const char* kt) {
@@ -510,19 +506,17 @@ __global__ void __launch_bounds__(64 * kBwdWaves, (kResident<T, kPad>))
   auto step = [&](int k0, const char* now, char* then) {
     const int next = k0 + kTile;
     if (next < n)
-      stage.load(kp, a.k.l, vp, a.v.l, a.D, a.Dv, next, n, then,
-                 then + kTileBytes);
+      stage.load(kp, a.k.l, vp, a.v.l, a.D, a.Dv, next, n, then);
     pass(std::false_type{}, k0, now);
-    if (next < n) stage.store(n - next, then, then + kTileBytes);
+    if (next < n) stage.store(n - next, then);
     __syncthreads();
   };
   stage.clear(a.D, a.Dv, even);
   stage.clear(a.D, a.Dv, odd);
   __syncthreads();
   if (begin < n) {
-    stage.load(kp, a.k.l, vp, a.v.l, a.D, a.Dv, begin, n, even,
-               even + kTileBytes);
-    stage.store(n - begin, even, even + kTileBytes);
+    stage.load(kp, a.k.l, vp, a.v.l, a.D, a.Dv, begin, n, even);
+    stage.store(n - begin, even);
   }
   __syncthreads();
   const int full = (n - begin) / kTile;
@@ -608,7 +602,7 @@ __global__ void __launch_bounds__(64 * kBwdWaves,
                      chunk_of_maps<T, kPad>(u * 2 + half, a.D));
       if (kDk)
         y = load_chunk(row_of<T>(a.v, b, hk, key),
-                       chunk_of_row<T>(u * 2 + half, a.Dv));
+                       chunk_of_row<T, kPad>(u * 2 + half, a.Dv));
     }
     kf[u / S::kSteps][u % S::kSteps] = x;
     vf[u] = y;
@@ -627,7 +621,7 @@ __global__ void __launch_bounds__(64 * kBwdWaves,
   int steps = group * q_tiles;
   steps = steps - step0 < per ? steps : step0 + per;
   if (key_tile * 32 * kWaves >= n) steps = 0;
-  Stage<T, S::kWidth, kTile, 64 * kWaves, kDirect> stage;
+  StagePair<T, S::kWidth, kTile, 64 * kWaves, kDirect> stage;
   float4 st;
   float lam = 0.f, next_lam = 0.f;
   // the tile that is being loaded
@@ -636,7 +630,7 @@ __global__ void __launch_bounds__(64 * kBwdWaves,
     next_lam = lam_of(a, next_h);
     stage.load(row_of<T>(a.q, b, next_h, 0), a.q.l,
                row_of<T>(a.dout, b, next_h, 0), a.dout.l, a.D, a.Dv, next_q,
-               a.Q, to, to + kTileBytes);
+               a.Q, to);
     const int q = next_q + (int)threadIdx.x;
     // rows that are not there have no weight
     st = float4{INFINITY, INFINITY, 0.f, 0.f};
@@ -645,7 +639,7 @@ __global__ void __launch_bounds__(64 * kBwdWaves,
           a.stats)[((long)b * a.H + next_h) * a.Q + q];
   };
   auto store = [&](char* to, float (*to_stats)[kTile]) {
-    stage.store(a.Q - next_q, to, to + kTileBytes);
+    stage.store(a.Q - next_q, to);
     if (threadIdx.x < kTile) {
       to_stats[0][threadIdx.x] = kFromLse ? -st.x / c : st.x;
       to_stats[1][threadIdx.x] = kFromLse ? -st.y / c : st.y;
@@ -806,14 +800,13 @@ hipError_t launch(K kernel, long blocks, int threads, const NpfDiffAttnArgs& a,
 
 template <typename T, int kPad, bool kDirect>
 hipError_t fwd_sized(const NpfDiffAttnArgs& a, hipStream_t stream) {
-  using S = Shape<T, kPad>;
   const long heads = (long)a.B * a.Hk, rows = (long)(a.H / a.Hk) * a.Q;
-  const long each = heads * a.splits * (S::kMapsApart ? 2 : 1);
+  const long each = heads * a.splits;
   if (a.waves == 1)
-    return launch(diff_fwd<T, kPad, 1, kDirect>, each * ((rows + 31) / 32), 64,
-                  a, stream);
+    return launch(diff_fwd<T, kPad, 1, kDirect>, each * ((rows + 31) / 32),
+                  128, a, stream);
   return launch(diff_fwd<T, kPad, 4, kDirect>, each * ((rows + 127) / 128),
-                256, a, stream);
+                512, a, stream);
 }
 
 template <typename T, int kPad, bool kDirect>

@@ -189,21 +189,26 @@ struct ChunkOf {
   int offset, count;
 };
 
-// of a row with two maps of `size` values, each padded to kPad
-template <typename T, int kPad>
-__device__ __forceinline__ ChunkOf chunk_of_maps(int chunk, int size) {
-  constexpr int per = kPad / kChunk<T>;
-  const int in_map = (chunk % per) * kChunk<T>;
-  const int left = size - in_map;
-  return {(chunk / per) * size + in_map,
+// of a row in parts of `per` chunks (a power of two: a map's, or the row's), of
+// which `size` values are there
+template <typename T>
+__device__ __forceinline__ ChunkOf chunk_of(int chunk, int per, int size) {
+  const int in_part = (chunk & (per - 1)) * kChunk<T>;
+  const int left = size - in_part;
+  return {(chunk >= per ? size : 0) + in_part,
           left < 0 ? 0 : left > kChunk<T> ? kChunk<T> : left};
 }
 
-template <typename T>
+// of a row with two maps of `size` values, each padded to kPad
+template <typename T, int kPad>
+__device__ __forceinline__ ChunkOf chunk_of_maps(int chunk, int size) {
+  return chunk_of<T>(chunk, kPad / kChunk<T>, size);
+}
+
+// of a row of up to 2 kPad values
+template <typename T, int kPad>
 __device__ __forceinline__ ChunkOf chunk_of_row(int chunk, int size) {
-  const int left = size - chunk * kChunk<T>;
-  return {chunk * kChunk<T>,
-          left < 0 ? 0 : left > kChunk<T> ? kChunk<T> : left};
+  return chunk_of<T>(chunk, 2 * kPad / kChunk<T>, size);
 }
 
 template <typename T>
@@ -221,8 +226,9 @@ __device__ __forceinline__ u32x4 load_chunk(const T* row, ChunkOf c) {
   return r;
 }
 
-// Two tiles of kRows rows each on their way from memory to LDS, the next pair
-// under the products of this one.
+// A tile of kRows rows on its way from memory to LDS, the next one under the
+// products of this one.  kThreads threads move it, `tid` of them this one; a
+// row is in parts of `per` chunks, of which `size` values are there.
 //
 // kDirect: 16-byte aligned rows of whole chunks.  The loads write LDS
 // themselves and hold no registers; a wave's 64 chunks land side by side, so
@@ -246,12 +252,26 @@ struct Stage<T, kWidth, kRows, kThreads, true> {
   // threads is a multiple of that, one offset a lane serves every step.
   static constexpr int kStep = kThreads / Lds::kChunks;
 
-  // `per`: chunks of a part of the row (a map, or the whole), of which `size`
-  // values are there
-  __device__ __forceinline__ static void one(const T* p, int l, int rows,
-                                             int per, int size, char* tile) {
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63;
+  // All but the last tile are whole, and take their loads from a uniform
+  // address and an offset of the lane that stays the same: no vector work a
+  // load.
+  __device__ __forceinline__ void load(const T* p, long l_, int per, int size,
+                                       int row0, int end, int tid,
+                                       char* tile) {
+    p += row0 * l_;
+    const int l = (int)l_, rows = end - row0;
+    if (rows >= kRows)
+      load_rows<true>(p, l, per, size, rows, tid, tile);
+    else
+      load_rows<false>(p, l, per, size, rows, tid, tile);
+  }
+
+  template <bool kWhole>
+  __device__ __forceinline__ static void load_rows(const T* p, int l, int per,
+                                                   int size, int rows, int tid,
+                                                   char* tile) {
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int lane = tid & 63;
 #pragma unroll
     for (int j = 0; j < kCount; ++j) {
       // chunk of lane 0 within the step, and its row
@@ -259,18 +279,17 @@ struct Stage<T, kWidth, kRows, kThreads, true> {
       int row = first / Lds::kChunks + lane / Lds::kChunks;
       const int chunk =
           lane % Lds::kChunks ^ Lds::permute(row + (kStep % 16 ? j * kStep : 0));
-      if (rows < kRows) {  // the last tile alone
+      if (!kWhole) {
         row += j * kStep;
-        row = (row < rows ? row : rows - 1) - j * kStep;
+        row = row < rows ? row : rows - 1;
       }
-      const T* src = p + (long)j * kStep * l;  // the same for all lanes
-      const int within = chunk % per * kChunk<T>;
-      if (within < size)
+      const char* src = reinterpret_cast<const char*>(
+          p + (kWhole ? (long)j * kStep * l : 0));  // the same for all lanes
+      const ChunkOf c = chunk_of<T>(chunk, per, size);
+      const unsigned at = (unsigned)(row * l + c.offset) * (int)sizeof(T);
+      if (c.count > 0)
         __builtin_amdgcn_global_load_lds(
-            (__attribute__((address_space(1))) void*)(src +
-                                                      (row * l +
-                                                       chunk / per * size +
-                                                       within)),
+            (__attribute__((address_space(1))) void*)(src + at),
             (__attribute__((address_space(3))) void*)(tile +
                                                       (j * kThreads + first) *
                                                           16),
@@ -278,23 +297,16 @@ struct Stage<T, kWidth, kRows, kThreads, true> {
     }
   }
 
-  __device__ __forceinline__ void load(const T* xp, long xl, const T* yp,
-                                       long yl, int map_size, int row_size,
-                                       int row0, int end, char* xt, char* yt) {
-    one(xp + row0 * xl, (int)xl, end - row0, Lds::kChunks / 2, map_size, xt);
-    one(yp + row0 * yl, (int)yl, end - row0, Lds::kChunks, row_size, yt);
+  // the tile becomes zeros, where some chunks will not be loaded
+  __device__ __forceinline__ static void clear(int per, int size, int tid,
+                                               char* tile) {
+    if (size == per * kChunk<T>) return;
+    for (int i = tid; i < kRows * Lds::kChunks; i += kThreads)
+      reinterpret_cast<u32x4*>(tile)[i] = u32x4{0, 0, 0, 0};
   }
 
-  // both tiles of a buffer become zeros, where some chunks will not be loaded
-  __device__ __forceinline__ static void clear(int map_size, int row_size,
-                                               char* tiles) {
-    if (2 * map_size == kWidth && row_size == kWidth) return;
-    for (int i = threadIdx.x; i < 2 * kRows * Lds::kChunks; i += kThreads)
-      reinterpret_cast<u32x4*>(tiles)[i] = u32x4{0, 0, 0, 0};
-  }
-
-  // before the barrier that shows the tiles to every wave
-  __device__ __forceinline__ void store(int, char*, char*) {
+  // before the barrier that shows the tile to every wave
+  __device__ __forceinline__ void store(int, int, char*) {
     __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0), the other counters free
   }
 };
@@ -306,41 +318,61 @@ struct Stage<T, kWidth, kRows, kThreads, false> {
   static constexpr int kCount = kRows / kStep;
   static_assert(kThreads % Lds::kChunks == 0 && kRows % kStep == 0);
 
-  u32x4 x[kCount], y[kCount];
+  u32x4 x[kCount];
 
-  __device__ __forceinline__ static void clear(int, int, char*) {}
+  __device__ __forceinline__ static void clear(int, int, int, char*) {}
 
-  __device__ __forceinline__ void load(const T* xp, long xl, const T* yp,
-                                       long yl, int map_size, int row_size,
-                                       int row0, int end, char*, char*) {
-    const int chunk = (int)threadIdx.x % Lds::kChunks;
-    const ChunkOf xc = chunk_of_maps<T, kWidth / 2>(chunk, map_size);
-    const ChunkOf yc = chunk_of_row<T>(chunk, row_size);
-    const int first = row0 + (int)threadIdx.x / Lds::kChunks;
+  __device__ __forceinline__ void load(const T* p, long l, int per, int size,
+                                       int row0, int end, int tid, char*) {
+    const ChunkOf c = chunk_of<T>(tid % Lds::kChunks, per, size);
+    const int first = row0 + tid / Lds::kChunks;
 #pragma unroll
     for (int j = 0; j < kCount; ++j) {
       const int row = first + j * kStep;
       const int at = row < end ? row : end - 1;
-      x[j] = load_chunk(xp + at * xl, xc);
-      y[j] = load_chunk(yp + at * yl, yc);
+      x[j] = load_chunk(p + at * l, c);
     }
   }
 
-  // `count` rows of the tiles are there
-  __device__ __forceinline__ void store(int count, char* xt, char* yt) {
-    const int first = (int)threadIdx.x / Lds::kChunks;
-    const int chunk = (int)threadIdx.x % Lds::kChunks;
+  // `count` rows of the tile are there
+  __device__ __forceinline__ void store(int count, int tid, char* tile) {
+    const int first = tid / Lds::kChunks, chunk = tid % Lds::kChunks;
     if (count < kRows) {
 #pragma unroll
       for (int j = 0; j < kCount; ++j)
-        if (first + j * kStep >= count) x[j] = y[j] = u32x4{0, 0, 0, 0};
+        if (first + j * kStep >= count) x[j] = u32x4{0, 0, 0, 0};
     }
 #pragma unroll
-    for (int j = 0; j < kCount; ++j) {
-      const int at = Lds::at(first + j * kStep, chunk);
-      *reinterpret_cast<u32x4*>(xt + at) = x[j];
-      *reinterpret_cast<u32x4*>(yt + at) = y[j];
-    }
+    for (int j = 0; j < kCount; ++j)
+      *reinterpret_cast<u32x4*>(tile + Lds::at(first + j * kStep, chunk)) =
+          x[j];
+  }
+};
+
+// Two tiles side by side, moved by all of a block's threads: rows of two maps
+// of map_size values, and rows of row_size values.
+template <typename T, int kWidth, int kRows, int kThreads, bool kDirect>
+struct StagePair {
+  using One = Stage<T, kWidth, kRows, kThreads, kDirect>;
+  static constexpr int kChunks = kWidth / kChunk<T>;
+  static constexpr int kTileBytes = kRows * kWidth * (int)sizeof(T);
+  One x, y;
+
+  __device__ __forceinline__ void load(const T* xp, long xl, const T* yp,
+                                       long yl, int map_size, int row_size,
+                                       int row0, int end, char* tiles) {
+    const int tid = threadIdx.x;
+    x.load(xp, xl, kChunks / 2, map_size, row0, end, tid, tiles);
+    y.load(yp, yl, kChunks, row_size, row0, end, tid, tiles + kTileBytes);
+  }
+  __device__ __forceinline__ static void clear(int map_size, int row_size,
+                                               char* tiles) {
+    One::clear(kChunks / 2, map_size, threadIdx.x, tiles);
+    One::clear(kChunks, row_size, threadIdx.x, tiles + kTileBytes);
+  }
+  __device__ __forceinline__ void store(int count, char* tiles) {
+    x.store(count, threadIdx.x, tiles);
+    y.store(count, threadIdx.x, tiles + kTileBytes);
   }
 };
 
@@ -372,9 +404,13 @@ __device__ __forceinline__ Halves halves(float x) {
   const unsigned low = r[0], high = r[1];
   return {__builtin_bit_cast(float, low), __builtin_bit_cast(float, high)};
 }
+// (NaN where one is: without the steps that keep it out)
+__device__ __forceinline__ float larger(float a, float b) {
+  return __builtin_elementwise_maximum(a, b);
+}
 __device__ __forceinline__ float both_max(float x) {
   const Halves h = halves(x);
-  return fmaxf(h.low, h.high);
+  return larger(h.low, h.high);
 }
 __device__ __forceinline__ float both_sum(float x) {
   const Halves h = halves(x);
