@@ -31,7 +31,7 @@ struct NpfDiffAttnArgs {
   int lengths64;
   // the plan
   int pad;     // D and Dv / 2 are padded to this
-  int waves;   // of a forward block
+  int waves;   // of a forward block, for each map
   int splits;  // parts of the key axis, forward
   int dq_splits;   // parts of the key axis, and of the query axis, backward
   int dkv_splits;

@@ -279,7 +279,7 @@ hipError_t join_backward(const NpfDiffAttnArgs& a, hipStream_t stream) {
   return hipGetLastError();
 }
 
-// Parts of an axis of `length` so that `blocks` of 4 waves become two a CU;
+// Parts of an axis of `length` so that `blocks` become as many as the chip holds;
 // none shorter than `least`, whose work would not pay for the join.
 int parts_for(long blocks, long wanted, int length, int least) {
   if (blocks <= 0 || 2 * blocks > wanted) return 1;
@@ -299,13 +299,16 @@ bool npf_diff_attn_plan(NpfDiffAttnArgs& a) {
   // between four.
   a.waves = rows <= 32 ? 1 : 4;
   // Blocks that the chip holds at once: of one wave by their LDS (4 tiles of
-  // 32 or 64 rows), of four by their registers (see kResident).
+  // 32 or 64 rows), of more by their registers (see kResident, kFwdResident).
   const int row_bytes = 2 * a.pad * (a.type == NPF_F32 ? 4 : 2);
   const long wanted1 = row_bytes <= 256 ? 1280 : row_bytes == 512 ? 512 : 256;
   const long wanted = row_bytes <= 256 ? 512 : 256;
   const long row_blocks4 = heads * ((rows + 127) / 128);
+  // (fp32 products are worth a join from 128 keys on: 8 x 8 heads of 96, 256 x
+  // 256, 92 us to 81)
   a.splits = a.waves == 1 ? parts_for(heads, wanted1, a.K, 64)
-                          : parts_for(row_blocks4, wanted, a.K, 256);
+                          : parts_for(row_blocks4, wanted, a.K,
+                                      a.type == NPF_F32 ? 128 : 256);
   a.dq_splits = parts_for(row_blocks4, wanted, a.K, 256);
   a.dkv_splits =
       parts_for(heads * ((a.K + 127) / 128), wanted, (int)rows, 256);

@@ -22,7 +22,7 @@ struct Shape {
   static constexpr int kRowBytes = kWidth * (int)sizeof(T);
   // keys (or queries) a tile: two buffers of two tiles in 64 KiB
   static constexpr int kTile = kRowBytes <= 256 ? 64 : 32;
-  // tiles of 32 that a wave takes through a pass at once
+  // tiles of 32 that a backward wave takes through a pass at once
   static constexpr int kSubs = sizeof(T) == 2 ? (kPad <= 32 ? 2 : 1)
                                               : (kPad <= 16 ? 2 : 1);
   // What a wave's registers hold decides how the gradients share launches: of
@@ -53,14 +53,15 @@ struct Shape {
 
 // Waves a SIMD is to hold: two, in half of the registers each and with every
 // matrix result in ordinary registers, where a kernel fits; else one.  (Long
-// training bf16, forward: 794 us with one, 475 with two; two that spill, 1384.)
+// training bf16, dk and dv in one launch that spills: 4349 us; apart, 988.)
 // Kernels of one map fit at twice the size.
 template <typename T, int kPad, bool kOneMap = false>
 constexpr int kResident =
     kPad * (int)sizeof(T) <= (kOneMap && sizeof(T) == 2 ? 256 : 128) ? 2 : 1;
 
 // The same of the forward kernel, whose waves hold one map; rows on their way
-// through registers (not kDirect) need room too.
+// through registers (not kDirect) need room too.  (Long: 430 us; waves with
+// both maps 475 with two a SIMD, 794 with one.)
 template <typename T, int kPad, bool kDirect>
 constexpr int kFwdResident =
     kPad * (int)sizeof(T) <= (kDirect ? 128 : 64) ? 4
@@ -98,21 +99,23 @@ __device__ __forceinline__ float exp_tile(f32x16& s, float c, float m,
 // bf16; "image": 16 x 4 heads, 1024 x 1024, maps of 16):
 //
 //            long bf16               image bf16   bound by
-//   forward  475 us, 0.58 PFLOP/s      36 us      vector unit 66% (image 88%)
-//   dq       529 us                    42 us      and matrix unit 49% of the
-//   dk, dv   582 + 406 us              51 us      time, at 1.9 GHz
+//   forward  430 us, 0.64 PFLOP/s      35 us      vector and matrix unit: their
+//   dq       529 us                    42 us      times add up to the kernel's
+//   dk, dv   582 + 406 us              51 us      (forward 530 + 393 thousand
+//                                                 clocks a SIMD)
+// 8 heads of 128, 4096 x 4096, bf16: forward 203 us, 0.68 PFLOP/s.
 //
 // A pair of scores costs two exponents (8 clocks a 64-lane wave each) and about
-// 9 other vector operations a lane; the matrix unit works beside them as long
-// as a SIMD has a second wave.  LDS is read at less than half of its rate, and
-// without bank conflicts.
+// 8 other vector operations a lane, and a wave's products and vector work hardly
+// overlap, however many waves a SIMD has.  LDS is read at less than half of its
+// rate, and without bank conflicts.
 
 // Forward: a wave holds 32 query rows and one map, and passes over the keys; a
 // block has kRowWaves waves for each map, which share the tiles (the first
 // map's waves move the keys', the second's the values') and meet at the end.
 // With up to 32 rows a head, blocks of one wave a map split the keys between
-// them (single queries against 32768 keys, 200 MB of bf16: 52 us, 3.9 TB/s, and
-// 8 us to join).
+// them (single queries against 32768 keys, 200 MB of bf16: 58 us, 3.45 TB/s,
+// with the join).
 template <typename T, int kPad, int kRowWaves, bool kDirect>
 __global__ void __launch_bounds__(128 * kRowWaves,
                                   (kFwdResident<T, kPad, kDirect>))
@@ -120,7 +123,9 @@ __global__ void __launch_bounds__(128 * kRowWaves,
   using S = Shape<T, kPad>;
   using Lds = Tile<T, S::kWidth>;
   constexpr int kTile = kRowWaves == 1 ? 32 * S::kSubs : S::kTile;
-  constexpr int kSubs = S::kSubs;
+  // tiles of 32 that a wave takes through a pass at once: what fits a quarter
+  // of a SIMD's registers (8 heads of 32, 4096^2, bf16: 93 us, with two 110)
+  constexpr int kSubs = kPad <= 16 ? 2 : 1;
   constexpr int kTileBytes = kTile * S::kRowBytes;
   // two objects, so that it shows that the next tiles' loads do not touch
   // what is being read
@@ -133,7 +138,7 @@ __global__ void __launch_bounds__(128 * kRowWaves,
   // contexts spread over the chip, and as blocks are dealt to the 8 XCDs in
   // turn, those of one head mostly share an L2.  With few rows nothing is
   // shared, and neighbours in memory are read at a time (single queries
-  // against 32768 keys: 52 us rather than 66).
+  // against 32768 keys: 15% faster).
   const int heads = a.B * a.Hk;
   int bh, row_tile, split;
   if (kRowWaves == 1) {
