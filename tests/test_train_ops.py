@@ -680,6 +680,21 @@ class TestDifferentialAttention:
         check_attn(run_attn("cuda", a, lengths=lens), attn_oracle(a, lengths=lens))
 
     @pytest.mark.gpu
+    @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+    @pytest.mark.parametrize("D", [8, 24, 64, 127, 128])
+    @pytest.mark.parametrize("Q, K", [(3, 60), (9, 127), (70, 33), (129, 255)])
+    def test_maps_meet_in_a_block(self, dtype, D, Q, K):
+        # key axes that are not split, of blocks with few rows and with many
+        a = attn_inputs(2, 2, 1, Q, K, D, 2 * D, dtype)
+        check_attn(run_attn("cuda", a), attn_oracle(a))
+        lens = [K // 2, 0]
+        check_attn(run_attn("cuda", a, lengths=lens), attn_oracle(a, lengths=lens))
+        t = {n: x.cuda() for n, x in a.items()}
+        alone = ops.differential_attention(t["keys"], t["queries"], t["values"], t["lam"])
+        # (without what a backward pass would need, and the same)
+        assert torch.equal(alone, run_attn("cuda", a)["out"])
+
+    @pytest.mark.gpu
     def test_refusals_of_the_kernel(self):
         a = {n: t.cuda() for n, t in
              attn_inputs(2, 2, 2, 3, 5, 4, 8, torch.float32).items()}
