@@ -38,13 +38,20 @@ struct Shape {
   static constexpr bool kQueriesInLds = sizeof(T) == 2 && kPad == 64;
   static constexpr int kSteps = kPad / (2 * kChunk<T>);  // chunk pairs a map
 
-  // Whether value `at` of `all` padded ones, of which `size` are there, is to
-  // be computed: the widest fp32 products leave out a last quarter of pure
-  // padding (a step at heads of 96: 1178 us to 983); the others are taken
-  // whole (the same question at heads of 64: 516 us to 570).
-  __device__ static __forceinline__ bool counts(int at, int all, int size) {
-    if (sizeof(T) == 2 || kPad < 128 || 2 * at < all) return true;
-    return at / (all / 4) * (all / 4) < size;
+  // The widest fp32 products are taken in two parts, and leave out the second,
+  // the last quarter, where it is padding alone (a step at heads of 96: 1178 us
+  // to 907); the others are taken whole (such questions at heads of 64: 503 us
+  // to 570).  Steps of a part, of n in all:
+  static constexpr int kParts = sizeof(T) == 4 && kPad == 128 ? 2 : 1;
+  __host__ __device__ static constexpr int from(int n, int part) {
+    return part ? n - n / 4 : 0;
+  }
+  __host__ __device__ static constexpr int upto(int n, int part) {
+    return part + 1 < kParts ? n - n / 4 : n;
+  }
+  // of `all` padded values `size` are there
+  __device__ static __forceinline__ bool taken(int part, int all, int size) {
+    return part == 0 || 4 * size > 3 * all;
   }
 
   static constexpr int kBlocks = kWidth / 32;  // 32 columns of a whole row
@@ -106,9 +113,9 @@ __device__ __forceinline__ float exp_tile(f32x16& s, float c, float m,
 // 8 heads of 128, 4096 x 4096, bf16: forward 203 us, 0.68 PFLOP/s.
 //
 // A pair of scores costs two exponents (8 clocks a 64-lane wave each) and about
-// 8 other vector operations a lane, and a wave's products and vector work hardly
-// overlap, however many waves a SIMD has.  LDS is read at less than half of its
-// rate, and without bank conflicts.
+// 8 other vector operations a lane, and a wave's products and vector work
+// hardly overlap, however many waves a SIMD has.  LDS is read at less than half
+// of its rate, and without bank conflicts.
 
 // Forward: a wave holds 32 query rows and one map, and passes over the keys; a
 // block has kRowWaves waves for each map, which share the tiles (the first
@@ -198,10 +205,15 @@ __global__ void __launch_bounds__(128 * kRowWaves,
       for (int t = 0; t < kSubs; ++t) {
         s[t] = f32x16{};
 #pragma unroll
-        for (int u = 0; u < S::kSteps; ++u)
-          if (S::counts(u * 2 * kChunk<T>, kPad, a.D))
-            s[t] = mma_chunk<T>(Lds::rows(kt, rb, sub0 + 32 * t, u), qf[u],
-                                s[t]);
+        for (int part = 0; part < S::kParts; ++part) {
+          if (!S::taken(part, kPad, a.D)) continue;
+#pragma unroll
+          for (int u = S::from(S::kSteps, part);
+               u < S::upto(S::kSteps, part); ++u) {
+            s[t] =
+                mma_chunk<T>(Lds::rows(kt, rb, sub0 + 32 * t, u), qf[u], s[t]);
+          }
+        }
       }
       if constexpr (kEdge) {
 #pragma unroll
@@ -233,10 +245,14 @@ __global__ void __launch_bounds__(128 * kRowWaves,
         l = exp_tile(s[t], c, mx, l);
         const Operand<T> p[1] = {Operand<T>(s[t])};
 #pragma unroll
-        for (int j = 0; j < S::kBlocks; ++j) {
-          f32x16* const acc[1] = {&o[j]};
-          if (S::counts(32 * j, 2 * kPad, a.Dv))
+        for (int part = 0; part < S::kParts; ++part) {
+          if (!S::taken(part, 2 * kPad, a.Dv)) continue;
+#pragma unroll
+          for (int j = S::from(S::kBlocks, part);
+               j < S::upto(S::kBlocks, part); ++j) {
+            f32x16* const acc[1] = {&o[j]};
             Lds::template transposed<1>(vt, cb, sub0 + 32 * t, 32 * j, p, acc);
+          }
         }
       }
     }
@@ -459,10 +475,15 @@ __global__ void __launch_bounds__(64 * kBwdWaves, (kResident<T, kPad>))
 #pragma unroll
         for (int i = 0; i < 16; ++i) g[t][i] = -st.z;
 #pragma unroll
-        for (int u = 0; u < 2 * S::kSteps; ++u)
-          if (S::counts(u * 2 * kChunk<T>, 2 * kPad, a.Dv))
+        for (int part = 0; part < S::kParts; ++part) {
+          if (!S::taken(part, 2 * kPad, a.Dv)) continue;
+#pragma unroll
+          for (int u = S::from(2 * S::kSteps, part);
+               u < S::upto(2 * S::kSteps, part); ++u) {
             g[t] =
                 mma_chunk<T>(Lds::rows(vt, rb, sub0 + 32 * t, u), gf[u], g[t]);
+          }
+        }
       }
       if (kSubs == 1) __builtin_amdgcn_sched_barrier(0);
       // one map after the other: a second tile of scores would not fit
@@ -474,14 +495,19 @@ __global__ void __launch_bounds__(64 * kBwdWaves, (kResident<T, kPad>))
         for (int t = 0; t < kSubs; ++t) {
           s[t] = f32x16{};
 #pragma unroll
-          for (int u = m * S::kSteps; u < (m + 1) * S::kSteps; ++u) {
-            if (!S::counts(u % S::kSteps * 2 * kChunk<T>, kPad, a.D)) continue;
-            u32x4 x;
-            if constexpr (kInLds)
-              x = Lds::rows(own, rb, 0, u);
-            else
-              x = qf[u];
-            s[t] = mma_chunk<T>(Lds::rows(kt, rb, sub0 + 32 * t, u), x, s[t]);
+          for (int part = 0; part < S::kParts; ++part) {
+            if (!S::taken(part, kPad, a.D)) continue;
+#pragma unroll
+            for (int i = S::from(S::kSteps, part);
+                 i < S::upto(S::kSteps, part); ++i) {
+              const int u = m * S::kSteps + i;
+              u32x4 x;
+              if constexpr (kInLds)
+                x = Lds::rows(own, rb, 0, u);
+              else
+                x = qf[u];
+              s[t] = mma_chunk<T>(Lds::rows(kt, rb, sub0 + 32 * t, u), x, s[t]);
+            }
           }
         }
         const float lse = m ? st.y : st.x;
@@ -497,11 +523,15 @@ __global__ void __launch_bounds__(64 * kBwdWaves, (kResident<T, kPad>))
           }
           const Operand<T> ds[1] = {Operand<T>(s[t])};
 #pragma unroll
-          for (int j = 0; j < S::kMapBlocks; ++j) {
-            f32x16* const acc[1] = {&dq[m][j]};
-            if (!S::counts(32 * j, kPad, a.D)) continue;
-            Lds::template transposed<1>(kt, cb, sub0 + 32 * t,
-                                        map_col<kPad>(m, j), ds, acc);
+          for (int part = 0; part < S::kParts; ++part) {
+            if (!S::taken(part, kPad, a.D)) continue;
+#pragma unroll
+            for (int j = S::from(S::kMapBlocks, part);
+                 j < S::upto(S::kMapBlocks, part); ++j) {
+              f32x16* const acc[1] = {&dq[m][j]};
+              Lds::template transposed<1>(kt, cb, sub0 + 32 * t,
+                                          map_col<kPad>(m, j), ds, acc);
+            }
           }
         }
         if (kSubs == 1) __builtin_amdgcn_sched_barrier(0);
@@ -668,10 +698,15 @@ __global__ void __launch_bounds__(64 * kBwdWaves,
         if (!kDv && !(kMaps >> m & 1)) continue;
         p[m] = kFromLse ? rows16(stats[m], sub, half) : f32x16{};
 #pragma unroll
-        for (int u = 0; u < S::kSteps; ++u)
-          if (S::counts(u * 2 * kChunk<T>, kPad, a.D))
+        for (int part = 0; part < S::kParts; ++part) {
+          if (!S::taken(part, kPad, a.D)) continue;
+#pragma unroll
+          for (int u = S::from(S::kSteps, part);
+               u < S::upto(S::kSteps, part); ++u) {
             p[m] = mma_chunk<T>(Lds::rows(qt, rb, sub, m * S::kSteps + u),
                                 kf[m][u], p[m]);
+          }
+        }
         if constexpr (kFromLse) {
 #pragma unroll
           for (int i = 0; i < 16; ++i)
@@ -690,21 +725,30 @@ __global__ void __launch_bounds__(64 * kBwdWaves,
         for (int i = 0; i < 16; ++i) x[i] = p[0][i] - p[1][i];
         const Operand<T> map[1] = {Operand<T>(x)};
 #pragma unroll
-        for (int j = 0; j < S::kBlocks; ++j) {
-          f32x16* const acc[1] = {&dv[j]};
-          if (!S::counts(32 * j, 2 * kPad, a.Dv)) continue;
-          Lds::template transposed<1>(gt, cb, sub, 32 * j, map, acc);
-          // (reads of later columns would be taken ahead into registers that
-          // are not there)
-          if (kPad * (int)sizeof(T) > 256) __builtin_amdgcn_sched_barrier(0);
+        for (int part = 0; part < S::kParts; ++part) {
+          if (!S::taken(part, 2 * kPad, a.Dv)) continue;
+#pragma unroll
+          for (int j = S::from(S::kBlocks, part);
+               j < S::upto(S::kBlocks, part); ++j) {
+            f32x16* const acc[1] = {&dv[j]};
+            Lds::template transposed<1>(gt, cb, sub, 32 * j, map, acc);
+            // (reads of later columns would be taken ahead into registers that
+            // are not there)
+            if (kPad * (int)sizeof(T) > 256) __builtin_amdgcn_sched_barrier(0);
+          }
         }
       }
       if (kDk) {
         x = rows16(stats[2], sub, half);
 #pragma unroll
-        for (int u = 0; u < 2 * S::kSteps; ++u)
-          if (S::counts(u * 2 * kChunk<T>, 2 * kPad, a.Dv))
+        for (int part = 0; part < S::kParts; ++part) {
+          if (!S::taken(part, 2 * kPad, a.Dv)) continue;
+#pragma unroll
+          for (int u = S::from(2 * S::kSteps, part);
+               u < S::upto(2 * S::kSteps, part); ++u) {
             x = mma_chunk<T>(Lds::rows(gt, rb, sub, u), vf[u], x);
+          }
+        }
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
           if (!(kMaps >> m & 1)) continue;
@@ -714,11 +758,15 @@ __global__ void __launch_bounds__(64 * kBwdWaves,
             p[m] *= rows16(stats[3], sub, half) - x;
           const Operand<T> ds[1] = {Operand<T>(p[m])};
 #pragma unroll
-          for (int j = 0; j < S::kMapBlocks; ++j) {
-            f32x16* const acc[1] = {&dk[m][j]};
-            if (!S::counts(32 * j, kPad, a.D)) continue;
-            Lds::template transposed<1>(qt, cb, sub, map_col<kPad>(m, j), ds,
-                                        acc);
+          for (int part = 0; part < S::kParts; ++part) {
+            if (!S::taken(part, kPad, a.D)) continue;
+#pragma unroll
+            for (int j = S::from(S::kMapBlocks, part);
+                 j < S::upto(S::kMapBlocks, part); ++j) {
+              f32x16* const acc[1] = {&dk[m][j]};
+              Lds::template transposed<1>(qt, cb, sub, map_col<kPad>(m, j), ds,
+                                          acc);
+            }
           }
         }
       }
@@ -868,8 +916,8 @@ bool direct(const NpfHeads& t) {
 
 template <typename T, int kPad>
 hipError_t sized(const NpfDiffAttnArgs& a, bool bwd, hipStream_t stream) {
-  if (a.D % kChunk<T> == 0 && a.Dv % kChunk<T> == 0 && direct<T>(a.k) && direct<T>(a.v) &&
-      (!bwd || (direct<T>(a.q) && direct<T>(a.dout))))
+  if (a.D % kChunk<T> == 0 && a.Dv % kChunk<T> == 0 && direct<T>(a.k) &&
+      direct<T>(a.v) && (!bwd || (direct<T>(a.q) && direct<T>(a.dout))))
     return bwd ? bwd_sized<T, kPad, true>(a, stream)
                : fwd_sized<T, kPad, true>(a, stream);
   return bwd ? bwd_sized<T, kPad, false>(a, stream)
