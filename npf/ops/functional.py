@@ -937,7 +937,8 @@ def differential_attention(keys, queries, values, lam, scale=None, key_lengths=N
     no part in any gradient.
 
     Scores, statistics and sums are fp32; the maps' values are rounded to the
-    inputs' type for the products with V.  Differentiable once in keys,
+    inputs' type for the products with V, and their gradients for those with
+    the keys and queries.  Differentiable once in keys,
     queries, values and lam, with sums in a fixed order.
     """
     if keys.dim() != 4 or queries.dim() != 4 or values.dim() != 4:
