@@ -1005,10 +1005,36 @@ def _with_gradients(parameters, norm_type):
 
 
 def _grad_norm_ref(grads, norm_type):
-    norms = [torch.linalg.vector_norm(g, norm_type) for g in grads if g.numel()]
-    if not norms:
-        return torch.zeros((), device=grads[0].device if grads else None)
-    return torch.linalg.vector_norm(torch.stack(norms), norm_type)
+    """The norm in 64 bits, whatever the gradients' types."""
+    device = grads[0].device if grads else None
+    some = [g for g in grads if g.numel()]
+    if not some:
+        return torch.zeros((), dtype=torch.float64, device=device)
+    norms = torch._foreach_norm(some, norm_type, dtype=torch.float64)
+    return torch.linalg.vector_norm(
+        torch.stack([n if n.device == device else n.to(device) for n in norms]),
+        norm_type,
+    )
+
+
+def _norm_type_of(grads):
+    """The type a norm is returned in: fp32, or fp64 where a gradient is."""
+    wide = any(g.dtype == torch.float64 for g in grads)
+    return torch.float64 if wide else torch.float32
+
+
+def _scale_ref_(grads, c):
+    """grads *= c, a 64-bit 0-d tensor; 16-bit gradients are rounded once."""
+    kinds = {}
+    for g in grads:
+        kinds.setdefault((g.device, g.dtype), []).append(g)
+    for (device, dtype), some in kinds.items():
+        factor = c.to(device, torch.float64 if dtype == torch.float64 else torch.float32)
+        if dtype in (torch.float32, torch.float64):
+            torch._foreach_mul_(some, factor)
+        else:
+            for g in some:
+                g.copy_(g.float() * factor)
 
 
 @torch.no_grad()
@@ -1017,12 +1043,12 @@ def grad_norm(parameters, norm_type=2.0):
 
     parameters: a tensor or an iterable of tensors; those without a gradient
     are left out.  norm_type: 1, 2 or inf.  Returns a 0-d tensor on the
-    gradients' device (fp32 on a GPU, fp64 where a gradient is), outside of any
-    autograd graph; no host wait.
+    gradients' device (fp32, or fp64 where a gradient is), outside of any
+    autograd graph; no host wait.  Sums are held in 64 bits.
     """
     params, grads = _with_gradients(parameters, norm_type)
     if grads is not None:
-        return _grad_norm_ref(grads, norm_type)
+        return _grad_norm_ref(grads, norm_type).to(_norm_type_of(grads))
     return _backend.extension().grad_norm(params, norm_type, -1.0)
 
 
@@ -1044,18 +1070,17 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     params, grads = _with_gradients(parameters, norm_type)
     ext = _backend.extension()
     if error_if_nonfinite or grads is not None:
-        total = (
-            ext.grad_norm(params, norm_type, -1.0) if grads is None
-            else _grad_norm_ref(grads, norm_type)
-        )
+        if grads is None:
+            total = ext.grad_norm(params, norm_type, -1.0)
+        else:
+            wide = _grad_norm_ref(grads, norm_type)
+            total = wide.to(_norm_type_of(grads))
         if error_if_nonfinite and not bool(torch.isfinite(total)):
             raise RuntimeError(
                 f"the norm of order {norm_type} of the gradients is {float(total)}, "
                 "so they cannot be clipped"
             )
         if grads is not None:
-            c = torch.clamp(max_norm / (total + 1e-6), max=1.0)
-            for g in grads:
-                g.mul_(c.to(g.device))
+            _scale_ref_(grads, torch.clamp(max_norm / (wide + 1e-6), max=1.0))
             return total
     return ext.grad_norm(params, norm_type, max_norm)
