@@ -23,6 +23,8 @@ struct NpfDiffAttnArgs {
   float* dq_part;         // backward: parts of a split sum, [dq_splits, B, H,
   float* dk_part;         // Q, 2D] and [dkv_splits, B, Hk, K, 2D or Dv], where
   float* dv_part;         // there are several
+  float* reach;           // backward, fp16: [v_chunks + o_chunks, B * Hk], the
+                          // largest norms of rows of values and of dout
   float scale;
   int B, H, Hk, Q, K, D, Dv;
   int type, lam_type;
@@ -35,7 +37,11 @@ struct NpfDiffAttnArgs {
   int splits;  // parts of the key axis, forward
   int dq_splits;   // parts of the key axis, and of the query axis, backward
   int dkv_splits;
+  int v_chunks;    // of kReachRows rows of values, and of dout of a key head's
+  int o_chunks;    // queries; 0 where `reach` is not wanted
 };
+
+constexpr int kReachRows = 64;
 
 // fills the plan; false where no kernel covers the sizes
 bool npf_diff_attn_plan(NpfDiffAttnArgs&);

@@ -199,6 +199,62 @@ __global__ void __launch_bounds__(256) row_stats(NpfDiffAttnArgs a) {
         float4{a.lse[2L * r], a.lse[2L * r + 1], d1, d2};
 }
 
+// The largest norm of a chunk of rows of values, or of dout times the larger of
+// 1 and |lam|; keys that are not there, and rows without keys, do not count.
+// (A NaN is left out: it makes every gradient that its row meets NaN.)
+// Measured: 16 x 4 heads, 1024 x 1024, maps of 16: 6 us of a step of 125; 2 x 16
+// heads on 4, 4096 x 4096, maps of 64: 22 us (48 MB) of 1835.
+template <typename T, int kLanes>
+__global__ void __launch_bounds__(256) row_reach(NpfDiffAttnArgs a) {
+  __shared__ float smem[4];
+  const int heads = a.B * a.Hk, bh = blockIdx.x % heads;
+  const int chunk = blockIdx.x / heads, b = bh / a.Hk, hk = bh % a.Hk;
+  const int group = a.H / a.Hk, n = keys_of(a, b);
+  const bool of_values = chunk < a.v_chunks;
+  const int row0 = (of_values ? chunk : chunk - a.v_chunks) * kReachRows;
+  const int rows = of_values ? n : n > 0 ? group * a.Q : 0;
+  const int c = (threadIdx.x % kLanes) * 4;
+  const int count = a.Dv - c < 4 ? a.Dv - c : 4;
+  // every row's loads before the first sum: one wait for memory, not one a row
+  constexpr int kEach = kReachRows * kLanes / 256;
+  T v[kEach][4] = {};
+  float weight[kEach];
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const int row = row0 + i * (256 / kLanes) + threadIdx.x / kLanes;
+    weight[i] = 1.f;
+    if (row >= rows) continue;
+    const int h = of_values ? hk : hk * group + row / a.Q;
+    const T* p = (of_values ? row_of<T>(a.v, b, h, row)
+                            : row_of<T>(a.dout, b, h, row % a.Q)) + c;
+    if (!of_values) weight[i] = fmaxf(1.f, fabsf(lam_of(a, h)));
+    if (count == 4) {
+      load_pack(v[i], p);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (e < count) v[i][e] = p[e];
+    }
+  }
+  float most = 0.f;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    float s = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s += (float)v[i][e] * (float)v[i][e];
+#pragma unroll
+    for (int off = kLanes / 2; off > 0; off >>= 1)
+      s += __shfl_xor(s, off, 64);
+    most = fmaxf(most, sqrtf(s) * weight[i]);
+  }
+  most = wave_allreduce_max(most);
+  if ((threadIdx.x & 63) == 0) smem[threadIdx.x >> 6] = most;
+  __syncthreads();
+  if (threadIdx.x == 0)
+    a.reach[(long)chunk * heads + bh] =
+        fmaxf(fmaxf(smem[0], smem[1]), fmaxf(smem[2], smem[3]));
+}
+
 // dlam of one head (of all heads where lam is one number)
 __global__ void __launch_bounds__(1024) sum_dlam(NpfDiffAttnArgs a,
                                                  int heads) {
@@ -262,6 +318,16 @@ void stats(const NpfDiffAttnArgs& a, hipStream_t stream) {
 }
 
 template <typename T>
+void reach(const NpfDiffAttnArgs& a, hipStream_t stream) {
+  if constexpr (kScaledGrads<T>)
+    with_lanes(a.Dv, [&](auto lanes) {
+      row_reach<T, lanes()>
+          <<<(unsigned)a.B * a.Hk * (a.v_chunks + a.o_chunks), 256, 0, stream>>>(
+              a);
+    });
+}
+
+template <typename T>
 void join_one(const NpfHeads& out, const float* part, int B, int H, int L,
               int size, int splits, hipStream_t stream) {
   if (!out.p || splits == 1) return;
@@ -312,6 +378,10 @@ bool npf_diff_attn_plan(NpfDiffAttnArgs& a) {
   a.dq_splits = parts_for(row_blocks4, wanted, a.K, 256);
   a.dkv_splits =
       parts_for(heads * ((a.K + 127) / 128), wanted, (int)rows, 256);
+  if (a.type == NPF_F16) {
+    a.v_chunks = (a.K + kReachRows - 1) / kReachRows;
+    a.o_chunks = (int)((rows + kReachRows - 1) / kReachRows);
+  }
   return true;
 }
 
@@ -338,7 +408,8 @@ hipError_t npf_diff_attn_fwd(const NpfDiffAttnArgs& a, hipStream_t stream) {
 
 hipError_t npf_diff_attn_bwd(const NpfDiffAttnArgs& a, hipStream_t stream) {
   if ((long)a.dq_splits * a.B * a.H * a.Q > 0x7fffffffL ||
-      (long)a.B * a.Hk * a.K > 0x7fffffffL)
+      (long)a.B * a.Hk * a.K > 0x7fffffffL ||
+      (long)a.B * a.Hk * (a.v_chunks + a.o_chunks) > 0x7fffffffL)
     return hipErrorInvalidConfiguration;
   hipError_t e = hipErrorInvalidValue;
   switch (a.type) {
@@ -353,6 +424,7 @@ hipError_t npf_diff_attn_bwd(const NpfDiffAttnArgs& a, hipStream_t stream) {
       if (e == hipSuccess) e = join_backward<npf_bf16>(a, stream);
       break;
     case NPF_F16:
+      reach<npf_f16>(a, stream);
       stats<npf_f16>(a, stream);
       e = npf_diff_attn_bwd_f16(a, stream);
       if (e == hipSuccess) e = join_backward<npf_f16>(a, stream);

@@ -423,6 +423,7 @@ __global__ void __launch_bounds__(64 * kBwdWaves, (kResident<T, kPad>))
   const float lam = lam_of(a, h), c = a.scale * kLog2e;
   // the row's statistics; the dk/dv kernel finds them in a.stats
   float4 st = {0.f, 0.f, 0.f, 0.f};
+  float square = 0.f;  // of the row of dout
 #pragma unroll
   for (int u = 0; u < 2 * S::kSteps; ++u) {
     if (!live) break;
@@ -437,10 +438,18 @@ __global__ void __launch_bounds__(64 * kBwdWaves, (kResident<T, kPad>))
     for (int i = 0; i < kChunk<T>; ++i) {
       st.z += (float)g[i] * ((float)o[i] + lam * (float)o2[i]);
       st.w += (float)g[i] * (float)o2[i];
+      if (kScaledGrads<T>) square += (float)g[i] * (float)g[i];
     }
   }
   st.z = both_sum(st.z);
   st.w = both_sum(st.w);
+  // maps are taken 2^e times as large, each row's by its own e
+  float e = 0.f;
+  if constexpr (kScaledGrads<T>)
+    e = reach_exponent(
+        reach_bound(sqrtf(both_sum(square)) * fmaxf(1.f, fabsf(lam)),
+                    reach_of(a, 0, a.v_chunks, bh)));
+  const float back = kScaledGrads<T> ? __builtin_amdgcn_exp2f(-e) : 1.f;
   if (live) {
     st.x = a.lse[2 * stat];
     st.y = a.lse[2 * stat + 1];
@@ -510,7 +519,7 @@ __global__ void __launch_bounds__(64 * kBwdWaves, (kResident<T, kPad>))
             }
           }
         }
-        const float lse = m ? st.y : st.x;
+        const float lse = (m ? st.y : st.x) - e;
 #pragma unroll
         for (int t = 0; t < kSubs; ++t) {
 #pragma unroll
@@ -566,7 +575,7 @@ __global__ void __launch_bounds__(64 * kBwdWaves, (kResident<T, kPad>))
   }
   if (k0 < n) pass(std::true_type{}, k0, full & 1 ? odd : even);
 
-  dlam = both_sum(dlam) + (split == 0 ? st.w : 0.f);
+  dlam = both_sum(dlam) * back + (split == 0 ? st.w : 0.f);
   if (!live) return;
   const long part = (long)split * a.B * a.H * a.Q + stat;
   if ((kMaps & 2) && half == 0) a.dlam_rows[part] = dlam;
@@ -581,7 +590,7 @@ __global__ void __launch_bounds__(64 * kBwdWaves, (kResident<T, kPad>))
       for (int g = 0; g < 4; ++g) {
         if (kPad == 16 && g / 2 != m) continue;
         const int d = (kPad == 16 ? 8 * (g % 2) : 32 * j + 8 * g) + 4 * half;
-        const f32x16 x = dq[m][j] * (m ? -lam * a.scale : a.scale);
+        const f32x16 x = dq[m][j] * back * (m ? -lam * a.scale : a.scale);
         if (a.dq_splits > 1)
           store4(sum + m * a.D + d, a.D - d, x[4 * g], x[4 * g + 1],
                  x[4 * g + 2], x[4 * g + 3]);
@@ -610,7 +619,7 @@ __global__ void __launch_bounds__(64 * kBwdWaves,
   // Of each tile's queries what the products start from, and what parts the
   // two maps: the scores' -lse_i / c in 16 bits, where the maps' rounding hides
   // that they are summed at that size (lse_i in 32 bits); -delta_1 and
-  // delta_2 - delta_1.
+  // delta_2 - delta_1 (for scaled maps lam times that).
   constexpr bool kFromLse = sizeof(T) == 2;
   __shared__ __attribute__((aligned(16))) float even_stats[4][kTile];
   __shared__ __attribute__((aligned(16))) float odd_stats[4][kTile];
@@ -648,6 +657,13 @@ __global__ void __launch_bounds__(64 * kBwdWaves,
 #pragma unroll
   for (int j = 0; j < S::kBlocks; ++j) dv[j] = f32x16{};
 
+  // maps are taken 2^e times as large, all rows' by one e: they meet in sums
+  float e = 0.f;
+  if constexpr (kScaledGrads<T> && kDk)
+    e = reach_exponent(reach_bound(reach_of(a, a.v_chunks, a.o_chunks, bh),
+                                   reach_of(a, 0, a.v_chunks, bh)));
+  const float back = kScaledGrads<T> ? __builtin_amdgcn_exp2f(-e) : 1.f;
+
   // (head, tile) pairs in one sequence, this split's part of it; none where
   // the block has no keys
   const int q_tiles = (a.Q + kTile - 1) / kTile;
@@ -676,10 +692,15 @@ __global__ void __launch_bounds__(64 * kBwdWaves,
   auto store = [&](char* to, float (*to_stats)[kTile]) {
     stage.store(a.Q - next_q, to);
     if (threadIdx.x < kTile) {
+      if (kScaledGrads<T>) {
+        st.x -= e;
+        st.y -= e;
+      }
       to_stats[0][threadIdx.x] = kFromLse ? -st.x / c : st.x;
       to_stats[1][threadIdx.x] = kFromLse ? -st.y / c : st.y;
       to_stats[2][threadIdx.x] = -st.z;
-      to_stats[3][threadIdx.x] = st.w - st.z;
+      to_stats[3][threadIdx.x] =
+          kScaledGrads<T> ? next_lam * (st.w - st.z) : st.w - st.z;
     }
     next_q += kTile;
     if (next_q >= a.Q) {
@@ -718,11 +739,18 @@ __global__ void __launch_bounds__(64 * kBwdWaves,
             p[m][i] =
                 __builtin_amdgcn_exp2f(__builtin_fmaf(p[m][i], c, -lse[i]));
         }
-        if (m) p[m] *= lam;
+        // (scaled maps take lam in the two sums below instead)
+        if (m && !kScaledGrads<T>) p[m] *= lam;
       }
       if (kDv) {
+        const float lam_back = lam * back;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] = p[0][i] - p[1][i];
+        for (int i = 0; i < 16; ++i) {
+          if constexpr (kScaledGrads<T>)
+            x[i] = __builtin_fmaf(-lam_back, p[1][i], p[0][i] * back);
+          else
+            x[i] = p[0][i] - p[1][i];
+        }
         const Operand<T> map[1] = {Operand<T>(x)};
 #pragma unroll
         for (int part = 0; part < S::kParts; ++part) {
@@ -752,10 +780,16 @@ __global__ void __launch_bounds__(64 * kBwdWaves,
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
           if (!(kMaps >> m & 1)) continue;
-          if (m == 0)
+          if (m == 0) {
             p[m] *= x;
-          else
+          } else if constexpr (kScaledGrads<T>) {
+            const f32x16 apart = rows16(stats[3], sub, half);
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              p[m][i] *= __builtin_fmaf(-lam, x[i], apart[i]);
+          } else {
             p[m] *= rows16(stats[3], sub, half) - x;
+          }
           const Operand<T> ds[1] = {Operand<T>(p[m])};
 #pragma unroll
           for (int part = 0; part < S::kParts; ++part) {
@@ -814,8 +848,8 @@ __global__ void __launch_bounds__(64 * kBwdWaves,
           const int d = (kPad == 16 ? 8 * (g % 2) : 32 * j + 8 * g) + 4 * half;
           float x[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            x[e] = live ? dk[m][j][4 * g + e] * a.scale : 0.f;
+          for (int i = 0; i < 4; ++i)
+            x[i] = live ? dk[m][j][4 * g + i] * back * a.scale : 0.f;
           if (a.dkv_splits > 1)
             store4(sum + m * a.D + d, a.D - d, x[0], x[1], x[2], x[3]);
           else

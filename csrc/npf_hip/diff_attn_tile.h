@@ -394,6 +394,34 @@ __device__ __forceinline__ float lam_of(const NpfDiffAttnArgs& a, int h) {
   return load_coded(a.lam, a.lam_type, h * a.lam_stride);
 }
 
+// In fp16 gradients of the maps are rounded as 2^e dS: unscaled, those above
+// 65504 would become inf where the gradients that follow from them are finite.
+// |dS| <= |G - delta|, and G and delta (a mean of G) are products of a row of
+// dout and rows of values, so 2 |dO_i| max_j |V_j| bounds it; twice that, and
+// the weight of the second map where it is above 1, leave room for the rounding
+// that delta has seen.  e brings the bound just below 2^15, which keeps 40
+// binary places under it from vanishing.
+template <typename T>
+constexpr bool kScaledGrads = std::is_same<T, npf_f16>::value;
+
+__device__ __forceinline__ float reach_bound(float dout, float values) {
+  return 4.f * dout * values;
+}
+// the largest e, within reason, with bound 2^e < 2^15; 0 where there is none
+__device__ __forceinline__ float reach_exponent(float bound) {
+  if (!(bound > 0.f && bound < INFINITY)) return 0.f;
+  const int e = 15 - __builtin_amdgcn_frexp_expf(bound);
+  return (float)(e < -60 ? -60 : e > 60 ? 60 : e);
+}
+// the largest of a head's chunks from `first` on, in every lane of a wave
+__device__ __forceinline__ float reach_of(const NpfDiffAttnArgs& a, int first,
+                                          int chunks, int bh) {
+  float x = 0.f;
+  for (int i = threadIdx.x & 63; i < chunks; i += 64)
+    x = fmaxf(x, a.reach[(long)(first + i) * a.B * a.Hk + bh]);
+  return wave_allreduce_max(x);
+}
+
 // x of the other lane half, for a reduction over both
 struct Halves {
   float low, high;

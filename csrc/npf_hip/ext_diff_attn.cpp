@@ -177,6 +177,12 @@ struct DiffAttn : torch::autograd::Function<DiffAttn> {
       a.dq_part = parts(dq_part, dq, a.dq_splits);
       a.dk_part = parts(dk_part, dk, a.dkv_splits);
       a.dv_part = parts(dv_part, dv, a.dkv_splits);
+      Tensor reach;
+      if (a.v_chunks) {
+        reach = npf_empty({(long)a.B * a.Hk * (a.v_chunks + a.o_chunks)},
+                          torch::kFloat32, q);
+        a.reach = reach.data_ptr<float>();
+      }
       a.out = heads_of(out);
       a.o2 = heads_of(o2);
       a.dout = heads_of(dout);

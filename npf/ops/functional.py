@@ -938,8 +938,10 @@ def differential_attention(keys, queries, values, lam, scale=None, key_lengths=N
 
     Scores, statistics and sums are fp32; the maps' values are rounded to the
     inputs' type for the products with V, and their gradients for those with
-    the keys and queries.  Differentiable once in keys,
-    queries, values and lam, with sums in a fixed order.
+    the keys and queries (in fp16 after a scaling by a power of two, so that
+    they neither pass the type's largest value nor fall below its smallest).
+    Differentiable once in keys, queries, values and lam, with sums in a fixed
+    order.
     """
     if keys.dim() != 4 or queries.dim() != 4 or values.dim() != 4:
         raise ValueError("keys, queries and values must be [batch, heads, length, size]")

@@ -11,7 +11,9 @@ import pytest
 import torch
 
 from npf import ops
-from test_train_ops import E32, SHAPES, check_clip, params_of
+from test_train_ops import (E32, SHAPES, assert_within, attn_inputs, attn_oracle,
+                            check_attn, check_clip, lowest_step, params_of,
+                            run_attn)
 
 HALF = [torch.bfloat16, torch.float16]
 
@@ -53,3 +55,122 @@ class TestComposedClip:
         assert (total - want).abs() <= 256 * 2.0 ** -53 * want
         off = (wide[0].grad - old / (want + 1e-6)).abs()
         assert (off <= 256 * 2.0 ** -53 * old.abs()).all()
+
+
+# --------------------------------------------------------------------------- #
+# differential attention: ranges of fp16
+# --------------------------------------------------------------------------- #
+
+
+def largest_map_gradient(a, scale):
+    """The largest |P (G - delta)| of both maps, and 4 max|dO| max|V| max(1, |lam|)."""
+    k, q, v, do = (a[n].double() for n in ("keys", "queries", "values", "dout"))
+    G = q.shape[1] // k.shape[1]
+    k, v = k.repeat_interleave(G, 1), v.repeat_interleave(G, 1)
+    D = q.shape[-1] // 2
+    dA = do @ v.transpose(-1, -2)
+    most = 0.0
+    for s in (slice(0, D), slice(D, 2 * D)):
+        P = (q[..., s] @ k[..., s].transpose(-1, -2) * scale).softmax(-1)
+        dS = P * (dA - (P * dA).sum(-1, keepdim=True))
+        most = max(most, dS.abs().max().item())
+    reach = 4 * do.norm(dim=-1).max() * v.norm(dim=-1).max() * max(1.0, a["lam"].abs().max())
+    return most, reach.item()
+
+
+def scaled_oracle(a, scale, lengths=None):
+    """attn_oracle where gradients of the maps are rounded as 2^e dS, with
+    2^e reach between 2^14 and 2^15, so that 2^-25 2^-e is lost where it is
+    small: results are linear in dout, and with dout 2^e as large the unscaled
+    form loses the same."""
+    _, reach = largest_map_gradient(a, scale)
+    e = math.floor(14 - math.log2(reach))
+    res = attn_oracle(dict(a, dout=a["dout"].double() * 2.0 ** e), scale, lengths)
+    for n in ("dq", "dk", "dv", "dlam"):
+        t = a["lam"].dtype if n == "dlam" else a["queries"].dtype
+        value, bound = res[n]
+        res[n] = (value * 2.0 ** -e, bound * 2.0 ** -e + lowest_step(t))
+    return res
+
+
+FP16_SIZES = [
+    # B, H, Hk, Q, K, D, Dv: one launch for all gradients of the keys, or
+    # several; whole 16-byte chunks or not; sums over split axes
+    (1, 2, 1, 70, 90, 16, 32),
+    (2, 4, 2, 33, 65, 20, 40),
+    (1, 2, 1, 300, 700, 24, 48),
+    (2, 2, 2, 40, 200, 64, 128),
+    (1, 2, 1, 260, 530, 63, 100),
+    (1, 2, 2, 130, 140, 128, 256),
+]
+
+
+class TestFp16Ranges:
+    def inputs(self, sizes, dout, values, spread=1.0, scale=1 / 64):
+        a = attn_inputs(*sizes, torch.float32)
+        # scores of size 3
+        size = math.sqrt(3 / scale / math.sqrt(sizes[5]))
+        a["queries"] *= size
+        a["keys"] *= size
+        a["values"] *= values
+        a["dout"] *= dout
+        a["dout"][:, :, ::2] *= spread
+        return {n: t if n == "lam" else t.half() for n, t in a.items()}, scale
+
+    @pytest.mark.gpu
+    @pytest.mark.parametrize("sizes", FP16_SIZES)
+    def test_gradients_of_maps_over_the_largest_value(self, sizes):
+        a, scale = self.inputs(sizes, 700.0, 24.0)
+        most, _ = largest_map_gradient(a, scale)
+        assert most > 65504
+        want = scaled_oracle(a, scale)
+        assert all(value.abs().max() < 60000 for n, (value, _) in want.items()
+                   if n != "dlam")
+        check_attn(run_attn("cuda", a, scale=scale), want)
+
+    @pytest.mark.gpu
+    @pytest.mark.parametrize("sizes", FP16_SIZES)
+    def test_small_gradients_of_maps(self, sizes):
+        # all of them below the smallest normal value, in part below its last step
+        a, scale = self.inputs(sizes, 2.0 ** -13, 2.0 ** -6, scale=64.0)
+        most, _ = largest_map_gradient(a, scale)
+        assert most < 2.0 ** -14
+        check_attn(run_attn("cuda", a, scale=scale), scaled_oracle(a, scale))
+
+    @pytest.mark.gpu
+    @pytest.mark.parametrize("sizes", FP16_SIZES[:4])
+    def test_rows_of_unequal_size(self, sizes):
+        a, scale = self.inputs(sizes, 0.5, 24.0, spread=1400.0)
+        check_attn(run_attn("cuda", a, scale=scale), scaled_oracle(a, scale))
+        B, K = sizes[0], sizes[4]
+        lens = [0] * (B - 1) + [K - 7]
+        check_attn(run_attn("cuda", a, scale=scale, lengths=lens),
+                   scaled_oracle(a, scale, lengths=lens))
+
+    @pytest.mark.gpu
+    @pytest.mark.parametrize("lam", [0.0, -40.0, 900.0])
+    def test_weights_of_the_second_map(self, lam):
+        a, scale = self.inputs(FP16_SIZES[0], 1.0, 1.0)
+        a["lam"] = torch.tensor(lam)
+        check_attn(run_attn("cuda", a, scale=scale), scaled_oracle(a, scale))
+
+    @pytest.mark.gpu
+    def test_zeros_and_values_that_are_not_finite(self):
+        a, scale = self.inputs((2, 2, 1, 40, 60, 16, 32), 1.0, 1.0)
+        zero = dict(a, dout=torch.zeros_like(a["dout"]))
+        got = run_attn("cuda", zero, scale=scale)
+        assert not any(got[n].any() for n in ("dq", "dk", "dv", "dlam"))
+        # one row's gradient: the rows and keys of the other entry stay
+        want = scaled_oracle(a, scale)
+        for bad in (math.inf, math.nan):
+            b = dict(a, dout=a["dout"].clone())
+            b["dout"][0, 1, 3, 5] = bad
+            got = run_attn("cuda", b, scale=scale)
+            assert not got["dk"][0].isfinite().any()
+            assert not got["dq"][0, 1, 3].isfinite().any()
+            for n in ("dq", "dk", "dv"):
+                value, bound = want[n]
+                assert_within(got[n][1], value[1], bound[1], n)
+            rows = [i for i in range(40) if i != 3]
+            value, bound = want["dq"]
+            assert_within(got["dq"][0, 1, rows], value[0, 1, rows], bound[0, 1, rows], "dq")
