@@ -231,9 +231,15 @@ __global__ void __launch_bounds__(128 * kRowWaves,
       top = both_max(top) * c;
       // The maximum is raised only where it is exceeded by 2^8: exponents stay
       // below that, far from any type's end, and most tiles leave the sums as
-      // they are.
-      if (__any(top > mx + 8.f)) {
-        const float up = fmaxf(mx, top);
+      // they are.  In fp16 it is held 2^7 too low, so that exponents reach from
+      // 2^15 down to steps of 2^-24: values below 2^-24 of the largest, of
+      // which a long context may hold most, count on down to 2^-31.  (Not
+      // where scores are so large that their products' rounding nears that.)
+      float under = 0.f;
+      if (std::is_same<T, npf_f16>::value && fabsf(top) < 1048576.f)
+        under = 7.f;
+      if (__any(top > mx + (8.f + under))) {
+        const float up = fmaxf(mx, top - under);
         const float f = __builtin_amdgcn_exp2f(mx - up);
         mx = up;
         l *= f;
@@ -657,12 +663,24 @@ __global__ void __launch_bounds__(64 * kBwdWaves,
 #pragma unroll
   for (int j = 0; j < S::kBlocks; ++j) dv[j] = f32x16{};
 
-  // maps are taken 2^e times as large, all rows' by one e: they meet in sums
-  float e = 0.f;
-  if constexpr (kScaledGrads<T> && kDk)
-    e = reach_exponent(reach_bound(reach_of(a, a.v_chunks, a.o_chunks, bh),
-                                   reach_of(a, 0, a.v_chunks, bh)));
-  const float back = kScaledGrads<T> ? __builtin_amdgcn_exp2f(-e) : 1.f;
+  // Maps are taken 2^e times as large, all rows' by one e: they meet in sums.
+  // For dv, P_1 - lam P_2 is rounded as 2^ea times itself, below 2^15 as well.
+  float e = 0.f, ea = 0.f;
+  if constexpr (kScaledGrads<T>) {
+    if (kDv) {
+      float most = 0.f;
+      for (int i = lane; i < group; i += 64)
+        most = fmaxf(most, fabsf(lam_of(a, hk * group + i)));
+      ea = reach_exponent(1.f + wave_allreduce_max(most));
+    }
+    e = kDk ? reach_exponent(reach_bound(reach_of(a, a.v_chunks, a.o_chunks, bh),
+                                         reach_of(a, 0, a.v_chunks, bh)))
+            : ea;
+  }
+  auto power = [](float x) {
+    return kScaledGrads<T> ? __builtin_amdgcn_exp2f(x) : 1.f;
+  };
+  const float back = power(-e), dv_back = power(-ea), to_dv = power(ea - e);
 
   // (head, tile) pairs in one sequence, this split's part of it; none where
   // the block has no keys
@@ -743,11 +761,11 @@ __global__ void __launch_bounds__(64 * kBwdWaves,
         if (m && !kScaledGrads<T>) p[m] *= lam;
       }
       if (kDv) {
-        const float lam_back = lam * back;
+        const float lam_dv = lam * to_dv;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           if constexpr (kScaledGrads<T>)
-            x[i] = __builtin_fmaf(-lam_back, p[1][i], p[0][i] * back);
+            x[i] = __builtin_fmaf(-lam_dv, p[1][i], p[0][i] * to_dv);
           else
             x[i] = p[0][i] - p[1][i];
         }
@@ -866,7 +884,8 @@ __global__ void __launch_bounds__(64 * kBwdWaves,
         const int d = 32 * j + 8 * g + 4 * half;
         float x[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = live ? dv[j][4 * g + e] : 0.f;
+        for (int i = 0; i < 4; ++i)
+          x[i] = live ? dv[j][4 * g + i] * dv_back : 0.f;
         if (a.dkv_splits > 1)
           store4(sum + d, a.Dv - d, x[0], x[1], x[2], x[3]);
         else

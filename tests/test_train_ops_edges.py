@@ -155,6 +155,72 @@ class TestFp16Ranges:
         check_attn(run_attn("cuda", a, scale=scale), scaled_oracle(a, scale))
 
     @pytest.mark.gpu
+    def test_weight_over_the_largest_value(self):
+        # P_1 - lam P_2 passes 65504, what follows from it does not
+        a, scale = self.inputs(FP16_SIZES[0], 2.0 ** -6, 2.0 ** -6)
+        a["lam"] = torch.tensor([3e5, -2e5])
+        want = scaled_oracle(a, scale)
+        assert all(want[n][0].abs().max() < 60000 for n in ("out", "dq", "dk", "dv"))
+        check_attn(run_attn("cuda", a, scale=scale), want)
+
+    @pytest.mark.gpu
+    @pytest.mark.parametrize("H, Hk, Q, K, D", [
+        (1, 1, 1, 50000, 16), (2, 1, 130, 20000, 16), (1, 1, 200, 9000, 64),
+        (1, 1, 40, 7000, 20), (1, 1, 3, 9000, 128),
+    ])
+    def test_many_small_map_values(self, H, Hk, Q, K, D):
+        # One key with the weight 1, all others with e^-18, below 2^-25, which
+        # is rounded to zero: most of a result is theirs, in both maps.
+        k = torch.full((1, Hk, K, 2 * D), -18.0 / D).half()
+        k[:, :, K // 3] = 0.0
+        q = torch.ones(1, H, Q, 2 * D).half()
+        v = torch.full((1, Hk, K, 2 * D), 16.0).half()
+        v[:, :, K // 3] = 2.0 ** -9
+        dout = torch.full((1, H, Q, 2 * D), 64.0).half()
+        a = dict(keys=k, queries=q, values=v, lam=torch.tensor(0.25), dout=dout)
+        got = run_attn("cuda", a, scale=1.0)
+        P = k[0, 0, :, :D].double().sum(-1).softmax(-1)
+        out = 0.75 * (P @ v[0, 0].double())
+        # a map's values are rounded to half a step u each and below 2^-14 of
+        # what is rounded, 2^-7 as large, to 2^-25; scores of 18 and sums of K
+        # terms in fp32; both maps, weighted 1 and 1/4; the result once more
+        u = 2.0 ** -11
+        rel = u + 64 * E32 * 18 + 2 * (K + 16) * E32
+        bound = 1.25 * ((P * rel + 2.0 ** -32) @ v[0, 0].double())
+        want = out.expand(1, H, Q, 2 * D)
+        assert_within(got["out"], want, (bound + u * out + 2.0 ** -25).expand_as(want), "out")
+        # a gradient of the values: H Q rows of 64, with the same P
+        dv = 0.75 * P[:, None] * 64.0 * (H // Hk) * Q
+        rel = 2 * u + 64 * E32 * 18 + 2 * (K + 16 + H * Q) * E32
+        bound = (1.25 / 0.75) * rel * dv + u * dv + 2.0 ** -25
+        assert_within(got["dv"], dv.expand(1, Hk, K, 2 * D), bound.expand(1, Hk, K, 2 * D), "dv")
+
+    @pytest.mark.gpu
+    def test_scores_of_millions(self):
+        # whose products' rounding is worth many powers of two: the largest
+        # score's key alone counts, and the gradients of its map are zero
+        a = attn_inputs(1, 2, 2, 70, 150, 16, 32, torch.float16)
+        a["queries"] *= 1500.0
+        a["keys"] *= 1500.0
+        q, k = a["queries"].double(), a["keys"].double()
+        first, second = (
+            (q[..., s] @ k[..., s].transpose(-1, -2)).topk(2)
+            for s in (slice(0, 16), slice(16, 32)))
+        for scores in (first.values, second.values):
+            # (fp32 sums of 16 terms of up to 2^26 are off by no more than 256)
+            assert (scores[..., 0] - scores[..., 1]).min() > 1000
+            assert 2 ** 24 < scores.max() < 2 ** 26
+        first, second = first.indices[..., 0], second.indices[..., 0]
+        pick = lambda i: a["values"].double().gather(
+            2, i[..., None].expand(-1, -1, -1, 32))
+        lam = a["lam"].double().reshape(1, 2, 1, 1)
+        want = pick(first) - lam * pick(second)
+        for lengths in (None, [150]):
+            got = run_attn("cuda", a, scale=1.0, lengths=lengths)
+            bound = 2.0 ** -11 * (3 * want.abs() + 2 * (lam * pick(second)).abs()) + 2.0 ** -24
+            assert_within(got["out"], want, bound, "out")
+
+    @pytest.mark.gpu
     def test_zeros_and_values_that_are_not_finite(self):
         a, scale = self.inputs((2, 2, 1, 40, 60, 16, 32), 1.0, 1.0)
         zero = dict(a, dout=torch.zeros_like(a["dout"]))
