@@ -1,7 +1,9 @@
 // Helpers of the binding files, and what each of them adds to npf._hip_C.
 #pragma once
 
+#include <ATen/TracerMode.h>
 #include <ATen/hip/EmptyTensor.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <hip/hip_runtime.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
@@ -25,6 +27,36 @@ inline int npf_type_code(const torch::Tensor& t, const char* name,
       TORCH_CHECK_TYPE(false, name, " has type ", t.scalar_type(),
                        ", which the kernel does not take");
   }
+}
+
+// The operators read and write memory themselves, past torch's dispatcher.  What
+// it would do for a call is refused rather than left out: recording it in a
+// trace (which would hold the first call's result as a constant) ...
+inline void npf_check_call(const char* op) {
+  using c10::impl::TorchDispatchModeKey;
+  TORCH_CHECK_NOT_IMPLEMENTED(
+      !at::tracer::impl::is_dispatch_enabled() &&
+          !c10::impl::TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::PROXY)
+               .has_value(),
+      op, " cannot be traced; NPF_DISABLE_OPS=", op,
+      " chooses the composed form");
+}
+
+// ... and what a tensor holds outside of its memory: a forward-mode tangent, or
+// all of a wrapper (of vmap, of a fake tensor) that has no memory of its own.
+inline void npf_check_plain(const torch::Tensor& t, const char* op) {
+  if (!t.defined()) return;
+  using c10::DispatchKey;
+  constexpr c10::DispatchKeySet wrappers(
+      {DispatchKey::Python, DispatchKey::FuncTorchBatched,
+       DispatchKey::FuncTorchGradWrapper, DispatchKey::Functionalize,
+       DispatchKey::Batched});
+  TORCH_CHECK_NOT_IMPLEMENTED(!t.key_set().has_any(wrappers), op,
+                              " takes no tensor that wraps another");
+  TORCH_CHECK_NOT_IMPLEMENTED(
+      !t._fw_grad(/*level=*/0).defined(), op,
+      " has no forward-mode derivative; NPF_DISABLE_OPS=", op,
+      " chooses the composed form");
 }
 
 // Contiguous memory beside `on`, from the allocator itself: torch::empty's way

@@ -13,6 +13,8 @@ namespace {
 using torch::Tensor;
 using OptTensor = std::optional<Tensor>;
 
+constexpr const char* kName = "differential_attention";
+
 NpfHeads heads_of(const Tensor& t) {
   return {t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)};
 }
@@ -150,6 +152,7 @@ struct DiffAttn : torch::autograd::Function<DiffAttn> {
     const Tensor &k = saved[0], &q = saved[1], &v = saved[2], &lam = saved[3],
                  &lengths = saved[4], &out = saved[5], &o2 = saved[6],
                  &lse = saved[7];
+    npf_check_plain(grads[0], kName);
     c10::DeviceGuard guard(q.device());
     NpfDiffAttnArgs a = common_args(q, k, v, lam,
                                     ctx->saved_data["scale"].toDouble(),
@@ -204,6 +207,9 @@ struct DiffAttn : torch::autograd::Function<DiffAttn> {
 Tensor differential_attention(const Tensor& k_, const Tensor& q_,
                               const Tensor& v_, const Tensor& lam, double scale,
                               const OptTensor& lengths_) {
+  npf_check_call(kName);
+  for (const Tensor* t : {&k_, &q_, &v_, &lam}) npf_check_plain(*t, kName);
+  if (lengths_) npf_check_plain(*lengths_, kName);
   const Tensor k = as_heads(k_), q = as_heads(q_), v = as_heads(v_);
   OptTensor lengths;
   if (lengths_) lengths = lengths_->contiguous();

@@ -109,6 +109,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     const int64_t needs = ctx->saved_data["needs"].toInt();
     const Tensor &x = saved[0], &residual = saved[1], &weight = saved[2],
                  &bias = saved[3], &stats = saved[4];
+    npf_check_plain(grads[0], "layer_norm");
     c10::DeviceGuard guard(x.device());
     NpfLayerNormArgs a = norm_args(x, residual, weight, bias);
     const Tensor dy = grads[0].contiguous();
@@ -145,6 +146,10 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 Tensor layer_norm(const Tensor& x, const OptTensor& residual_,
                   const OptTensor& weight_, const OptTensor& bias_,
                   double eps) {
+  npf_check_call("layer_norm");
+  npf_check_plain(x, "layer_norm");
+  for (const OptTensor* t : {&residual_, &weight_, &bias_})
+    if (*t) npf_check_plain(**t, "layer_norm");
   TORCH_CHECK_VALUE(x.is_cuda() && x.dim() >= 1 && x.size(-1) > 0,
                     "layer_norm takes rows of at least one value on a GPU");
   TORCH_CHECK_VALUE(x.size(-1) <= std::numeric_limits<int>::max() / 2,
@@ -249,6 +254,7 @@ void check_apart(const std::vector<NpfGradSpans>& all) {
 // scales them in place
 Tensor grad_norm(const std::vector<Tensor>& params, double norm_type,
                  double max_norm) {
+  npf_check_call("grad_norm");
   const int norm = norm_code(norm_type);
   std::vector<Tensor> grads;
   grads.reserve(params.size());
@@ -257,6 +263,7 @@ Tensor grad_norm(const std::vector<Tensor>& params, double norm_type,
     if (!g.defined()) continue;
     TORCH_CHECK_TYPE(g.layout() == torch::kStrided,
                      "gradients must be dense floating tensors");
+    npf_check_plain(g, "grad_norm");
     grads.push_back(g);
   }
   TORCH_CHECK_VALUE(!grads.empty(), "no gradients");

@@ -858,7 +858,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, residual=None):
     Statistics are fp32 and the sum of x and residual is not rounded; the
     result is rounded once.  Differentiable once in all four tensors; sums of
     the weight's gradient run in a fixed order.  Under autocast the inputs'
-    own types count.
+    own types count.  On a GPU forward-mode derivatives, traces and tensors
+    that wrap others raise NotImplementedError.
     """
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"layer_norm needs a last axis, got {tuple(x.shape)}")
@@ -941,7 +942,8 @@ def differential_attention(keys, queries, values, lam, scale=None, key_lengths=N
     the keys and queries (in fp16 after a scaling by a power of two, so that
     they neither pass the type's largest value nor fall below its smallest).
     Differentiable once in keys, queries, values and lam, with sums in a fixed
-    order.
+    order.  On a GPU forward-mode derivatives, traces and tensors that wrap
+    others raise NotImplementedError.
     """
     if keys.dim() != 4 or queries.dim() != 4 or values.dim() != 4:
         raise ValueError("keys, queries and values must be [batch, heads, length, size]")

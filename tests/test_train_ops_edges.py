@@ -240,3 +240,118 @@ class TestFp16Ranges:
             rows = [i for i in range(40) if i != 3]
             value, bound = want["dq"]
             assert_within(got["dq"][0, 1, rows], value[0, 1, rows], bound[0, 1, rows], "dq")
+
+
+# --------------------------------------------------------------------------- #
+# what reads memory past torch's dispatcher refuses what the latter would do
+# --------------------------------------------------------------------------- #
+
+
+def calls(device):
+    """name, call and a tensor that it takes, for each operator of the
+    extension; the others' inputs are made beforehand."""
+    g = torch.Generator().manual_seed(0)
+    x = torch.randn(4, 8, generator=g).to(device)
+    kqv = torch.randn(1, 2, 5, 8, generator=g).to(device)
+    lam = torch.tensor(0.3, device=device)
+    w = torch.ones(8, device=device)
+    ext = ops.extension()
+
+    def norm_of(grad):
+        p = torch.zeros(grad.shape, device=device, requires_grad=True)
+        p.grad = grad
+        return ext.grad_norm([p], 2.0, 0.5)
+
+    return [
+        ("layer_norm x", lambda t: ext.layer_norm(t, None, w, None, 1e-5), x),
+        ("layer_norm residual", lambda t: ext.layer_norm(x, t, None, None, 1e-5), x),
+        ("layer_norm weight", lambda t: ext.layer_norm(x, None, t, None, 1e-5), w),
+        ("layer_norm bias", lambda t: ext.layer_norm(x, None, None, t, 1e-5), w),
+        ("differential_attention k",
+         lambda t: ext.differential_attention(t, kqv, kqv, lam, 1.0, None), kqv),
+        ("differential_attention q",
+         lambda t: ext.differential_attention(kqv, t, kqv, lam, 1.0, None), kqv),
+        ("differential_attention v",
+         lambda t: ext.differential_attention(kqv, kqv, t, lam, 1.0, None), kqv),
+        ("differential_attention lam",
+         lambda t: ext.differential_attention(kqv, kqv, kqv, t, 1.0, None), lam),
+        ("grad_norm", norm_of, x),
+    ]
+
+
+@pytest.mark.skipif(not ops.has_extension(), reason="the extension is not built")
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+class TestPastTheDispatcher:
+    # (on the CPU the refusals come before the one of CPU tensors)
+
+    def test_forward_mode(self, device):
+        import torch.autograd.forward_ad as fwad
+
+        for name, call, t in calls(device):
+            with fwad.dual_level():
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    call(fwad.make_dual(t, torch.ones_like(t)))
+            if name != "grad_norm":
+                with pytest.raises(NotImplementedError, match="wraps|forward-mode"):
+                    torch.func.jvp(call, (t,), (torch.ones_like(t),))
+
+    def test_traces(self, device):
+        from torch.fx.experimental.proxy_tensor import make_fx
+
+        for name, call, t in calls(device):
+            with pytest.raises(NotImplementedError, match="traced"):
+                torch.jit.trace(call, (t,), check_trace=False)
+            for mode in ("real", "fake"):
+                with pytest.raises(NotImplementedError, match="traced|wraps"):
+                    make_fx(call, tracing_mode=mode)(t)
+
+    def test_wrappers(self, device):
+        for name, call, t in calls(device):
+            if name != "grad_norm":
+                with pytest.raises(NotImplementedError, match="wraps"):
+                    torch.func.vmap(call)(torch.stack([t, t]))
+
+    def test_gradients_of_gradients_in_forward_mode(self, device):
+        import torch.autograd.forward_ad as fwad
+
+        if device == "cpu":
+            pytest.skip("a backward pass of the extension needs a GPU")
+        x = torch.randn(4, 8, device=device, requires_grad=True)
+        kqv = torch.randn(1, 2, 5, 8, device=device, requires_grad=True)
+        lam = torch.tensor(0.3, device=device)
+        for y, t in ((ops.layer_norm(x), x),
+                     (ops.differential_attention(kqv, kqv, kqv[..., :4], lam), kqv)):
+            with fwad.dual_level():
+                dy = fwad.make_dual(torch.ones_like(y), torch.ones_like(y))
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    torch.autograd.grad(y, t, dy)
+
+
+@pytest.mark.skipif(not ops.has_extension(), reason="the extension is not built")
+def test_fake_tensors_are_refused():
+    # (which say that they are on a GPU, and have no memory)
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        x = torch.empty(4, 8, device="cuda")
+        kqv = torch.empty(1, 2, 5, 8, device="cuda")
+        lam = torch.empty((), device="cuda")
+        p = torch.empty(4, 8, device="cuda", requires_grad=True)
+        p.grad = x
+        for call in (lambda: ops.layer_norm(x), lambda: ops.grad_norm([p]),
+                     lambda: ops.clip_grad_norm_([p], 1.0),
+                     lambda: ops.differential_attention(kqv, kqv, kqv, lam)):
+            with pytest.raises(NotImplementedError, match="wraps"):
+                call()
+
+
+def test_composed_forward_mode():
+    import torch.autograd.forward_ad as fwad
+
+    x, t = torch.randn(4, 8).double(), torch.randn(4, 8).double()
+    with fwad.dual_level():
+        got = fwad.unpack_dual(ops.layer_norm(fwad.make_dual(x, t))).tangent
+    want = (ops.layer_norm(x + 1e-6 * t) - ops.layer_norm(x - 1e-6 * t)) / 2e-6
+    # differences of second order in 64 bits: 1e-12 of third derivatives, and
+    # 2^-53 over the step
+    assert (got - want).abs().max() <= 1e-8
