@@ -62,7 +62,8 @@ __global__ void __launch_bounds__(kJoinThreads) join(NpfDiffAttnArgs a) {
       o[m] = part[0][m][t] + part[1][m][t] + part[2][m][t] + part[3][m][t];
       o[m] = any ? o[m] / weight_sum[m] : 0.f;
     }
-    row_of<T>(a.out, b, h, q)[t] = (T)(o[0] - lam_of(a, h) * o[1]);
+    row_of<T>(a.out, b, h, q)[t] =
+        (T)(any ? o[0] - lam_of(a, h) * o[1] : 0.f);
     if (a.o2.p) row_of<T>(a.o2, b, h, q)[t] = (T)o[1];
   }
   if (a.lse && t < 2)

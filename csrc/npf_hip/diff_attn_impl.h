@@ -335,7 +335,7 @@ __global__ void __launch_bounds__(128 * kRowWaves,
     return reinterpret_cast<f32x4*>(
         at + ((i % kPieces * kRowWaves + row_wave) * 64 + lane) * 16);
   };
-  const float lam = lam_of(a, h);
+  const float lam = n ? lam_of(a, h) : 0.f;  // (it may be inf)
   T* out = row_of<T>(m ? a.o2 : a.out, b, h, q);
   const bool stores = live && (m == 0 || a.o2.p);
 #pragma unroll
@@ -400,7 +400,8 @@ __global__ void __launch_bounds__(64 * kBwdWaves, (kResident<T, kPad>))
   const bool live = row < rows;
   const int h = hk * group + (live ? row / a.Q : 0);
   const int q = live ? row % a.Q : 0;
-  int begin = 0, n = keys_of(a, b);  // this split's keys
+  const int keys = keys_of(a, b);
+  int begin = 0, n = keys;  // this split's
   if (a.dq_splits > 1) {
     const int per = split_keys(n, a.dq_splits, kTile);
     begin = split * per < n ? split * per : n;
@@ -426,13 +427,14 @@ __global__ void __launch_bounds__(64 * kBwdWaves, (kResident<T, kPad>))
     else
       qf[u] = x;
   }
-  const float lam = lam_of(a, h), c = a.scale * kLog2e;
+  // rows without keys have no part in any gradient, whatever lam and dout hold
+  const float lam = keys ? lam_of(a, h) : 0.f, c = a.scale * kLog2e;
   // the row's statistics; the dk/dv kernel finds them in a.stats
   float4 st = {0.f, 0.f, 0.f, 0.f};
   float square = 0.f;  // of the row of dout
 #pragma unroll
   for (int u = 0; u < 2 * S::kSteps; ++u) {
-    if (!live) break;
+    if (!live || keys == 0) break;
     const ChunkOf at = chunk_of_row<T, kPad>(u * 2 + half, a.Dv);
     T g[kChunk<T>], o[kChunk<T>], o2[kChunk<T>];
     const u32x4 x = load_chunk(row_of<T>(a.out, b, h, q), at);

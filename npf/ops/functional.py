@@ -913,11 +913,15 @@ def _differential_attention_ref(keys, queries, values, lam, scale, key_lengths):
         if key_lengths is None:
             maps.append(logits.softmax(-1))
         else:
-            row = live.transpose(-1, -2)
+            out_of = ~live.transpose(-1, -2)
             low = torch.finfo(logits.dtype).min
-            maps.append(logits.masked_fill(~row, low).softmax(-1) * row)
+            maps.append(logits.masked_fill(out_of, low).softmax(-1).masked_fill(out_of, 0))
     lam = lam.to(maps[0].dtype).reshape(-1, 1, 1)
-    return torch.matmul(maps[0] - lam * maps[1], values.contiguous()).to(dtype)
+    out = torch.matmul(maps[0] - lam * maps[1], values.contiguous())
+    if key_lengths is not None:
+        # rows without keys take nothing of lam, nor give of their gradient
+        out = out.masked_fill(~live.any(2, keepdim=True), 0)
+    return out.to(dtype)
 
 
 def differential_attention(keys, queries, values, lam, scale=None, key_lengths=None):

@@ -355,3 +355,47 @@ def test_composed_forward_mode():
     # differences of second order in 64 bits: 1e-12 of third derivatives, and
     # 2^-53 over the step
     assert (got - want).abs().max() <= 1e-8
+
+
+# --------------------------------------------------------------------------- #
+# rows without keys
+# --------------------------------------------------------------------------- #
+
+HERE = [("cpu", torch.float32)] + [
+    pytest.param("cuda", t, marks=pytest.mark.gpu)
+    for t in (torch.float32, torch.bfloat16, torch.float16)
+]
+
+
+class TestRowsWithoutKeys:
+    """Batch entries without contexts: zeros, whatever stands in their places."""
+
+    # few rows and many, sums over split axes, D 128
+    SIZES = [(3, 2, 1, 5, 9, 4, 8), (3, 2, 1, 2, 300, 16, 32),
+             (3, 2, 2, 140, 600, 16, 32), (3, 1, 1, 40, 70, 128, 256)]
+
+    @pytest.mark.parametrize("device, dtype", HERE)
+    @pytest.mark.parametrize("sizes", SIZES)
+    @pytest.mark.parametrize("bad", [math.inf, math.nan])
+    def test_gradients_that_are_not_finite(self, device, dtype, sizes, bad):
+        a = attn_inputs(*sizes, dtype)
+        lens = [sizes[4] // 2, 0, sizes[4]]
+        zero = dict(a, dout=a["dout"].clone())
+        zero["dout"][1] = 0.0
+        want = run_attn(device, zero, lengths=lens)
+        a["dout"][1] = bad
+        got = run_attn(device, a, lengths=lens)
+        for n in want:
+            assert torch.equal(got[n], want[n]), n
+        assert torch.isfinite(got["dlam"]).all()
+
+    @pytest.mark.parametrize("device, dtype", HERE)
+    @pytest.mark.parametrize("sizes", SIZES)
+    @pytest.mark.parametrize("bad", [math.inf, math.nan])
+    def test_weight_that_is_not_finite(self, device, dtype, sizes, bad):
+        a = attn_inputs(*sizes, dtype)
+        a["lam"][:] = bad
+        got = run_attn(device, a, lengths=[sizes[4], 0, 1])
+        for n in ("out", "dq", "dk", "dv"):
+            assert torch.equal(got[n][1], torch.zeros_like(got[n][1])), n
+        assert got["out"][0].isnan().all() or got["out"][0].isinf().any()
