@@ -164,13 +164,15 @@ __global__ void __launch_bounds__(kThreads)
   const double t = norm_of(partial, n, norm, smem);
   if (total && blockIdx.x == 0 && threadIdx.x == 0) store_coded(total, total_type, 0, t);
   const double ratio = max_norm / (t + 1e-6);
-  // a norm that is no number makes every gradient none
-  const float scale = ratio >= 1. ? 1.f : (float)ratio;
-  if (scale == 1.f) return;  // nothing to change
+  if (ratio >= 1.) return;  // nothing to change
+  // (a norm that is no number makes every gradient none)
+  const float scale = (float)ratio;
   // from the last chunk back: what the first pass read last is still cached
   for (int c = s.first_chunk[s.n] - 1 - (int)blockIdx.x; c >= 0;
        c -= gridDim.x) {
     const int i = span_of(s, c);
+    // a factor next to 1 is not 1 in 64 bits alone
+    if (scale == 1.f && s.type[i] != NPF_F64) continue;
     const long per = kGradChunkBytes / size_of(s.type[i]);
     const long at = (long)(c - s.first_chunk[i]) * per;
     const long m = s.count[i] - at < per ? s.count[i] - at : per;

@@ -57,6 +57,23 @@ class TestComposedClip:
         assert (off <= 256 * 2.0 ** -53 * old.abs()).all()
 
 
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("below", [1e-9, 1e-12, 0.5])
+def test_clip_factors_next_to_one(device, below):
+    # which fp32 does not tell from 1
+    wide = params_of([(300,)], torch.float64, device)
+    narrow = params_of([(200,)], torch.float32, device)
+    old = [p.grad.clone() for p in wide + narrow]
+    norm = torch.cat([g.double() for g in old]).norm()
+    # (the factor's own 1e-6 is made up for)
+    ops.clip_grad_norm_(wide + narrow, ((norm + 1e-6) * (1 - below)).item())
+    # sums of 500 terms, a root, a quotient and products in 64 bits
+    want = old[0] * (1 - below)
+    assert ((wide[0].grad - want).abs() <= 512 * 2.0 ** -53 * want.abs()).all()
+    want = old[1].double() * (1 - below)
+    assert ((narrow[0].grad - want).abs() <= 2.5 * E32 * want.abs()).all()
+
+
 # --------------------------------------------------------------------------- #
 # differential attention: ranges of fp16
 # --------------------------------------------------------------------------- #
