@@ -286,9 +286,19 @@ class NPFTrainer:
         if self.ddp is not None:
             self.ddp.reduce_()
         if self.grad_clip_norm is not None:
-            ops.clip_grad_norm_(self.module.parameters(), self.grad_clip_norm)
+            self._clip_gradients()
         self.optimizer.step()
         return loss.detach()
+
+    def _clip_gradients(self):
+        params = list(self.module.parameters())
+        try:
+            ops.clip_grad_norm_(params, self.grad_clip_norm)
+        except (NotImplementedError, TypeError, ValueError):
+            # The operator refuses gradients that are on several GPUs, share
+            # memory, have gaps in it or are complex, before any of them
+            # changes; torch's own clipping takes those.
+            torch.nn.utils.clip_grad_norm_(params, self.grad_clip_norm)
 
     def _maybe_graph_step(self, inputs, y):
         """Replay the step as one hipGraph when eligible (fixed-address

@@ -74,6 +74,72 @@ def test_clip_factors_next_to_one(device, below):
     assert ((narrow[0].grad - want).abs() <= 2.5 * E32 * want.abs()).all()
 
 
+class Oddly(torch.nn.Module):
+    """A model whose gradients the clipping operator refuses, one way each."""
+
+    def __init__(self, way, device="cpu"):
+        super().__init__()
+        dtype = torch.complex64 if way == "complex" else torch.float32
+        self.a = torch.nn.Parameter(torch.full((3, 4), 0.5, dtype=dtype))
+        self.b = torch.nn.Parameter(torch.full((3, 4), 2.0))
+        both = torch.zeros(2, 3, 8, device=device)
+        at = {"gaps": (both[0, :, ::2], both[1, :, 1::2]),
+              "shared": (both[0, :, :4], both[0, :, :4])}.get(way)
+        if at:
+            for p, g in zip((self.a, self.b), at):
+                p.register_post_accumulate_grad_hook(self.moved_to(g))
+
+    @staticmethod
+    def moved_to(place):
+        def hook(p):
+            p.grad = place.copy_(p.grad)
+        return hook
+
+    def forward(self, X):
+        return (X @ self.a.abs() @ self.b.t()).square().mean()
+
+
+class Itself(torch.nn.Module):
+    def forward(self, out, y):
+        return out
+
+
+class TestTrainerClips:
+    """Gradients that the operator refuses are clipped as they were before
+    there was one."""
+
+    @pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+    @pytest.mark.parametrize("way", ["complex", "gaps", "shared", "plain"])
+    def test_as_the_library(self, device, way):
+        from npf.train import NPFTrainer
+
+        X = torch.linspace(-1, 1, 15).reshape(5, 3).to(device)
+        t = NPFTrainer(Oddly(way, device), Itself, optimizer=torch.optim.SGD,
+                       lr=1.0, device=device, grad_clip_norm=0.1)
+        before = [p.detach().clone() for p in t.module.parameters()]
+        t.train_step(dict(X=X), None)
+        got = [b - p.detach() for b, p in zip(before, t.module.parameters())]
+        m = Oddly(way, device).to(device)
+        m(X).backward()
+        total = torch.nn.utils.clip_grad_norm_(m.parameters(), 0.1)
+        assert total > 0.1
+        if way == "shared" and device == "cuda":
+            # the library's one launch scales the same values twice at once
+            assert all(torch.isfinite(g).all() for g in got)
+            return
+        for g, p in zip(got, m.parameters()):
+            # norms of 24 terms, the factor and the step, in fp32
+            assert ((g - p.grad).abs() <= 64 * E32 * (2.0 + p.grad.abs())).all()
+
+    def test_negative_limits_are_the_librarys(self):
+        from npf.train import NPFTrainer
+
+        X = torch.linspace(-1, 1, 15).reshape(5, 3)
+        t = NPFTrainer(Oddly("plain"), Itself, optimizer=torch.optim.SGD,
+                       lr=0.0, device="cpu", grad_clip_norm=-0.1)
+        t.train_step(dict(X=X), None)
+
+
 # --------------------------------------------------------------------------- #
 # differential attention: ranges of fp16
 # --------------------------------------------------------------------------- #
