@@ -59,6 +59,12 @@ inline void npf_check_plain(const torch::Tensor& t, const char* op) {
       " chooses the composed form");
 }
 
+// Memory holds the values of a negated view (the imaginary part of a conjugate)
+// with the other sign.
+inline torch::Tensor npf_signed(const torch::Tensor& t) {
+  return t.defined() && t.is_neg() ? t.resolve_neg() : t;
+}
+
 // Contiguous memory beside `on`, from the allocator itself: torch::empty's way
 // there through the dispatcher takes longer than a launch (a layer norm with
 // its gradients makes 6 such calls: 67 us of host time, with torch::empty 70).

@@ -124,7 +124,8 @@ Tensor attn_forward(const Tensor& q, const Tensor& k, const Tensor& v,
 }
 
 // along the last axis the kernels take contiguous values alone
-Tensor as_heads(const Tensor& t) {
+Tensor as_heads(const Tensor& t_) {
+  const Tensor t = npf_signed(t_);
   return t.size(-1) == 1 || t.stride(-1) == 1 ? t : t.contiguous();
 }
 
@@ -205,14 +206,15 @@ struct DiffAttn : torch::autograd::Function<DiffAttn> {
 };
 
 Tensor differential_attention(const Tensor& k_, const Tensor& q_,
-                              const Tensor& v_, const Tensor& lam, double scale,
-                              const OptTensor& lengths_) {
+                              const Tensor& v_, const Tensor& lam_,
+                              double scale, const OptTensor& lengths_) {
   npf_check_call(kName);
-  for (const Tensor* t : {&k_, &q_, &v_, &lam}) npf_check_plain(*t, kName);
+  for (const Tensor* t : {&k_, &q_, &v_, &lam_}) npf_check_plain(*t, kName);
   if (lengths_) npf_check_plain(*lengths_, kName);
   const Tensor k = as_heads(k_), q = as_heads(q_), v = as_heads(v_);
+  const Tensor lam = npf_signed(lam_);
   OptTensor lengths;
-  if (lengths_) lengths = lengths_->contiguous();
+  if (lengths_) lengths = npf_signed(*lengths_).contiguous();
   c10::DeviceGuard guard(q.device());
   if (at::GradMode::is_enabled() &&
       (k.requires_grad() || q.requires_grad() || v.requires_grad() ||

@@ -112,7 +112,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     npf_check_plain(grads[0], "layer_norm");
     c10::DeviceGuard guard(x.device());
     NpfLayerNormArgs a = norm_args(x, residual, weight, bias);
-    const Tensor dy = grads[0].contiguous();
+    const Tensor dy = npf_signed(grads[0]).contiguous();
     Tensor dx, dweight, dbias, partial;
     if (needs & 3) dx = npf_empty(dy.sizes(), dy.scalar_type(), dy);
     if (needs & 4)
@@ -143,20 +143,22 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
   }
 };
 
-Tensor layer_norm(const Tensor& x, const OptTensor& residual_,
+Tensor layer_norm(const Tensor& x_, const OptTensor& residual_,
                   const OptTensor& weight_, const OptTensor& bias_,
                   double eps) {
   npf_check_call("layer_norm");
-  npf_check_plain(x, "layer_norm");
+  npf_check_plain(x_, "layer_norm");
   for (const OptTensor* t : {&residual_, &weight_, &bias_})
     if (*t) npf_check_plain(**t, "layer_norm");
+  const Tensor x = npf_signed(x_);
   TORCH_CHECK_VALUE(x.is_cuda() && x.dim() >= 1 && x.size(-1) > 0,
                     "layer_norm takes rows of at least one value on a GPU");
   TORCH_CHECK_VALUE(x.size(-1) <= std::numeric_limits<int>::max() / 2,
                     "layer_norm: rows are too wide");
   npf_type_code(x, "x");
-  const Tensor residual = residual_.value_or(Tensor());
-  Tensor weight = weight_.value_or(Tensor()), bias = bias_.value_or(Tensor());
+  const Tensor residual = npf_signed(residual_.value_or(Tensor()));
+  Tensor weight = npf_signed(weight_.value_or(Tensor()));
+  Tensor bias = npf_signed(bias_.value_or(Tensor()));
   if (residual.defined()) check_like(residual, x, "residual");
   if (weight.defined()) {
     check_columns(weight, x, "weight");
@@ -200,7 +202,7 @@ std::vector<NpfGradSpans> spans_of(const std::vector<Tensor>& grads) {
   for (const Tensor& g : grads) {
     TORCH_CHECK_VALUE(g.is_cuda() && g.device() == grads[0].device(),
                       "all gradients must be on one GPU");
-    TORCH_CHECK_VALUE(g.is_non_overlapping_and_dense(),
+    TORCH_CHECK_VALUE(g.is_non_overlapping_and_dense() && !g.is_neg(),
                       "gradients must be dense in memory");
     const int type = npf_type_code(g, "a gradient", true);
     if (g.numel() == 0) continue;

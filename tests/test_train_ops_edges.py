@@ -12,8 +12,8 @@ import torch
 
 from npf import ops
 from test_train_ops import (E32, SHAPES, assert_within, attn_inputs, attn_oracle,
-                            check_attn, check_clip, lowest_step, params_of,
-                            run_attn)
+                            check_attn, check_clip, lowest_step, norm_inputs,
+                            params_of, run_attn, run_norm)
 
 HALF = [torch.bfloat16, torch.float16]
 
@@ -482,3 +482,55 @@ class TestRowsWithoutKeys:
         for n in ("out", "dq", "dk", "dv"):
             assert torch.equal(got[n][1], torch.zeros_like(got[n][1])), n
         assert got["out"][0].isnan().all() or got["out"][0].isinf().any()
+
+
+class TestNegatedViews:
+    """Views whose memory holds the other sign (the imaginary part of a
+    conjugate is one)."""
+
+    @pytest.mark.gpu
+    def test_attention(self):
+        a = {n: t.cuda() for n, t in
+             attn_inputs(2, 2, 1, 5, 9, 4, 1, torch.float32).items()}
+        want = run_attn("cuda", a)
+
+        def call(t):
+            t = {n: x.detach().requires_grad_(True) for n, x in t.items()}
+            out = ops.differential_attention(t["keys"], t["queries"], t["values"], t["lam"])
+            names = ("keys", "queries", "values", "lam")
+            grads = torch.autograd.grad(out, [t[n] for n in names], t["dout"].detach())
+            return dict(zip(("dk", "dq", "dv", "dlam"), grads), out=out)
+
+        for n in a:
+            negated = torch._neg_view(-a[n])
+            assert negated.is_neg()
+            got = call(dict(a, **{n: negated}))
+            for r in want:
+                assert torch.equal(got[r], want[r]), (n, r)
+        for n in ("values", "lam"):
+            z = torch.complex(a[n], -a[n]).conj().imag
+            assert z.is_neg() and torch.equal(z, a[n])
+            got = call(dict(a, **{n: z}))
+            for r in want:
+                assert torch.equal(got[r], want[r]), (n, r)
+
+    @pytest.mark.gpu
+    def test_norm(self):
+        args = [t.cuda() for t in norm_inputs(6, 20, torch.float32, torch.float32, True)]
+        want = run_norm("cuda", *args)
+        for i in range(5):
+            some = list(args)
+            some[i] = torch._neg_view(-args[i])
+            leaves = [t.detach().requires_grad_(True) for t in some[:4]]
+            y = ops.layer_norm(leaves[0], leaves[2], leaves[3], residual=leaves[1])
+            got = dict(zip(("dx", "dr", "dw", "db"),
+                           torch.autograd.grad(y, leaves, some[4])), y=y)
+            for r in want:
+                assert torch.equal(got[r], want[r]), (i, r)
+
+    @pytest.mark.gpu
+    def test_gradients(self):
+        p = torch.zeros(50, device="cuda", requires_grad=True)
+        p.grad = torch._neg_view(torch.ones(50, device="cuda"))
+        with pytest.raises(ValueError, match="dense"):
+            ops.clip_grad_norm_([p], 1.0)
