@@ -893,6 +893,14 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, residual=None):
 
 
 def _differential_attention_ref(keys, queries, values, lam, scale, key_lengths):
+    # (autocast would round fp32 inputs of the products to 16 bits)
+    with torch.autocast(queries.device.type, enabled=False):
+        return _differential_attention_wide(
+            keys, queries, values, lam, scale, key_lengths
+        )
+
+
+def _differential_attention_wide(keys, queries, values, lam, scale, key_lengths):
     dtype = queries.dtype
     keys, queries, values = _widened(keys), _widened(queries), _widened(values)
     H, K, Hk = queries.shape[1], keys.shape[2], keys.shape[1]
@@ -945,8 +953,8 @@ def differential_attention(keys, queries, values, lam, scale=None, key_lengths=N
     inputs' type for the products with V, and their gradients for those with
     the keys and queries (in fp16 after a scaling by a power of two, so that
     they neither pass the type's largest value nor fall below its smallest).
-    Differentiable once in keys, queries, values and lam, with sums in a fixed
-    order.  On a GPU forward-mode derivatives, traces and tensors that wrap
+    Under autocast the inputs' own types count.  Differentiable once in keys,
+    queries, values and lam, with sums in a fixed order.  On a GPU forward-mode derivatives, traces and tensors that wrap
     others raise NotImplementedError.
     """
     if keys.dim() != 4 or queries.dim() != 4 or values.dim() != 4:

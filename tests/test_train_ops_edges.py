@@ -534,3 +534,14 @@ class TestNegatedViews:
         p.grad = torch._neg_view(torch.ones(50, device="cuda"))
         with pytest.raises(ValueError, match="dense"):
             ops.clip_grad_norm_([p], 1.0)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("disabled", ["", "differential_attention"])
+def test_attention_under_autocast_keeps_its_types(device, disabled, monkeypatch):
+    monkeypatch.setenv("NPF_DISABLE_OPS", disabled)
+    a = attn_inputs(2, 2, 1, 5, 50, 8, 16, torch.float32)
+    with torch.autocast(device, dtype=torch.bfloat16):
+        got = run_attn(device, a)
+    assert got["out"].dtype == torch.float32
+    check_attn(got, attn_oracle(a))
