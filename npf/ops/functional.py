@@ -954,8 +954,8 @@ def differential_attention(keys, queries, values, lam, scale=None, key_lengths=N
     the keys and queries (in fp16 after a scaling by a power of two, so that
     they neither pass the type's largest value nor fall below its smallest).
     Under autocast the inputs' own types count.  Differentiable once in keys,
-    queries, values and lam, with sums in a fixed order.  On a GPU forward-mode derivatives, traces and tensors that wrap
-    others raise NotImplementedError.
+    queries, values and lam, with sums in a fixed order.  On a GPU forward-mode
+    derivatives, traces and tensors that wrap others raise NotImplementedError.
     """
     if keys.dim() != 4 or queries.dim() != 4 or values.dim() != 4:
         raise ValueError("keys, queries and values must be [batch, heads, length, size]")

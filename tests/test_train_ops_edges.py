@@ -541,7 +541,10 @@ class TestNegatedViews:
 def test_attention_under_autocast_keeps_its_types(device, disabled, monkeypatch):
     monkeypatch.setenv("NPF_DISABLE_OPS", disabled)
     a = attn_inputs(2, 2, 1, 5, 50, 8, 16, torch.float32)
+    t = {n: x.to(device).requires_grad_(n != "dout") for n, x in a.items()}
     with torch.autocast(device, dtype=torch.bfloat16):
-        got = run_attn(device, a)
-    assert got["out"].dtype == torch.float32
-    check_attn(got, attn_oracle(a))
+        out = ops.differential_attention(t["keys"], t["queries"], t["values"], t["lam"])
+    assert out.dtype == torch.float32
+    names = ("keys", "queries", "values", "lam")
+    grads = torch.autograd.grad(out, [t[n] for n in names], t["dout"])
+    check_attn(dict(zip(("dk", "dq", "dv", "dlam"), grads), out=out), attn_oracle(a))
