@@ -548,3 +548,93 @@ def test_attention_under_autocast_keeps_its_types(device, disabled, monkeypatch)
     names = ("keys", "queries", "values", "lam")
     grads = torch.autograd.grad(out, [t[n] for n in names], t["dout"])
     check_attn(dict(zip(("dk", "dq", "dv", "dlam"), grads), out=out), attn_oracle(a))
+
+
+# --------------------------------------------------------------------------- #
+# launches that ordinary training steps do not make
+# --------------------------------------------------------------------------- #
+
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+class TestOtherLaunches:
+    @pytest.mark.gpu
+    @pytest.mark.parametrize("dtype", TYPES)
+    @pytest.mark.parametrize("D, Dv", [(4, 7), (64, 64), (64, 100), (128, 256), (20, 30)])
+    @pytest.mark.parametrize("lengths", [None, [37, 0]])
+    def test_gradients_of_keys_and_values_alone(self, dtype, D, Dv, lengths):
+        # rows' sums without the kernel of dq; dk and dv each by itself
+        a = attn_inputs(2, 4, 2, 45, 70, D, Dv, dtype)
+        want = attn_oracle(a, lengths=lengths)
+        lens = None if lengths is None else torch.tensor(lengths, device="cuda")
+        for names in (("dk",), ("dv",), ("dk", "dv")):
+            t = {n: x.cuda() for n, x in a.items()}
+            leaves = [t[{"dk": "keys", "dv": "values"}[n]].requires_grad_(True) for n in names]
+            out = ops.differential_attention(
+                t["keys"], t["queries"], t["values"], t["lam"], key_lengths=lens)
+            check_attn(dict(zip(names, torch.autograd.grad(out, leaves, t["dout"]))), want)
+
+    @pytest.mark.gpu
+    @pytest.mark.parametrize("dtype", TYPES)
+    @pytest.mark.parametrize("sizes", [
+        (2, 2, 1, 700, 129, 16, 32), (2, 2, 1, 700, 600, 16, 32), (2, 1, 1, 600, 300, 64, 128),
+        (2, 2, 2, 530, 140, 128, 200), (2, 4, 1, 150, 90, 20, 40),
+    ])
+    def test_lengths_and_queries_in_parts(self, dtype, sizes):
+        # (a key head has at least 512 rows of queries: their axis is split)
+        a = attn_inputs(*sizes, dtype)
+        for lengths in ([0, sizes[4]], [sizes[4] - 1, 33]):
+            check_attn(run_attn("cuda", a, lengths=lengths), attn_oracle(a, lengths=lengths))
+
+    @pytest.mark.gpu
+    @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+    def test_one_weight_for_many_rows(self, dtype):
+        a = attn_inputs(3, 4, 2, 1100, 40, 8, 16, dtype, lam_each=False)
+        check_attn(run_attn("cuda", a), attn_oracle(a))
+        # the key axis in parts, each with its own sums
+        a = attn_inputs(1, 4, 2, 200, 1200, 8, 16, dtype, lam_each=False)
+        check_attn(run_attn("cuda", a), attn_oracle(a))
+
+
+class TestNotFinite:
+    """Keys and values that count and are not finite."""
+
+    SIZES = [(1, 2, 1, 70, 150, 16, 32), (1, 2, 1, 3, 700, 16, 32),
+             (1, 2, 2, 40, 90, 128, 256), (1, 1, 1, 300, 600, 20, 40)]
+
+    @pytest.mark.gpu
+    @pytest.mark.parametrize("dtype", TYPES)
+    @pytest.mark.parametrize("sizes", SIZES)
+    @pytest.mark.parametrize("place", ["first", "last"])
+    def test_infinite_scores(self, dtype, sizes, place):
+        # one key with -inf in both maps: rows of positive queries give it the
+        # weight 0, as if it were not there; scores of the others are +inf
+        D, at = sizes[5], 0 if place == "first" else sizes[4] - 1
+        a = attn_inputs(*sizes, dtype)
+        for c in (0, D):
+            a["queries"][..., c] = a["queries"][..., c].abs() + 0.25
+            a["queries"][:, :, 1::2, c] *= -1.0
+        rest = [i for i in range(sizes[4]) if i != at]
+        b = dict(a, keys=a["keys"][:, :, rest], values=a["values"][:, :, rest])
+        want, bound = attn_oracle(b)["out"]
+        a["keys"][:, :, at, 0] = a["keys"][:, :, at, D] = -math.inf
+        got = run_attn("cuda", a)["out"]
+        assert_within(got[:, :, ::2], want[:, :, ::2], bound[:, :, ::2], "out")
+        assert got[:, :, 1::2].isnan().all()
+
+    @pytest.mark.gpu
+    @pytest.mark.parametrize("dtype", TYPES)
+    @pytest.mark.parametrize("sizes", SIZES)
+    def test_not_a_number(self, dtype, sizes):
+        a = attn_inputs(*sizes, dtype)
+        want, bound = attn_oracle(a)["out"]
+        bad = dict(a, keys=a["keys"].clone())
+        bad["keys"][0, 0, 33, 1] = math.nan
+        got = run_attn("cuda", bad)["out"]
+        assert got[0, 0].isnan().all()  # (a head of that key head's group)
+        bad = dict(a, values=a["values"].clone())
+        bad["values"][0, 0, 33, 3] = math.nan
+        got = run_attn("cuda", bad)["out"]
+        assert got[0, 0, :, 3].isnan().all()
+        rest = [i for i in range(sizes[6]) if i != 3]
+        assert_within(got[..., rest], want[..., rest], bound[..., rest], "out")
