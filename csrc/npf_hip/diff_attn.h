@@ -45,6 +45,8 @@ constexpr int kReachRows = 64;
 
 // fills the plan; false where no kernel covers the sizes
 bool npf_diff_attn_plan(NpfDiffAttnArgs&);
+// whether each launch of a pass has fewer than 2^32 threads, as HIP asks
+bool npf_diff_attn_fits(const NpfDiffAttnArgs&, bool backward);
 // floats of `split`
 long npf_diff_attn_workspace(const NpfDiffAttnArgs&);
 hipError_t npf_diff_attn_fwd(const NpfDiffAttnArgs&, hipStream_t);

@@ -386,6 +386,22 @@ bool npf_diff_attn_plan(NpfDiffAttnArgs& a) {
   return true;
 }
 
+bool npf_diff_attn_fits(const NpfDiffAttnArgs& a, bool backward) {
+  const long rows = (long)(a.H / a.Hk) * a.Q, heads = (long)a.B * a.Hk;
+  const long tiles = heads * ((rows + 127) / 128);
+  auto fits = [](long blocks, long threads) {
+    return blocks <= 0xffffffffL / threads;
+  };
+  // (joins are of few rows: parts are planned where blocks are few)
+  if (!backward)
+    return a.waves == 1 ? fits(heads * a.splits * ((rows + 31) / 32), 128)
+                        : fits(tiles * a.splits, 512);
+  return fits(tiles * a.dq_splits, 256) &&
+         fits(heads * ((a.K + 127) / 128) * a.dkv_splits, 256) &&
+         fits(heads * ((long)a.v_chunks + a.o_chunks), 256) &&
+         fits(heads * rows, 64);  // the sums of rows, of 64 lanes at most
+}
+
 long npf_diff_attn_workspace(const NpfDiffAttnArgs& a) {
   if (a.splits <= 1) return 0;
   return split_row_floats(a.Dv) * a.splits * a.B * a.H * a.Q;

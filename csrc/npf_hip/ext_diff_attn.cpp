@@ -104,6 +104,11 @@ Tensor attn_forward(const Tensor& q, const Tensor& k, const Tensor& v,
                     const Tensor& lam, double scale, const Tensor& lengths,
                     bool save, Tensor* o2, Tensor* lse) {
   NpfDiffAttnArgs a = common_args(q, k, v, lam, scale, lengths);
+  // (what the backward pass would refuse is refused here)
+  TORCH_CHECK_VALUE(npf_diff_attn_fits(a, false) &&
+                        (!save || npf_diff_attn_fits(a, true)),
+                    "differential_attention: too many heads and rows for a "
+                    "launch");
   Tensor out = heads_like(q, a.B, a.H, a.Q, a.Dv);
   a.out = heads_of(out);
   if (save) {

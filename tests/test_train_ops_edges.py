@@ -596,6 +596,38 @@ class TestOtherLaunches:
         check_attn(run_attn("cuda", a), attn_oracle(a))
 
 
+class TestMostHeads:
+    """Launches end at 2^32 threads, of which each head takes a block of its own."""
+
+    def heads(self, n, Q, dtype=torch.bfloat16):
+        row = torch.full((1, 1, 1, 2), 0.5, dtype=dtype, device="cuda")
+        return row.expand(1, n, 1, 2), row.expand(1, n, Q, 2)
+
+    @pytest.mark.gpu
+    def test_refusals(self):
+        lam = torch.tensor(0.25, device="cuda")
+        for n, Q in ((2 ** 25 + 8, 1), (2 ** 23 + 8, 33)):
+            k, q = self.heads(n, Q)
+            with pytest.raises(ValueError, match="too many heads"):
+                ops.differential_attention(k, q, k, lam)
+        k, q = self.heads(2 ** 24 + 8, 1)
+        lam.requires_grad_(True)
+        with pytest.raises(ValueError, match="too many heads"):
+            ops.differential_attention(k, q, k, lam)
+
+    @pytest.mark.gpu
+    def test_most(self):
+        lam = torch.tensor(0.25, device="cuda", requires_grad=True)
+        for dtype in (torch.bfloat16, torch.float16):
+            k, q = self.heads(2 ** 22 + 3, 2, dtype)
+            out = ops.differential_attention(k, q, k, lam)
+            # one key: both maps are 1
+            assert torch.equal(out, torch.full_like(out, 0.375))
+            (dlam,) = torch.autograd.grad(out, lam, torch.ones_like(out))
+            # -0.5 for each of 4 (2^22 + 3) values, in 64 bits and rounded
+            assert dlam.item() == -2.0 * (2 ** 22 + 3)
+
+
 class TestNotFinite:
     """Keys and values that count and are not finite."""
 
