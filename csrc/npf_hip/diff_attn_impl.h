@@ -59,12 +59,17 @@ struct Shape {
 };
 
 // Waves a SIMD is to hold: two, in half of the registers each and with every
-// matrix result in ordinary registers, where a kernel fits; else one.  (Long
-// training bf16, dk and dv in one launch that spills: 4349 us; apart, 988.)
-// Kernels of one map fit at twice the size.
-template <typename T, int kPad, bool kOneMap = false>
+// matrix result in ordinary registers, up to 128 bytes of a map; else one.
+// Kernels of one map go to twice the size in 16 bits, where the next rows do
+// not pass through registers (kDirect).  (Long training bf16, dk and dv in one
+// launch that spills: 4349 us; apart, 958.  Steps of 2 x 8 heads, 1024 x 1024,
+// rows through registers, two waves and one: bf16 heads of 60 230 and 300 us,
+// though dk and dv then spill 27 to 32 registers, heads of 20 107 and 107, fp32
+// heads of 18 277 and 332; kernels of one map at bf16 heads of 100 547 and 495.)
+template <typename T, int kPad, bool kDirect, bool kOneMap = false>
 constexpr int kResident =
-    kPad * (int)sizeof(T) <= (kOneMap && sizeof(T) == 2 ? 256 : 128) ? 2 : 1;
+    kPad * (int)sizeof(T) <= (kOneMap && kDirect && sizeof(T) == 2 ? 256 : 128)
+        ? 2 : 1;
 
 // The same of the forward kernel, whose waves hold one map; rows on their way
 // through registers (not kDirect) need room too.  (Long: 430 us; waves with
@@ -373,7 +378,7 @@ constexpr int kBwdWaves = 4;  // of a backward block
 // dq of the maps in kMaps (bits), and with the second map each row's part of
 // dlam: a wave holds 32 query rows and passes over the keys
 template <typename T, int kPad, bool kDirect, int kMaps>
-__global__ void __launch_bounds__(64 * kBwdWaves, (kResident<T, kPad>))
+__global__ void __launch_bounds__(64 * kBwdWaves, (kResident<T, kPad, kDirect>))
     diff_bwd_dq(NpfDiffAttnArgs a) {
   using S = Shape<T, kPad>;
   using Lds = Tile<T, S::kWidth>;
@@ -612,7 +617,7 @@ __global__ void __launch_bounds__(64 * kBwdWaves, (kResident<T, kPad>))
 // passes over the queries of the heads that share them
 template <typename T, int kPad, bool kDirect, int kMaps, bool kDv>
 __global__ void __launch_bounds__(64 * kBwdWaves,
-                                  (kResident<T, kPad, !kDv && kMaps != 3>))
+                                  (kResident<T, kPad, kDirect, !kDv && kMaps != 3>))
     diff_bwd_dkv(NpfDiffAttnArgs a) {
   using S = Shape<T, kPad>;
   using Lds = Tile<T, S::kWidth>;
