@@ -138,6 +138,13 @@ __global__ void __launch_bounds__(128 * kRowWaves,
   // tiles of 32 that a wave takes through a pass at once: what fits a quarter
   // of a SIMD's registers (8 heads of 32, 4096^2, bf16: 93 us, with two 110)
   constexpr int kSubs = kPad <= 16 ? 2 : 1;
+  // With few rows memory bounds the kernel, and the maps keep what rounding to
+  // 16 bits leaves of them (single queries against 32768 keys: 57 to 60 us, and
+  // the result's error falls from 1.48 to 1.0 times that of its last rounding).
+  // With many rows it would cost more than it gives: a step 117 -> 130 us
+  // (image), 1740 -> 2020 (long), padded fp16, 7 x 8 heads of 48, 333 x 2049, 53
+  // -> 81; errors there are 1.4 to 1.5 times the last rounding's.
+  constexpr bool kTwice = sizeof(T) == 2 && kRowWaves == 1;
   constexpr int kTileBytes = kTile * S::kRowBytes;
   // two objects, so that it shows that the next tiles' loads do not touch
   // what is being read
@@ -254,16 +261,14 @@ __global__ void __launch_bounds__(128 * kRowWaves,
 #pragma unroll
       for (int t = 0; t < kSubs; ++t) {
         l = exp_tile(s[t], c, mx, l);
-        const Operand<T> p[1] = {Operand<T>(s[t])};
+        const Product<T, S::kWidth, kTwice> p(s[t]);
 #pragma unroll
         for (int part = 0; part < S::kParts; ++part) {
           if (!S::taken(part, 2 * kPad, a.Dv)) continue;
 #pragma unroll
           for (int j = S::from(S::kBlocks, part);
-               j < S::upto(S::kBlocks, part); ++j) {
-            f32x16* const acc[1] = {&o[j]};
-            Lds::template transposed<1>(vt, cb, sub0 + 32 * t, 32 * j, p, acc);
-          }
+               j < S::upto(S::kBlocks, part); ++j)
+            p.add(vt, cb, sub0 + 32 * t, 32 * j, o[j]);
         }
       }
     }
@@ -386,6 +391,13 @@ __global__ void __launch_bounds__(64 * kBwdWaves, (kResident<T, kPad, kDirect>))
   constexpr bool kInLds = S::kQueriesInLds;
   constexpr int kTile = kInLds ? 32 * S::kSubs : S::kTile;
   constexpr int kSubs = S::kSubs;
+  // For heads of up to 32 the maps' gradients keep what rounding to 16 bits
+  // leaves of them.  Rows of them sum to zero, so what the keys of a row share
+  // (scale q_i, more of it the fewer values a head has) cancels in dq but not in
+  // the rounding: rounded once, dq's error is 1.53 times that of its own last
+  // rounding at heads of 16 (now 1.07; a step 130 us rather than 117, image) and
+  // 1.44 times at heads of 64 (1.02; 1855 us rather than 1740, long).
+  constexpr bool kTwice = sizeof(T) == 2 && kPad <= 32;
   constexpr int kTileBytes = kTile * S::kRowBytes;
   // two objects, so that it shows that the next tiles' loads do not touch
   // what is being read
@@ -543,17 +555,14 @@ __global__ void __launch_bounds__(64 * kBwdWaves, (kResident<T, kPad, kDirect>))
             s[t][i] = p * (m ? g[t][i] + apart : g[t][i]);
             if (m) dlam += s[t][i];
           }
-          const Operand<T> ds[1] = {Operand<T>(s[t])};
+          const Product<T, S::kWidth, kTwice> ds(s[t]);
 #pragma unroll
           for (int part = 0; part < S::kParts; ++part) {
             if (!S::taken(part, kPad, a.D)) continue;
 #pragma unroll
             for (int j = S::from(S::kMapBlocks, part);
-                 j < S::upto(S::kMapBlocks, part); ++j) {
-              f32x16* const acc[1] = {&dq[m][j]};
-              Lds::template transposed<1>(kt, cb, sub0 + 32 * t,
-                                          map_col<kPad>(m, j), ds, acc);
-            }
+                 j < S::upto(S::kMapBlocks, part); ++j)
+              ds.add(kt, cb, sub0 + 32 * t, map_col<kPad>(m, j), dq[m][j]);
           }
         }
         if (kSubs == 1) __builtin_amdgcn_sched_barrier(0);

@@ -78,15 +78,25 @@ __device__ __forceinline__ f32x16 mma_chunk(u32x4 a, u32x4 b, f32x16 c) {
 }
 
 // A 32x32 tile of map values or of their gradients as an operand.  In 16 bits
-// its values are rounded here, once; statistics have seen them in 32.
+// its values are rounded here; statistics have seen them in 32.
 template <typename T>
 struct Operand {
-  typename Vec8<T>::type v[2];
+  using V = typename Vec8<T>::type;
+  V v[2];
   __device__ __forceinline__ explicit Operand(const f32x16& x) {
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[t][e] = (T)x[8 * t + e];
+  }
+  // what the rounding of x has left (exact in 32 bits), to be rounded in turn
+  __device__ __forceinline__ f32x16 rest(f32x16 x) const {
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        x[8 * t + e] = __builtin_fmaf((float)v[t][e], -1.f, x[8 * t + e]);
+    return x;
   }
 };
 template <>
@@ -180,6 +190,38 @@ struct Tile {
         for (int m = 0; m < kMaps; ++m) *acc[m] = mma(v, p[m].v[i], *acc[m]);
       }
     }
+  }
+};
+
+// acc += tile^T x as Tile::transposed; kTwice: x is taken as the sum of its
+// rounded values and of what rounding left, for 16 bits and more of each
+template <typename T, int kWidth, bool kTwice>
+struct Product {
+  static constexpr int kParts = kTwice ? 2 : 1;
+  Operand<T> p[kParts];
+  __device__ __forceinline__ explicit Product(const f32x16& x)
+      : Product(Operand<T>(x), x) {}
+  __device__ __forceinline__ void add(const char* tile, int base, int row0,
+                                      int col0, f32x16& acc) const {
+    f32x16* at[kParts];
+#pragma unroll
+    for (int i = 0; i < kParts; ++i) at[i] = &acc;
+    Tile<T, kWidth>::template transposed<kParts>(tile, base, row0, col0, p, at);
+  }
+
+ private:
+  __device__ __forceinline__ Product(const Operand<T>& high, const f32x16& x)
+      : p{high, Operand<T>(high.rest(x))} {}
+};
+template <typename T, int kWidth>
+struct Product<T, kWidth, false> {
+  Operand<T> p[1];
+  __device__ __forceinline__ explicit Product(const f32x16& x)
+      : p{Operand<T>(x)} {}
+  __device__ __forceinline__ void add(const char* tile, int base, int row0,
+                                      int col0, f32x16& acc) const {
+    f32x16* const at[1] = {&acc};
+    Tile<T, kWidth>::template transposed<1>(tile, base, row0, col0, p, at);
   }
 };
 
