@@ -60,9 +60,12 @@ inline void npf_check_plain(const torch::Tensor& t, const char* op) {
 }
 
 // Memory holds the values of a negated view (the imaginary part of a conjugate)
-// with the other sign.
+// with the other sign, and there is none of a gradient that torch knows to be
+// zero.
 inline torch::Tensor npf_signed(const torch::Tensor& t) {
-  return t.defined() && t.is_neg() ? t.resolve_neg() : t;
+  if (!t.defined()) return t;
+  if (t._is_zerotensor()) return torch::zeros(t.sizes(), t.options());
+  return t.is_neg() ? t.resolve_neg() : t;
 }
 
 // Contiguous memory beside `on`, from the allocator itself: torch::empty's way

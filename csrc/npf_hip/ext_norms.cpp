@@ -202,7 +202,8 @@ std::vector<NpfGradSpans> spans_of(const std::vector<Tensor>& grads) {
   for (const Tensor& g : grads) {
     TORCH_CHECK_VALUE(g.is_cuda() && g.device() == grads[0].device(),
                       "all gradients must be on one GPU");
-    TORCH_CHECK_VALUE(g.is_non_overlapping_and_dense() && !g.is_neg(),
+    TORCH_CHECK_VALUE(g.is_non_overlapping_and_dense() && !g.is_neg() &&
+                          !g._is_zerotensor(),
                       "gradients must be dense in memory");
     const int type = npf_type_code(g, "a gradient", true);
     if (g.numel() == 0) continue;

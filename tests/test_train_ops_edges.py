@@ -529,6 +529,27 @@ class TestNegatedViews:
                 assert torch.equal(got[r], want[r]), (i, r)
 
     @pytest.mark.gpu
+    def test_zeros_without_memory(self):
+        # as torch makes them for gradients that are known to be zero
+        zero = lambda *shape: torch._efficientzerotensor(shape, device="cuda")
+        x = torch.randn(4, 8, device="cuda", requires_grad=True)
+        assert torch.equal(ops.layer_norm(zero(4, 8)), torch.zeros(4, 8, device="cuda"))
+        y = ops.layer_norm(x)
+        (dx,) = torch.autograd.grad(y, x, zero(4, 8))
+        assert torch.equal(dx, torch.zeros_like(dx))
+        q = torch.randn(1, 1, 3, 8, device="cuda", requires_grad=True)
+        lam = torch.tensor(0.25, device="cuda")
+        out = ops.differential_attention(q, q, zero(1, 1, 3, 4), lam)
+        assert torch.equal(out, torch.zeros_like(out))
+        out = ops.differential_attention(q, q, q, lam)
+        (dq,) = torch.autograd.grad(out, q, zero(1, 1, 3, 8))
+        assert torch.equal(dq, torch.zeros_like(dq))
+        p = torch.zeros(50, device="cuda", requires_grad=True)
+        p.grad = zero(50)
+        with pytest.raises(ValueError, match="dense"):
+            ops.clip_grad_norm_([p], 1.0)
+
+    @pytest.mark.gpu
     def test_gradients(self):
         p = torch.zeros(50, device="cuda", requires_grad=True)
         p.grad = torch._neg_view(torch.ones(50, device="cuda"))
