@@ -23,7 +23,7 @@ struct NpfDiffAttnArgs {
   float* dq_part;         // backward: parts of a split sum, [dq_splits, B, H,
   float* dk_part;         // Q, 2D] and [dkv_splits, B, Hk, K, 2D or Dv], where
   float* dv_part;         // there are several
-  float* reach;           // backward, fp16: [v_chunks + o_chunks, B * Hk], the
+  float* reach;           // backward, fp16: [B * Hk, v_chunks + o_chunks], the
                           // largest norms of rows of values and of dout
   float scale;
   int B, H, Hk, Q, K, D, Dv;
@@ -37,8 +37,10 @@ struct NpfDiffAttnArgs {
   int splits;  // parts of the key axis, forward
   int dq_splits;   // parts of the key axis, and of the query axis, backward
   int dkv_splits;
-  int v_chunks;    // of kReachRows rows of values, and of dout of a key head's
-  int o_chunks;    // queries; 0 where `reach` is not wanted
+  int v_chunks;    // of a key head's rows of values, and of its queries' rows
+  int o_chunks;    // of dout; 0 where `reach` is not wanted
+  int v_rows;      // of a chunk, whole steps of kReachRows
+  int o_rows;
 };
 
 constexpr int kReachRows = 64;

@@ -212,47 +212,51 @@ __global__ void __launch_bounds__(256) row_reach(NpfDiffAttnArgs a) {
   const int chunk = blockIdx.x / heads, b = bh / a.Hk, hk = bh % a.Hk;
   const int group = a.H / a.Hk, n = keys_of(a, b);
   const bool of_values = chunk < a.v_chunks;
-  const int row0 = (of_values ? chunk : chunk - a.v_chunks) * kReachRows;
-  const int rows = of_values ? n : n > 0 ? group * a.Q : 0;
+  const int step = of_values ? a.v_rows : a.o_rows;
+  const int row0 = (of_values ? chunk : chunk - a.v_chunks) * step;
+  int rows = of_values ? n : n > 0 ? group * a.Q : 0;
+  rows = rows - row0 < step ? rows : row0 + step;
   const int c = (threadIdx.x % kLanes) * 4;
   const int count = a.Dv - c < 4 ? a.Dv - c : 4;
-  // every row's loads before the first sum: one wait for memory, not one a row
   constexpr int kEach = kReachRows * kLanes / 256;
-  T v[kEach][4] = {};
-  float weight[kEach];
-#pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    const int row = row0 + i * (256 / kLanes) + threadIdx.x / kLanes;
-    weight[i] = 1.f;
-    if (row >= rows) continue;
-    const int h = of_values ? hk : hk * group + row / a.Q;
-    const T* p = (of_values ? row_of<T>(a.v, b, h, row)
-                            : row_of<T>(a.dout, b, h, row % a.Q)) + c;
-    if (!of_values) weight[i] = fmaxf(1.f, fabsf(lam_of(a, h)));
-    if (count == 4) {
-      load_pack(v[i], p);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (e < count) v[i][e] = p[e];
-    }
-  }
   float most = 0.f;
+  for (int at = row0; at < rows; at += kReachRows) {
+    // every row's loads before the first sum: one wait for memory, not one a row
+    T v[kEach][4] = {};
+    float weight[kEach];
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    float s = 0.f;
+    for (int i = 0; i < kEach; ++i) {
+      const int row = at + i * (256 / kLanes) + threadIdx.x / kLanes;
+      weight[i] = 1.f;
+      if (row >= rows) continue;
+      const int h = of_values ? hk : hk * group + row / a.Q;
+      const T* p = (of_values ? row_of<T>(a.v, b, h, row)
+                              : row_of<T>(a.dout, b, h, row % a.Q)) + c;
+      if (!of_values) weight[i] = fmaxf(1.f, fabsf(lam_of(a, h)));
+      if (count == 4) {
+        load_pack(v[i], p);
+      } else {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) s += (float)v[i][e] * (float)v[i][e];
+        for (int e = 0; e < 4; ++e)
+          if (e < count) v[i][e] = p[e];
+      }
+    }
 #pragma unroll
-    for (int off = kLanes / 2; off > 0; off >>= 1)
-      s += __shfl_xor(s, off, 64);
-    most = fmaxf(most, sqrtf(s) * weight[i]);
+    for (int i = 0; i < kEach; ++i) {
+      float s = 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s += (float)v[i][e] * (float)v[i][e];
+#pragma unroll
+      for (int off = kLanes / 2; off > 0; off >>= 1)
+        s += __shfl_xor(s, off, 64);
+      most = fmaxf(most, sqrtf(s) * weight[i]);
+    }
   }
   most = wave_allreduce_max(most);
   if ((threadIdx.x & 63) == 0) smem[threadIdx.x >> 6] = most;
   __syncthreads();
   if (threadIdx.x == 0)
-    a.reach[(long)chunk * heads + bh] =
+    a.reach[(long)bh * (a.v_chunks + a.o_chunks) + chunk] =
         fmaxf(fmaxf(smem[0], smem[1]), fmaxf(smem[2], smem[3]));
 }
 
@@ -380,8 +384,16 @@ bool npf_diff_attn_plan(NpfDiffAttnArgs& a) {
   a.dkv_splits =
       parts_for(heads * ((a.K + 127) / 128), wanted, (int)rows, 256);
   if (a.type == NPF_F16) {
-    a.v_chunks = (a.K + kReachRows - 1) / kReachRows;
-    a.o_chunks = (int)((rows + kReachRows - 1) / kReachRows);
+    // no more than 1024 chunks, as every block reads them all (2 heads of 64, 4 x
+    // 1000000, a step: with up to 256 chunks 1731 us, 1024 1508, 15625 1966; the
+    // same in bf16, which needs none, 1308)
+    auto chunks = [](int n, int* each) {
+      const int steps = (n + kReachRows - 1) / kReachRows;
+      *each = (steps + 1023) / 1024 * kReachRows;
+      return *each ? (n + *each - 1) / *each : 0;
+    };
+    a.v_chunks = chunks(a.K, &a.v_rows);
+    a.o_chunks = chunks((int)rows, &a.o_rows);
   }
   return true;
 }

@@ -473,7 +473,7 @@ __global__ void __launch_bounds__(64 * kBwdWaves, (kResident<T, kPad, kDirect>))
   if constexpr (kScaledGrads<T>)
     e = reach_exponent(
         reach_bound(sqrtf(both_sum(square)) * fmaxf(1.f, fabsf(lam)),
-                    reach_of(a, 0, a.v_chunks, bh)));
+                    reach_of_values(a, bh)));
   const float back = kScaledGrads<T> ? __builtin_amdgcn_exp2f(-e) : 1.f;
   if (live) {
     st.x = a.lse[2 * stat];
@@ -689,8 +689,8 @@ __global__ void __launch_bounds__(64 * kBwdWaves,
         most = fmaxf(most, fabsf(lam_of(a, hk * group + i)));
       ea = reach_exponent(1.f + wave_allreduce_max(most));
     }
-    e = kDk ? reach_exponent(reach_bound(reach_of(a, a.v_chunks, a.o_chunks, bh),
-                                         reach_of(a, 0, a.v_chunks, bh)))
+    e = kDk ? reach_exponent(
+                  reach_bound(reach_of_dout(a, bh), reach_of_values(a, bh)))
             : ea;
   }
   auto power = [](float x) {

@@ -455,13 +455,21 @@ __device__ __forceinline__ float reach_exponent(float bound) {
   const int e = 15 - __builtin_amdgcn_frexp_expf(bound);
   return (float)(e < -60 ? -60 : e > 60 ? 60 : e);
 }
-// the largest of a head's chunks from `first` on, in every lane of a wave
-__device__ __forceinline__ float reach_of(const NpfDiffAttnArgs& a, int first,
-                                          int chunks, int bh) {
+// the largest of `chunks` of a head's chunks, in every lane of a wave
+__device__ __forceinline__ float reach_of(const float* reach, int chunks) {
   float x = 0.f;
-  for (int i = threadIdx.x & 63; i < chunks; i += 64)
-    x = fmaxf(x, a.reach[(long)(first + i) * a.B * a.Hk + bh]);
+#pragma unroll 4
+  for (int i = threadIdx.x & 63; i < chunks; i += 64) x = fmaxf(x, reach[i]);
   return wave_allreduce_max(x);
+}
+__device__ __forceinline__ float reach_of_values(const NpfDiffAttnArgs& a,
+                                                 int bh) {
+  return reach_of(a.reach + (long)bh * (a.v_chunks + a.o_chunks), a.v_chunks);
+}
+__device__ __forceinline__ float reach_of_dout(const NpfDiffAttnArgs& a,
+                                               int bh) {
+  return reach_of(
+      a.reach + (long)bh * (a.v_chunks + a.o_chunks) + a.v_chunks, a.o_chunks);
 }
 
 // x of the other lane half, for a reduction over both

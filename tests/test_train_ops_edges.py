@@ -18,34 +18,39 @@ from test_train_ops import (E32, SHAPES, assert_within, attn_inputs, attn_oracle
 HALF = [torch.bfloat16, torch.float16]
 
 
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
 class TestComposedClip:
     """The composed form, whose sums and factor are held in more bits than
     16-bit gradients, like the kernels'."""
 
+    @pytest.fixture(autouse=True)
+    def composed(self, monkeypatch):
+        monkeypatch.setenv("NPF_DISABLE_OPS", "grad_norm")
+
     @pytest.mark.parametrize("dtype", HALF)
     @pytest.mark.parametrize("p", [1.0, 2.0, math.inf])
-    def test_half(self, dtype, p):
+    def test_half(self, device, dtype, p):
         for max_norm in (0.5, 1e9, 0.0):
-            check_clip(params_of(SHAPES, dtype, "cpu"), max_norm, p)
-        params = params_of(SHAPES, dtype, "cpu")
+            check_clip(params_of(SHAPES, dtype, device), max_norm, p)
+        params = params_of(SHAPES, dtype, device)
         assert ops.grad_norm(params, p).dtype == torch.float32
 
-    def test_norm_over_the_types_largest(self):
+    def test_norm_over_the_types_largest(self, device):
         # finite gradients whose norm, about 1e5, no fp16 value holds
-        params = params_of([(1000000,)], torch.float16, "cpu", std=100.0)
+        params = params_of([(1000000,)], torch.float16, device, std=100.0)
         check_clip(params, 1.0, error_if_nonfinite=True)
         assert params[0].grad.any()
 
-    def test_squares_that_overflow_fp32(self):
-        check_clip(params_of([(50,)], torch.float32, "cpu", std=1e25), 1.0)
+    def test_squares_that_overflow_fp32(self, device):
+        check_clip(params_of([(50,)], torch.float32, device, std=1e25), 1.0)
 
-    def test_mixed(self):
+    def test_mixed(self, device):
         params = []
         for i, dtype in enumerate((torch.bfloat16, torch.float32, torch.float16)):
-            params += params_of([(n,) for n in range(1, 20)], dtype, "cpu", seed=i)
+            params += params_of([(n,) for n in range(1, 20)], dtype, device, seed=i)
         assert ops.grad_norm(params).dtype == torch.float32
         check_clip(params, 3.0)
-        wide = params_of([(7,)], torch.float64, "cpu")
+        wide = params_of([(7,)], torch.float64, device)
         old = wide[0].grad.clone()
         want = torch.linalg.vector_norm(torch.cat(
             [p.grad.double().reshape(-1) for p in params + wide]))
@@ -229,6 +234,21 @@ class TestFp16Ranges:
         lens = [0] * (B - 1) + [K - 7]
         check_attn(run_attn("cuda", a, scale=scale, lengths=lens),
                    scaled_oracle(a, scale, lengths=lens))
+
+    @pytest.mark.gpu
+    @pytest.mark.parametrize("sizes, last", [
+        ((1, 1, 1, 3, 70001, 4, 8), (12000.0, 700.0)),
+        ((1, 2, 1, 35000, 5, 4, 8), (300.0, 200.0)),
+    ])
+    def test_more_rows_than_chunks(self, sizes, last):
+        # (norms of rows are taken in chunks, from 65536 rows on of several steps)
+        a, scale = self.inputs(sizes, 0.5, 4.0)
+        without = largest_map_gradient(a, scale)[1]
+        # the largest at the very end, without which 2^e dS would be inf
+        a["values"][:, :, -1], a["dout"][:, :, -1] = last
+        most, _ = largest_map_gradient(a, scale)
+        assert most * 2.0 ** (14 - math.log2(without)) > 65504
+        check_attn(run_attn("cuda", a, scale=scale), scaled_oracle(a, scale))
 
     @pytest.mark.gpu
     @pytest.mark.parametrize("lam", [0.0, -40.0, 900.0])
