@@ -711,3 +711,37 @@ class TestNotFinite:
         assert got[0, 0, :, 3].isnan().all()
         rest = [i for i in range(sizes[6]) if i != 3]
         assert_within(got[..., rest], want[..., rest], bound[..., rest], "out")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_training_calls_repeat_and_replay(dtype):
+    """The same bits in every call, eager or replayed, with lengths and shared heads."""
+    a = {n: t.cuda() for n, t in attn_inputs(2, 4, 2, 140, 600, 16, 32, dtype).items()}
+    lens = torch.tensor([600, 411], dtype=torch.int32, device="cuda")
+
+    def call():
+        t = {n: x.detach().requires_grad_(n != "dout") for n, x in a.items()}
+        out = ops.differential_attention(
+            t["keys"], t["queries"], t["values"], t["lam"], key_lengths=lens)
+        names = ("keys", "queries", "values", "lam")
+        return (out.detach(), *torch.autograd.grad(out, [t[n] for n in names], t["dout"]))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        static = call()
+    for i in range(4):
+        for n, size in (("queries", 1.0), ("values", 10.0 ** i), ("dout", 30.0 ** (2 - i))):
+            a[n].normal_().mul_(size)
+        lens[1] = 411 - 200 * i if i < 3 else 0
+        first = call()
+        g.replay()
+        torch.cuda.synchronize()
+        for x, y, z in zip(static, first, call()):
+            assert torch.equal(x, y) and torch.equal(x, z)
+            assert torch.isfinite(x).all()
