@@ -27,9 +27,9 @@ struct Shape {
                                               : (kPad <= 16 ? 2 : 1);
   // What a wave's registers hold decides how the gradients share launches: of
   // the keys both at once, else dk and dv apart, else dk of each map apart; of
-  // the queries both maps at once, else apart.  (Long: dk and dv apart 988 us,
+  // the queries both maps at once, else apart.  (Long: dk and dv apart 959 us,
   // together 1260; heads of 128, 2 x 8 x 1024 x 1024, a whole step with dk of
-  // each map apart: bf16 313 us, together 517.)
+  // each map apart: bf16 308 us, together 517.)
   static constexpr bool kBothGrads = kPad * (int)sizeof(T) < 128;
   static constexpr bool kDkMapsApart = kPad == 128;
   static constexpr bool kDqMapsApart = kPad * (int)sizeof(T) > 256;
@@ -73,7 +73,8 @@ constexpr int kResident =
 
 // The same of the forward kernel, whose waves hold one map; rows on their way
 // through registers (not kDirect) need room too.  (Long: 430 us; waves with
-// both maps 475 with two a SIMD, 794 with one.)
+// both maps 475 with two a SIMD, 794 with one.  128 registers hold all but 9 at
+// 128 bytes a map, 2 at 64.)
 template <typename T, int kPad, bool kDirect>
 constexpr int kFwdResident =
     kPad * (int)sizeof(T) <= (kDirect ? 128 : 64) ? 4
@@ -111,22 +112,21 @@ __device__ __forceinline__ float exp_tile(f32x16& s, float c, float m,
 // bf16; "image": 16 x 4 heads, 1024 x 1024, maps of 16):
 //
 //            long bf16               image bf16   bound by
-//   forward  430 us, 0.64 PFLOP/s      35 us      vector and matrix unit: their
-//   dq       529 us                    42 us      times add up to the kernel's
-//   dk, dv   582 + 406 us              51 us      (forward 530 + 393 thousand
-//                                                 clocks a SIMD)
+//   forward  430 us, 0.64 PFLOP/s      34 us      vector and matrix unit (long:
+//   dq       525 us                    58 us      478 + 393 of 746 thousand
+//   dk, dv   569 + 390 us              51 us      clocks a SIMD, forward)
 // 8 heads of 128, 4096 x 4096, bf16: forward 203 us, 0.68 PFLOP/s.
 //
 // A pair of scores costs two exponents (8 clocks a 64-lane wave each) and about
-// 8 other vector operations a lane, and a wave's products and vector work
-// hardly overlap, however many waves a SIMD has.  LDS is read at less than half
-// of its rate, and without bank conflicts.
+// 8 other vector operations a lane, and little of a wave's products and vector
+// work overlaps, however many waves a SIMD has.  LDS is read at less than a
+// third of its rate (long), and but for 0.4% of dq's reads without bank conflicts.
 
 // Forward: a wave holds 32 query rows and one map, and passes over the keys; a
 // block has kRowWaves waves for each map, which share the tiles (the first
 // map's waves move the keys', the second's the values') and meet at the end.
 // With up to 32 rows a head, blocks of one wave a map split the keys between
-// them (single queries against 32768 keys, 200 MB of bf16: 58 us, 3.45 TB/s,
+// them (single queries against 32768 keys, 200 MB of bf16: 60 us, 3.35 TB/s,
 // with the join).
 template <typename T, int kPad, int kRowWaves, bool kDirect>
 __global__ void __launch_bounds__(128 * kRowWaves,
