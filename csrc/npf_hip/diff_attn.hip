@@ -155,11 +155,12 @@ __global__ void __launch_bounds__(256)
 // For gradients of keys and values alone, without the dq kernel that would
 // leave them: delta_i of each row, beside its lse: kLanes lanes of 4 values a row
 template <typename T, int kLanes>
-__global__ void __launch_bounds__(256) row_stats(NpfDiffAttnArgs a) {
+__global__ void __launch_bounds__(256)
+    row_stats(NpfDiffAttnArgs a, unsigned first) {
   // (rows are checked to fit 31 bits; divisions of 64 bits would cost more
   // than the sums)
   const unsigned rows = (unsigned)a.B * a.H * a.Q;
-  const unsigned r = blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
+  const unsigned r = first + blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
   if (r >= rows) return;  // whole groups of lanes
   const int q = (int)(r % (unsigned)a.Q), bh = (int)(r / (unsigned)a.Q);
   const int h = bh % a.H, b = bh / a.H;
@@ -316,10 +317,15 @@ hipError_t join_forward(const NpfDiffAttnArgs& a, hipStream_t stream) {
 template <typename T>
 void stats(const NpfDiffAttnArgs& a, hipStream_t stream) {
   if (a.dq.p || a.dlam) return;
-  with_lanes(a.Dv, [&](auto lanes) {
-    row_stats<T, lanes()>
-        <<<row_blocks((long)a.B * a.H * a.Q, lanes()), 256, 0, stream>>>(a);
-  });
+  // (a launch has fewer than 2^32 threads: of 2^25 rows 64 lanes at most)
+  const long rows = (long)a.B * a.H * a.Q;
+  for (long first = 0; first < rows; first += 1L << 25) {
+    const long some = rows - first < 1L << 25 ? rows - first : 1L << 25;
+    with_lanes(a.Dv, [&](auto lanes) {
+      row_stats<T, lanes()><<<row_blocks(some, lanes()), 256, 0, stream>>>(
+          a, (unsigned)first);
+    });
+  }
 }
 
 template <typename T>
@@ -410,8 +416,7 @@ bool npf_diff_attn_fits(const NpfDiffAttnArgs& a, bool backward) {
                         : fits(tiles * a.splits, 512);
   return fits(tiles * a.dq_splits, 256) &&
          fits(heads * ((a.K + 127) / 128) * a.dkv_splits, 256) &&
-         fits(heads * ((long)a.v_chunks + a.o_chunks), 256) &&
-         fits(heads * rows, 64);  // the sums of rows, of 64 lanes at most
+         fits(heads * ((long)a.v_chunks + a.o_chunks), 256);
 }
 
 long npf_diff_attn_workspace(const NpfDiffAttnArgs& a) {

@@ -141,7 +141,7 @@ __global__ void __launch_bounds__(128 * kRowWaves,
   // With few rows memory bounds the kernel, and the maps keep what rounding to
   // 16 bits leaves of them (single queries against 32768 keys: 57 to 60 us, and
   // the result's error falls from 1.48 to 1.0 times that of its last rounding).
-  // With many rows it would cost more than it gives: a step 117 -> 130 us
+  // With many rows it would cost more than it gives: a step 128 -> 141 us
   // (image), 1740 -> 2020 (long), padded fp16, 7 x 8 heads of 48, 333 x 2049, 53
   // -> 81; errors there are 1.4 to 1.5 times the last rounding's.
   constexpr bool kTwice = sizeof(T) == 2 && kRowWaves == 1;
@@ -395,7 +395,7 @@ __global__ void __launch_bounds__(64 * kBwdWaves, (kResident<T, kPad, kDirect>))
   // leaves of them.  Rows of them sum to zero, so what the keys of a row share
   // (scale q_i, more of it the fewer values a head has) cancels in dq but not in
   // the rounding: rounded once, dq's error is 1.53 times that of its own last
-  // rounding at heads of 16 (now 1.07; a step 130 us rather than 117, image) and
+  // rounding at heads of 16 (now 1.07; a step 128 us rather than 117, image) and
   // 1.44 times at heads of 64 (1.02; 1855 us rather than 1740, long).
   constexpr bool kTwice = sizeof(T) == 2 && kPad <= 32;
   constexpr int kTileBytes = kTile * S::kRowBytes;
@@ -625,8 +625,8 @@ __global__ void __launch_bounds__(64 * kBwdWaves, (kResident<T, kPad, kDirect>))
 // dk of the maps in kMaps (bits) and, with kDv, dv: a wave holds 32 keys and
 // passes over the queries of the heads that share them
 template <typename T, int kPad, bool kDirect, int kMaps, bool kDv>
-__global__ void __launch_bounds__(64 * kBwdWaves,
-                                  (kResident<T, kPad, kDirect, !kDv && kMaps != 3>))
+__global__ void __launch_bounds__(
+    64 * kBwdWaves, (kResident<T, kPad, kDirect, !kDv && kMaps != 3>))
     diff_bwd_dkv(NpfDiffAttnArgs a) {
   using S = Shape<T, kPad>;
   using Lds = Tile<T, S::kWidth>;

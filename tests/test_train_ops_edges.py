@@ -669,6 +669,27 @@ class TestMostHeads:
             assert dlam.item() == -2.0 * (2 ** 22 + 3)
 
 
+    @pytest.mark.gpu
+    def test_more_rows_than_a_launch_sums(self):
+        # 2^25 rows a launch of the rows' sums, where no gradient needs the
+        # kernel of dq: one key, whose map gives (1 - lam) dout to its value
+        n = 2 ** 25 + 100
+        k = torch.full((1, 1, 1, 2), 0.5, dtype=torch.bfloat16, device="cuda")
+        v = k.clone().requires_grad_(True)
+        q = k.expand(1, 1, n, 2)
+        lam = torch.tensor(0.25, device="cuda")
+        out = ops.differential_attention(k, q, v, lam)
+        dout = torch.zeros_like(out)
+        dout[0, 0, -1] = 3.0  # (of the second launch)
+        kg = k.clone().requires_grad_(True)
+        dv, = torch.autograd.grad(out, v, dout)
+        assert torch.equal(dv, torch.full_like(dv, 2.25))
+        out = ops.differential_attention(kg, q, v, lam)
+        dk, = torch.autograd.grad(out, kg, dout)
+        # the map's gradient is G - delta = 0
+        assert torch.equal(dk, torch.zeros_like(dk))
+
+
 class TestNotFinite:
     """Keys and values that count and are not finite."""
 
