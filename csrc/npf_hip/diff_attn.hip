@@ -204,7 +204,7 @@ __global__ void __launch_bounds__(256)
 // The largest norm of a chunk of rows of values, or of dout times the larger of
 // 1 and |lam|; keys that are not there, and rows without keys, do not count.
 // (A NaN is left out: it makes every gradient that its row meets NaN.)
-// Measured: 16 x 4 heads, 1024 x 1024, maps of 16: 6 us of a step of 125; 2 x 16
+// Measured: 16 x 4 heads, 1024 x 1024, maps of 16: 6 us of a step of 141; 2 x 16
 // heads on 4, 4096 x 4096, maps of 64: 22 us (48 MB) of 1835.
 template <typename T, int kLanes>
 __global__ void __launch_bounds__(256) row_reach(NpfDiffAttnArgs a) {

@@ -113,7 +113,7 @@ __device__ __forceinline__ float exp_tile(f32x16& s, float c, float m,
 //
 //            long bf16               image bf16   bound by
 //   forward  430 us, 0.64 PFLOP/s      34 us      vector and matrix unit (long:
-//   dq       525 us                    58 us      478 + 393 of 746 thousand
+//   dq       525 us                    53 us      478 + 393 of 746 thousand
 //   dk, dv   569 + 390 us              51 us      clocks a SIMD, forward)
 // 8 heads of 128, 4096 x 4096, bf16: forward 203 us, 0.68 PFLOP/s.
 //
@@ -126,7 +126,7 @@ __device__ __forceinline__ float exp_tile(f32x16& s, float c, float m,
 // block has kRowWaves waves for each map, which share the tiles (the first
 // map's waves move the keys', the second's the values') and meet at the end.
 // With up to 32 rows a head, blocks of one wave a map split the keys between
-// them (single queries against 32768 keys, 200 MB of bf16: 60 us, 3.35 TB/s,
+// them (single queries against 32768 keys, 200 MB of bf16: 59 us, 3.4 TB/s,
 // with the join).
 template <typename T, int kPad, int kRowWaves, bool kDirect>
 __global__ void __launch_bounds__(128 * kRowWaves,
@@ -139,7 +139,7 @@ __global__ void __launch_bounds__(128 * kRowWaves,
   // of a SIMD's registers (8 heads of 32, 4096^2, bf16: 93 us, with two 110)
   constexpr int kSubs = kPad <= 16 ? 2 : 1;
   // With few rows memory bounds the kernel, and the maps keep what rounding to
-  // 16 bits leaves of them (single queries against 32768 keys: 57 to 60 us, and
+  // 16 bits leaves of them (single queries against 32768 keys: 57 to 59 us, and
   // the result's error falls from 1.48 to 1.0 times that of its last rounding).
   // With many rows it would cost more than it gives: a step 128 -> 141 us
   // (image), 1740 -> 2020 (long), padded fp16, 7 x 8 heads of 48, 333 x 2049, 53
@@ -395,7 +395,7 @@ __global__ void __launch_bounds__(64 * kBwdWaves, (kResident<T, kPad, kDirect>))
   // leaves of them.  Rows of them sum to zero, so what the keys of a row share
   // (scale q_i, more of it the fewer values a head has) cancels in dq but not in
   // the rounding: rounded once, dq's error is 1.53 times that of its own last
-  // rounding at heads of 16 (now 1.07; a step 128 us rather than 117, image) and
+  // rounding at heads of 16 (now 1.07; a step 125 us rather than 117, image) and
   // 1.44 times at heads of 64 (1.02; 1855 us rather than 1740, long).
   constexpr bool kTwice = sizeof(T) == 2 && kPad <= 32;
   constexpr int kTileBytes = kTile * S::kRowBytes;

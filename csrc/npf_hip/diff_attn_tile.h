@@ -92,10 +92,21 @@ struct Operand {
   // what the rounding of x has left (exact in 32 bits), to be rounded in turn
   __device__ __forceinline__ f32x16 rest(f32x16 x) const {
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int t = 0; t < 2; ++t) {
+      const u32x4 pairs = __builtin_bit_cast(u32x4, v[t]);
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        x[8 * t + e] = __builtin_fmaf((float)v[t][e], -1.f, x[8 * t + e]);
+      for (int e = 0; e < 8; ++e) {
+        float y;
+        if constexpr (std::is_same<T, npf_bf16>::value) {
+          // (from the pair as it stands: else each value is rounded anew)
+          const unsigned u = pairs[e / 2];
+          y = __builtin_bit_cast(float, e & 1 ? u & 0xffff0000u : u << 16);
+        } else {
+          y = (float)v[t][e];
+        }
+        x[8 * t + e] -= y;
+      }
+    }
     return x;
   }
 };
