@@ -77,6 +77,19 @@ inline torch::Tensor npf_empty(at::IntArrayRef sizes, at::ScalarType type,
       at::detail::empty_cuda(sizes, type, on.device(), std::nullopt));
 }
 
+// What a forward pass saved may come back through the program's own hooks
+// (offloading, compression): it has to be what the kernels read.
+inline void npf_check_saved(const torch::Tensor& t, const torch::Tensor& like,
+                            at::ScalarType type, at::IntArrayRef sizes,
+                            const char* op) {
+  TORCH_CHECK_VALUE(t.defined() && t.device() == like.device() &&
+                        t.layout() == torch::kStrided &&
+                        t.scalar_type() == type && t.sizes() == sizes &&
+                        !t.is_neg() && !t._is_zerotensor(),
+                    op, ": a saved tensor came back changed");
+  npf_check_plain(t, op);
+}
+
 inline void npf_check(hipError_t e, const char* what) {
   TORCH_CHECK(e == hipSuccess, what, ": ", hipGetErrorString(e));
 }

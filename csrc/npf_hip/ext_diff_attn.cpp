@@ -159,10 +159,23 @@ struct DiffAttn : torch::autograd::Function<DiffAttn> {
                  &lengths = saved[4], &out = saved[5], &o2 = saved[6],
                  &lse = saved[7];
     npf_check_plain(grads[0], kName);
+    // (common_args looks at their sizes, types and strides)
+    for (const Tensor* t : {&k, &q, &v, &lam})
+      npf_check_saved(*t, grads[0], t->scalar_type(), t->sizes(), kName);
+    if (lengths.defined())
+      npf_check_saved(lengths, q, lengths.scalar_type(), lengths.sizes(), kName);
     c10::DeviceGuard guard(q.device());
     NpfDiffAttnArgs a = common_args(q, k, v, lam,
                                     ctx->saved_data["scale"].toDouble(),
                                     lengths);
+    const std::vector<int64_t> sizes = {a.B, a.H, a.Q, a.Dv};
+    for (const Tensor* t : {&out, &o2}) {
+      npf_check_saved(*t, q, q.scalar_type(), sizes, kName);
+      check_heads(*t, q, "the saved result");
+    }
+    npf_check_saved(lse, q, torch::kFloat32, {(long)a.B * a.H * a.Q * 2}, kName);
+    TORCH_CHECK_VALUE(grads[0].sizes() == sizes && lse.is_contiguous(), kName,
+                      ": a saved tensor came back changed");
     const Tensor dout = as_heads(grads[0]);
     check_heads(dout, q, "dout");
     Tensor dk, dq, dv, dlam;

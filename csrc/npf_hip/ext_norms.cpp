@@ -110,6 +110,24 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     const Tensor &x = saved[0], &residual = saved[1], &weight = saved[2],
                  &bias = saved[3], &stats = saved[4];
     npf_check_plain(grads[0], "layer_norm");
+    const Tensor& like = grads[0];
+    const int64_t D = like.size(-1), rows = like.numel() / D;
+    for (const Tensor* t : {&x, &residual})
+      if (t == &x || t->defined()) {
+        npf_check_saved(*t, like, like.scalar_type(), {rows, D}, "layer_norm");
+        TORCH_CHECK_VALUE(D == 1 || t->stride(1) == 1,
+                          "layer_norm: a saved tensor came back changed");
+      }
+    for (const Tensor* t : {&weight, &bias, &stats})
+      if (t == &stats || t->defined()) {
+        npf_check_saved(*t, like,
+                        t == &stats ? torch::kFloat32 : t->scalar_type(),
+                        t == &stats ? at::IntArrayRef{2, rows}
+                                    : at::IntArrayRef{D},
+                        "layer_norm");
+        TORCH_CHECK_VALUE(t->is_contiguous(),
+                          "layer_norm: a saved tensor came back changed");
+      }
     c10::DeviceGuard guard(x.device());
     NpfLayerNormArgs a = norm_args(x, residual, weight, bias);
     const Tensor dy = npf_signed(grads[0]).contiguous();

@@ -766,3 +766,65 @@ def test_training_calls_repeat_and_replay(dtype):
         for x, y, z in zip(static, first, call()):
             assert torch.equal(x, y) and torch.equal(x, z)
             assert torch.isfinite(x).all()
+
+
+class TestSavedTensors:
+    """Hooks of the program that take what a forward pass saves, and give it back."""
+
+    CALLS = ["norm", "attention"]
+
+    def call(self, which):
+        g = torch.Generator().manual_seed(3)
+        if which == "norm":
+            t = [torch.randn(s, generator=g).cuda().requires_grad_(True)
+                 for s in ((6, 24), (6, 24), (24,), (24,))]
+            return ops.layer_norm(t[0], t[2], t[3], residual=t[1]), t
+        a = attn_inputs(2, 2, 1, 5, 9, 4, 8, torch.float32)
+        t = [a[n].cuda().requires_grad_(True) for n in ("keys", "queries", "values", "lam")]
+        lens = torch.tensor([9, 4], device="cuda")
+        return ops.differential_attention(*t, key_lengths=lens), t
+
+    @pytest.mark.gpu
+    @pytest.mark.parametrize("which", CALLS)
+    def test_offloaded(self, which):
+        y, t = self.call(which)
+        want = torch.autograd.grad(y.square().sum(), t)
+        with torch.autograd.graph.save_on_cpu():
+            y, t = self.call(which)
+        for x, z in zip(torch.autograd.grad(y.square().sum(), t), want):
+            assert torch.equal(x, z)
+
+    @pytest.mark.gpu
+    @pytest.mark.parametrize("which", CALLS)
+    @pytest.mark.parametrize("change", [
+        lambda t: t.cpu(), lambda t: t.half() if t.is_floating_point() else t.short(),
+        lambda t: t[:0], lambda t: torch._neg_view(t) if t.is_floating_point() else t.cpu(),
+    ])
+    def test_changed(self, which, change):
+        # one saved tensor after the other comes back as it was not; none of
+        # that reaches a kernel
+        count = 0
+        for at in range(20):
+            seen = []
+
+            def pack(t):
+                seen.append(t)
+                return (len(seen) - 1, t)
+
+            def unpack(it):
+                return change(it[1]) if it[0] == at else it[1]
+
+            with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+                y, t = self.call(which)
+            if at >= len(seen):
+                break
+            try:
+                grads = torch.autograd.grad(y, t, torch.ones_like(y))
+            except (ValueError, TypeError, RuntimeError):
+                count += 1
+            else:
+                # (a weight or lam may be of another floating type)
+                assert seen[at].dim() == 1 and seen[at].is_floating_point()
+                assert change(seen[at]).dtype == torch.float16
+                assert all(torch.isfinite(x).all() for x in grads)
+        assert count >= 3
