@@ -313,12 +313,13 @@ Tensor grad_norm(const std::vector<Tensor>& params, double norm_type,
     npf_check(npf_grad_total(p, n, norm, t, type, stream), "grad_norm");
     return total;
   }
+  // (an inference tensor raises here, before any gradient changes)
+  for (const Tensor& g : grads) g.unsafeGetTensorImpl()->bump_version();
   for (const NpfGradSpans& s : all) {
     npf_check(npf_grad_scale(s, p, n, norm, max_norm, t, type, stream),
               "clip_grad_norm_");
     t = nullptr;
   }
-  for (const Tensor& g : grads) g.unsafeGetTensorImpl()->bump_version();
   return total;
 }
 

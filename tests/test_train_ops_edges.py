@@ -828,3 +828,14 @@ class TestSavedTensors:
                 assert change(seen[at]).dtype == torch.float16
                 assert all(torch.isfinite(x).all() for x in grads)
         assert count >= 3
+
+
+@pytest.mark.gpu
+def test_inference_gradients_stay():
+    p = torch.zeros(4, device="cuda", requires_grad=True)
+    with torch.inference_mode():
+        grad = torch.full((4,), 3.0, device="cuda")
+    p.grad = grad
+    with pytest.raises(RuntimeError, match="[Ii]nference"):
+        ops.clip_grad_norm_([p], 1.0)
+    assert torch.equal(grad.cpu(), torch.full((4,), 3.0))
