@@ -357,25 +357,29 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 // the parts' sums, in their order: 16 columns and 64 slices of the parts a
-// block, weight and bias in blocks of their own
+// block at a time, weight and bias in blocks of their own
 __global__ void __launch_bounds__(1024) ln_dw_join(NpfLayerNormArgs a) {
   __shared__ float smem[64][17];
   const int cl = threadIdx.x & 15, slice = threadIdx.x >> 4;
-  const int c = blockIdx.x * 16 + cl;
   void* out = blockIdx.y == 0 ? a.dweight : a.dbias;
   if (!out) return;
-  float s = 0.f;
-  if (c < a.width)
+  for (int c0 = blockIdx.x * 16; c0 < a.width; c0 += gridDim.x * 16) {
+    const int c = c0 + cl;
+    float s = 0.f;
+    if (c < a.width)
 #pragma unroll 4
-    for (int p = slice; p < a.parts; p += 64)
-      s += a.partial[(2L * p + blockIdx.y) * a.width + c];
-  smem[slice][cl] = s;
-  __syncthreads();
-  if (slice > 0 || c >= a.width) return;
-  s = 0.f;
+      for (int p = slice; p < a.parts; p += 64)
+        s += a.partial[(2L * p + blockIdx.y) * a.width + c];
+    smem[slice][cl] = s;
+    __syncthreads();
+    if (slice == 0 && c < a.width) {
+      s = 0.f;
 #pragma unroll
-  for (int i = 0; i < 64; ++i) s += smem[i][cl];
-  store_coded(out, a.weight_type, c, s);
+      for (int i = 0; i < 64; ++i) s += smem[i][cl];
+      store_coded(out, a.weight_type, c, s);
+    }
+    __syncthreads();
+  }
 }
 
 // -------------------------------- dispatch -------------------------------- //
@@ -433,6 +437,7 @@ void with_layout(Layout l, F f) {
 // 137, 170 us.
 constexpr long kBlocks = 1024;
 constexpr int kLoopParts = 128;
+constexpr int kJoinColumns = 1 << 24;  // of a launch of ln_dw_join
 
 template <typename T, typename W>
 void fwd_rows(const NpfLayerNormArgs& a, Layout l, hipStream_t stream) {
@@ -489,8 +494,11 @@ hipError_t launch_bwd(const NpfLayerNormArgs& a, int type,
       ln_dw_part<T><<<dim3((a.width + kThreads - 1) / kThreads, a.parts),
                       kThreads, 0, stream>>>(a);
   }
-  if (a.partial)
-    ln_dw_join<<<dim3((a.width + 15) / 16, 2), 1024, 0, stream>>>(a);
+  if (a.partial) {
+    // (a launch has fewer than 2^32 threads: the widest rows take turns)
+    const unsigned n = a.width >= kJoinColumns ? kJoinColumns : a.width;
+    ln_dw_join<<<dim3((n + 15) / 16, 2), 1024, 0, stream>>>(a);
+  }
   return hipGetLastError();
 }
 

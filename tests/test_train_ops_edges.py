@@ -839,3 +839,21 @@ def test_inference_gradients_stay():
     with pytest.raises(RuntimeError, match="[Ii]nference"):
         ops.clip_grad_norm_([p], 1.0)
     assert torch.equal(grad.cpu(), torch.full((4,), 3.0))
+
+
+@pytest.mark.gpu
+def test_norm_of_the_widest_rows():
+    # more columns than a launch's threads hold at 64 a column
+    width = 2 ** 26 + 37
+    x = torch.randn(1, width, device="cuda")
+    w = torch.ones(width, device="cuda", requires_grad=True)
+    b = torch.zeros(width, device="cuda", requires_grad=True)
+    y = ops.layer_norm(x, w, b)
+    dw, db = torch.autograd.grad(y, (w, b), torch.full_like(y, 2.0))
+    # one row: the sums have one term each, and 2 h is exact
+    assert torch.equal(dw, 2.0 * y[0].detach())
+    assert torch.equal(db, torch.full_like(db, 2.0))
+    var, mean = torch.var_mean(x.double(), correction=0)
+    h = (x.double() - mean) * torch.rsqrt(var + 1e-5)
+    # sums of 2^26 terms, 2^18 a thread one after the other
+    assert (y - h).abs().max() <= 2 ** 18 * E32 * (1 + h.abs().max())
