@@ -261,24 +261,29 @@ __global__ void __launch_bounds__(256) row_reach(NpfDiffAttnArgs a) {
         fmaxf(fmaxf(smem[0], smem[1]), fmaxf(smem[2], smem[3]));
 }
 
-// dlam of one head (of all heads where lam is one number)
+// dlam of one head after the other (of all heads where lam is one number)
+constexpr int kDlamBlocks = 1 << 20;
+
 __global__ void __launch_bounds__(1024) sum_dlam(NpfDiffAttnArgs a,
                                                  int heads) {
   __shared__ double smem[1024];
-  double s = 0.;
   // (sizes are checked to fit 31 bits)
   const unsigned per = (unsigned)heads * a.Q;
   const unsigned all = (unsigned)a.dq_splits * a.B * per;
+  for (int h = blockIdx.x; h < a.lam_heads; h += gridDim.x) {
+    double s = 0.;
 #pragma unroll 4
-  for (unsigned i = threadIdx.x; i < all; i += 1024)
-    s += a.dlam_rows[(long)(i / per * a.H + blockIdx.x * heads) * a.Q + i % per];
-  smem[threadIdx.x] = s;
-  __syncthreads();
-  for (int n = 512; n > 0; n >>= 1) {
-    if (threadIdx.x < n) smem[threadIdx.x] += smem[threadIdx.x + n];
+    for (unsigned i = threadIdx.x; i < all; i += 1024)
+      s += a.dlam_rows[(long)(i / per * a.H + h * heads) * a.Q + i % per];
+    smem[threadIdx.x] = s;
+    __syncthreads();
+    for (int n = 512; n > 0; n >>= 1) {
+      if (threadIdx.x < n) smem[threadIdx.x] += smem[threadIdx.x + n];
+      __syncthreads();
+    }
+    if (threadIdx.x == 0) store_coded(a.dlam, a.lam_type, h, -smem[0]);
     __syncthreads();
   }
-  if (threadIdx.x == 0) store_coded(a.dlam, a.lam_type, blockIdx.x, -smem[0]);
 }
 
 // lanes of 4 values for a row of `size`, as a compile-time number
@@ -465,6 +470,8 @@ hipError_t npf_diff_attn_bwd(const NpfDiffAttnArgs& a, hipStream_t stream) {
       break;
   }
   if (e != hipSuccess || !a.dlam) return e;
-  sum_dlam<<<a.lam_heads, 1024, 0, stream>>>(a, a.H / a.lam_heads);
+  // (a launch has fewer than 2^32 threads)
+  const int blocks = a.lam_heads <= kDlamBlocks ? a.lam_heads : kDlamBlocks;
+  sum_dlam<<<blocks, 1024, 0, stream>>>(a, a.H / a.lam_heads);
   return hipGetLastError();
 }

@@ -670,6 +670,20 @@ class TestMostHeads:
 
 
     @pytest.mark.gpu
+    def test_one_weight_each(self):
+        # (1024 threads sum a head's part of the gradient: 2^22 heads a launch)
+        n = 2 ** 22 + 5
+        k, q = self.heads(n, 1)
+        lam = torch.full((n,), 0.25, device="cuda", requires_grad=True)
+        out = ops.differential_attention(k, q, k, lam)
+        dout = torch.ones_like(out)
+        dout[0, -1] = 3.0
+        (dlam,) = torch.autograd.grad(out, lam, dout)
+        want = torch.full((n,), -1.0, device="cuda")
+        want[-1] = -3.0
+        assert torch.equal(dlam, want)
+
+    @pytest.mark.gpu
     def test_more_rows_than_a_launch_sums(self):
         # 2^25 rows a launch of the rows' sums, where no gradient needs the
         # kernel of dq: one key, whose map gives (1 - lam) dout to its value
