@@ -11,6 +11,7 @@ import pytest
 import torch
 
 from npf import ops
+from npf.architectures import get_attender
 from test_train_ops import (E32, SHAPES, assert_within, attn_inputs, attn_oracle,
                             check_attn, check_clip, lowest_step, norm_inputs,
                             params_of, run_attn, run_norm)
@@ -807,6 +808,28 @@ class TestSavedTensors:
             y, t = self.call(which)
         for x, z in zip(torch.autograd.grad(y.square().sum(), t), want):
             assert torch.equal(x, z)
+
+    @pytest.mark.gpu
+    @pytest.mark.parametrize("name", ["differential", "differential_transformer"])
+    @pytest.mark.parametrize("reentrant", [False, True])
+    def test_recomputed(self, name, reentrant):
+        from torch.utils.checkpoint import checkpoint
+
+        torch.manual_seed(0)
+        att = get_attender(name, 32, 32, 32, n_heads=4).cuda()
+        x = torch.randn(2, 9, 32, device="cuda", requires_grad=True)
+        leaves = [x, *att.parameters()]
+
+        def grads(out):
+            for t in leaves:
+                t.grad = None
+            out.square().sum().backward()
+            return [t.grad.clone() for t in leaves]
+
+        want = grads(att(x, x, x))
+        got = grads(checkpoint(lambda t: att(t, t, t), x, use_reentrant=reentrant))
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
 
     @pytest.mark.gpu
     @pytest.mark.parametrize("which", CALLS)
